@@ -619,6 +619,150 @@ int32_t scemb_compute_row_pointers_size_per_device(int32_t global_device_count,
                                                    int32_t num_sc_per_device,
                                                    int32_t enable_minibatching);
 
+/* ---- Dense operators (no counterpart in the reference) -------------------
+ * What a ranking model runs beside its tables: layer norm, the ordering of
+ * tokens by expert, and AdamW over its dense weights. Element types: */
+#define SCEMB_F32 0
+#define SCEMB_BF16 1
+#define SCEMB_F16 2
+
+/* Layer norm over the last dimension. For each of `rows` rows of `dim`
+ * values (x_stride values apart):
+ *   mean = sum(x) / dim,  rstd = 1 / sqrt(sum((x - mean)^2) / dim + epsilon),
+ *   y = (x - mean) * rstd * weight + bias,
+ * in float32, rounded once to x's type. weight and bias ([dim], both of
+ * weight_type: float32 or x's type) may be NULL (one, zero). mean and rstd
+ * ([rows] float32, what the gradient reads) may be NULL. y is [rows, dim]
+ * contiguous. */
+int scemb_layer_norm(const void* x, int32_t type, int64_t rows, int64_t dim,
+                     int64_t x_stride, const void* weight, const void* bias,
+                     int32_t weight_type, float epsilon, void* y, float* mean,
+                     float* rstd, void* stream);
+
+/* Its gradients. With xhat = (x - mean) * rstd and h = y_grad * weight:
+ *   x_grad = rstd * (h - sum(h) / dim - xhat * sum(h * xhat) / dim),
+ *   weight_grad = sum over rows of y_grad * xhat,
+ *   bias_grad = sum over rows of y_grad.
+ * x_grad is [rows, dim] contiguous and of x's type, as is y_grad;
+ * weight_grad and bias_grad (each may be NULL) are of weight_type. The sums
+ * over rows are taken in an order that rows, dim and the type decide:
+ * repeated calls give the same bits. */
+size_t scemb_layer_norm_grad_workspace_size(int32_t type, int64_t rows,
+                                            int64_t dim);
+int scemb_layer_norm_grad(const void* y_grad, int64_t y_grad_stride,
+                          const void* x, int64_t x_stride, int32_t type,
+                          int64_t rows, int64_t dim, const float* mean,
+                          const float* rstd, const void* weight,
+                          int32_t weight_type, void* x_grad,
+                          void* weight_grad, void* bias_grad, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Orders `n` choices of experts by expert, choices of one expert in their
+ * own order. ids (id_bytes 4: int32, 8: int64) outside [0, num_experts) are
+ * dropped choices and go to the end. positions[i] is choice i's place,
+ * sources[p] the choice at place p, offsets[e] the first place of expert e
+ * (offsets[num_experts]: the number of choices that are not dropped). */
+#define SCEMB_MAX_EXPERTS 1024
+size_t scemb_sort_by_expert_workspace_size(int64_t n, int32_t num_experts);
+int scemb_sort_by_expert(const void* ids, int32_t id_bytes, int64_t n,
+                         int32_t num_experts, int32_t* positions,
+                         int32_t* sources, int32_t* offsets, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Such an order of tokens * choices choices, choice t * choices + k being
+ * token t's k-th. A position outside [0, tokens * choices) counts as
+ * dropped. */
+typedef struct scemb_expert_order {
+  const int32_t* positions; /* [tokens * choices] */
+  const int32_t* offsets;   /* [num_experts + 1] */
+  int64_t tokens;
+  int32_t choices;
+  int32_t num_experts;
+} scemb_expert_order_t;
+
+/* rows[positions[t, k]] = x[t], zero for dropped choices: every row of
+ * `rows` ([tokens * choices, dim] contiguous) is written. */
+int scemb_tokens_to_experts(const void* x, int32_t type, int64_t x_stride,
+                            int64_t dim, const scemb_expert_order_t* order,
+                            void* rows, void* stream);
+
+/* y[t] = sum over k of weights[t, k] * rows[positions[t, k]], in float32,
+ * rounded once; dropped choices are not read and add nothing. weights
+ * ([tokens, choices] contiguous, float32 or rows' type) NULL: one. With that
+ * it is the gradient of scemb_tokens_to_experts. */
+int scemb_tokens_from_experts(const void* rows, int32_t type,
+                              int64_t rows_stride, int64_t dim,
+                              const void* weights, int32_t weights_type,
+                              const scemb_expert_order_t* order, void* y,
+                              void* stream);
+
+/* Its gradients: rows_grad[positions[t, k]] = weights[t, k] * y_grad[t]
+ * (every row written, zero for dropped choices) and weights_grad[t, k] =
+ * the inner product of y_grad[t] and rows[positions[t, k]] (zero for dropped
+ * choices). */
+int scemb_tokens_from_experts_grad(
+    const void* y_grad, int64_t y_grad_stride, const void* rows, int32_t type,
+    int64_t rows_stride, int64_t dim, const void* weights,
+    int32_t weights_type, const scemb_expert_order_t* order, void* rows_grad,
+    void* weights_grad, void* stream);
+
+/* AdamW over many tensors. Tensor i's moments are the values from
+ * first_i = sum over j < i of numel_j rounded up to SCEMB_ADAMW_BLOCK on.
+ * With g = grad * grad_scale and t the step (from 1):
+ *   m = beta_1 * m + (1 - beta_1) * g,  v = beta_2 * v + (1 - beta_2) * g^2,
+ *   p = p * (1 - learning_rate * weight_decay)
+ *       - learning_rate / (1 - beta_1^t)
+ *         * m / (sqrt(v) / sqrt(1 - beta_2^t) + epsilon),
+ * in float32; p is rounded to its type, and also written to `copy` in
+ * bfloat16 where that is given. Parameters are float32 or bfloat16, gradients
+ * too. A NULL grad leaves the tensor and its moments as they are.
+ *
+ * Moments of 8 bits are kept in blocks of SCEMB_ADAMW_BLOCK values, each with
+ * two float32 scales: m = m_scale * (q / 127) * |q / 127| with q signed, and
+ * sqrt(v) = v_scale * (q / 255)^2 with q unsigned. The scales are the block's
+ * largest |m| and sqrt(v); q is rounded to nearest, except that only v = 0
+ * gets q = 0: a small second moment never turns into a division by epsilon.
+ * A gradient that is not finite makes its block's scales so. */
+#define SCEMB_ADAMW_BLOCK 256
+typedef struct scemb_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* copy;
+  int64_t numel;
+  int32_t param_type;
+  int32_t grad_type;
+  int32_t decay;    /* whether weight_decay applies */
+  int32_t reserved;
+} scemb_adamw_tensor_t;
+typedef struct scemb_adamw_state {
+  void* m;        /* [size] float32 or int8 */
+  void* v;        /* [size] float32 or uint8 */
+  float* m_scale; /* [size / SCEMB_ADAMW_BLOCK] with 8 bits */
+  float* v_scale;
+  int64_t size;   /* a multiple of SCEMB_ADAMW_BLOCK */
+  int32_t bits;   /* 8 or 32 */
+  int32_t reserved;
+} scemb_adamw_state_t;
+typedef struct scemb_adamw_options {
+  double learning_rate;
+  double beta_1;
+  double beta_2;
+  double epsilon;
+  double weight_decay;
+  double grad_scale;
+  int64_t step;
+  /* Device scalars that take the place of the values above (NULL: none). */
+  const float* learning_rate_ptr;
+  const int64_t* step_ptr;
+  const float* grad_scale_ptr;
+} scemb_adamw_options_t;
+int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
+                       int32_t num_tensors, const scemb_adamw_state_t* state,
+                       const scemb_adamw_options_t* options, void* stream);
+/* Moments of 8 bits as float32 ([size] each). */
+int scemb_adamw_moments(const scemb_adamw_state_t* state, float* m, float* v,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,443 @@
+// AdamW over many tensors at once, with moments in float32 or in 8 bits.
+//
+// One launch takes up to kMaxTensors tensors, whose addresses travel in the
+// kernel arguments; a work-group has kChunk consecutive values of one of them.
+// The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
+// bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy.
+//
+// Moments of 8 bits are decoded, moved, used and encoded in registers. A block
+// of 256 values is the four values of each lane of a wavefront, so its scale
+// is a maximum over lanes. Products and sums are rounded one by one (the file
+// is compiled without contraction) and the roots and quotients behind a code
+// are correctly rounded, so a code is a function of its block alone, whatever
+// kernel computes it.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "dense.h"
+
+namespace scemb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPer = 4;                    // consecutive values of a lane
+constexpr int kStep = kThreads * kPer;     // values of a work-group at a time
+constexpr int kChunk = 4 * kStep;          // values of a work-group
+constexpr int kQuant = SCEMB_ADAMW_BLOCK;  // values that share a scale
+constexpr int kMaxTensors = 64;            // a launch: a tensor a lane
+static_assert(kQuant == kWave * kPer, "a block is one step of a wavefront");
+
+struct Tensor {
+  void* param;
+  const void* grad;
+  void* copy;
+  int64_t numel;
+  uint32_t block;  // its first block of moments
+  uint8_t param_bf16;
+  uint8_t grad_bf16;
+  uint8_t decay;
+  uint8_t aligned;  // four values can be loaded and stored at once
+};
+
+struct Moments {
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+};
+
+// What a step multiplies with, in float32.
+struct Factors {
+  float grad_scale;
+  float beta_1;
+  float gain_1;  // 1 - beta_1
+  float beta_2;
+  float gain_2;  // 1 - beta_2
+  float rate;    // learning_rate / (1 - beta_1^t)
+  float root;    // 1 / sqrt(1 - beta_2^t)
+  float epsilon;
+  float keep;    // 1 - learning_rate * weight_decay
+};
+
+struct AdamArgs {
+  uint32_t first[kMaxTensors];  // first work-group of each tensor
+  Tensor tensors[kMaxTensors];
+  Moments moments;
+  Factors factors;
+  // Device scalars and what the factors are then made of.
+  const float* learning_rate_ptr;
+  const int64_t* step_ptr;
+  const float* grad_scale_ptr;
+  double learning_rate;
+  double beta_1;
+  double beta_2;
+  double weight_decay;
+  int64_t step;
+  int32_t n;
+};
+static_assert(sizeof(AdamArgs) <= 3584,
+              "the arguments must fit the kernel argument block");
+
+__host__ __device__ inline void SetRates(double learning_rate, double beta_1,
+                                         double beta_2, double weight_decay,
+                                         int64_t step, Factors* f) {
+  const double t = static_cast<double>(step);
+  f->rate = static_cast<float>(learning_rate / (1.0 - pow(beta_1, t)));
+  f->root = static_cast<float>(1.0 / sqrt(1.0 - pow(beta_2, t)));
+  f->keep = static_cast<float>(1.0 - learning_rate * weight_decay);
+}
+
+template <typename T>
+__device__ __forceinline__ void Load4(const T* p, int64_t at, int count,
+                                      bool whole, float (&x)[kPer]) {
+  if (whole) {
+    const auto v = LoadVec<T, kPer>(p + at);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = static_cast<float>(v.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      x[j] = j < count ? static_cast<float>(p[at + j]) : 0.f;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void Store4(T* p, int64_t at, int count, bool whole,
+                                       const float (&x)[kPer]) {
+  if (whole) {
+    Vec<T, kPer> v;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v.v[j] = static_cast<T>(x[j]);
+    StoreVec<T, kPer>(p + at, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (j < count) p[at + j] = static_cast<T>(x[j]);
+    }
+  }
+}
+
+__device__ __forceinline__ float DecodeM(int8_t q, float scale) {
+  const float x = static_cast<float>(q) * (1.f / 127.f);
+  return x * fabsf(x) * scale;
+}
+__device__ __forceinline__ float DecodeR(uint8_t q, float scale) {
+  const float x = static_cast<float>(q) * (1.f / 255.f);
+  return x * x * scale;
+}
+
+// Rounded to nearest, ties to even. A scale of zero has only zeros below it.
+__device__ __forceinline__ int8_t EncodeM(float m, float scale) {
+  const float q = fminf(
+      rintf(sqrtf(fabsf(m) / (scale > 0.f ? scale : 1.f)) * 127.f), 127.f);
+  return static_cast<int8_t>(m < 0.f ? -q : q);
+}
+__device__ __forceinline__ uint8_t EncodeR(float r, float scale) {
+  const float q =
+      fminf(rintf(sqrtf(r / (scale > 0.f ? scale : 1.f)) * 255.f), 255.f);
+  return static_cast<uint8_t>(r > 0.f && q < 1.f ? 1.f : q);
+}
+
+// One chunk of one tensor: values [begin, begin + kChunk) of it.
+template <int kBits, typename P, typename G>
+__device__ __forceinline__ void UpdateChunk(const Tensor& t, const Moments& s,
+                                            const Factors& f, int64_t begin) {
+  P* param = static_cast<P*>(t.param);
+  const G* grad = static_cast<const G*>(t.grad);
+  bf16* copy = static_cast<bf16*>(t.copy);
+  const float keep = t.decay ? f.keep : 1.f;
+  const int64_t arena = static_cast<int64_t>(t.block) * kQuant;
+  for (int64_t base = begin; base < begin + kChunk; base += kStep) {
+    const int64_t at = base + threadIdx.x * kPer;
+    // The wavefront's 256 values: all of its lanes go on, or none.
+    if (at - (threadIdx.x % kWave) * kPer >= t.numel) break;
+    const int64_t left = t.numel - at;
+    const int count = left < 0 ? 0 : left < kPer ? static_cast<int>(left)
+                                                 : kPer;
+    const bool whole = count == kPer && t.aligned;
+    const int64_t slot = arena + at;
+    float p[kPer], g[kPer], m[kPer], v[kPer], r[kPer];
+    Load4<P>(param, at, count, whole, p);
+    Load4<G>(grad, at, count, whole, g);
+    if constexpr (kBits == 8) {
+      const auto qm =
+          LoadVec<int8_t, kPer>(static_cast<const int8_t*>(s.m) + slot);
+      const auto qv =
+          LoadVec<uint8_t, kPer>(static_cast<const uint8_t*>(s.v) + slot);
+      const float ms = s.m_scale[slot / kQuant];
+      const float vs = s.v_scale[slot / kQuant];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        m[j] = DecodeM(qm.v[j], ms);
+        const float root = DecodeR(qv.v[j], vs);
+        v[j] = root * root;
+      }
+    } else {
+      const auto vm =
+          LoadVec<float, kPer>(static_cast<const float*>(s.m) + slot);
+      const auto vv =
+          LoadVec<float, kPer>(static_cast<const float*>(s.v) + slot);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        m[j] = vm.v[j];
+        v[j] = vv.v[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float x = g[j] * f.grad_scale;
+      m[j] = m[j] * f.beta_1 + x * f.gain_1;
+      v[j] = v[j] * f.beta_2 + x * x * f.gain_2;
+      r[j] = sqrtf(v[j]);
+      p[j] = p[j] * keep - m[j] / (r[j] * f.root + f.epsilon) * f.rate;
+    }
+    Store4<P>(param, at, count, whole, p);
+    if (copy != nullptr) Store4<bf16>(copy, at, count, whole, p);
+    if constexpr (kBits == 8) {
+      // Past the tensor's end the codes decode to zero and so do these; the
+      // moments there are written back as they were.
+      float ms = 0.f, vs = 0.f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (j >= count) m[j] = r[j] = 0.f;
+        ms = LaneMaxBits::Of(ms, fabsf(m[j]));
+        vs = LaneMaxBits::Of(vs, r[j]);
+      }
+      ms = LaneReduce<LaneMaxBits, kWave>(ms);
+      vs = LaneReduce<LaneMaxBits, kWave>(vs);
+      Vec<int8_t, kPer> qm;
+      Vec<uint8_t, kPer> qv;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        qm.v[j] = EncodeM(m[j], ms);
+        qv.v[j] = EncodeR(r[j], vs);
+      }
+      StoreVec<int8_t, kPer>(static_cast<int8_t*>(s.m) + slot, qm);
+      StoreVec<uint8_t, kPer>(static_cast<uint8_t*>(s.v) + slot, qv);
+      if (threadIdx.x % kWave == 0) {
+        s.m_scale[slot / kQuant] = ms;
+        s.v_scale[slot / kQuant] = vs;
+      }
+    } else {
+      // Slots past the tensor's end belong to no value: their gradient was
+      // read as zero, so zeros stay zeros.
+      Vec<float, kPer> vm, vv;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        vm.v[j] = m[j];
+        vv.v[j] = v[j];
+      }
+      StoreVec<float, kPer>(static_cast<float*>(s.m) + slot, vm);
+      StoreVec<float, kPer>(static_cast<float*>(s.v) + slot, vv);
+    }
+  }
+}
+
+template <int kBits>
+__global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs a) {
+  const int lane = threadIdx.x % kWave;
+  const uint64_t before =
+      __ballot(lane < a.n && a.first[lane] <= blockIdx.x);
+  const int i = __builtin_amdgcn_readfirstlane(__popcll(before) - 1);
+  const Tensor t = a.tensors[i];
+  Factors f = a.factors;
+  if (a.learning_rate_ptr != nullptr || a.step_ptr != nullptr) {
+    SetRates(a.learning_rate_ptr != nullptr
+                 ? static_cast<double>(*a.learning_rate_ptr)
+                 : a.learning_rate,
+             a.beta_1, a.beta_2, a.weight_decay,
+             a.step_ptr != nullptr ? *a.step_ptr : a.step, &f);
+  }
+  if (a.grad_scale_ptr != nullptr) f.grad_scale = *a.grad_scale_ptr;
+  const int64_t begin =
+      static_cast<int64_t>(blockIdx.x - a.first[i]) * kChunk;
+  if (t.param_bf16) {
+    if (t.grad_bf16) {
+      UpdateChunk<kBits, bf16, bf16>(t, a.moments, f, begin);
+    } else {
+      UpdateChunk<kBits, bf16, float>(t, a.moments, f, begin);
+    }
+  } else if (t.grad_bf16) {
+    UpdateChunk<kBits, float, bf16>(t, a.moments, f, begin);
+  } else {
+    UpdateChunk<kBits, float, float>(t, a.moments, f, begin);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void DecodeMoments(
+    const int8_t* qm, const uint8_t* qv, const float* m_scale,
+    const float* v_scale, int64_t size, float* m, float* v) {
+  const int64_t at =
+      (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kPer;
+  if (at >= size) return;
+  const auto cm = LoadVec<int8_t, kPer>(qm + at);
+  const auto cv = LoadVec<uint8_t, kPer>(qv + at);
+  const float ms = m_scale[at / kQuant];
+  const float vs = v_scale[at / kQuant];
+  Vec<float, kPer> om, ov;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    om.v[j] = DecodeM(cm.v[j], ms);
+    const float root = DecodeR(cv.v[j], vs);
+    ov.v[j] = root * root;
+  }
+  StoreVec<float, kPer>(m + at, om);
+  StoreVec<float, kPer>(v + at, ov);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+
+int CheckState(const scemb_adamw_state_t* s) {
+  if (s == nullptr || (s->bits != 8 && s->bits != 32) || s->size < 0 ||
+      s->size % kQuant != 0 || s->size / kQuant > 0xffffffffll) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: state missing, bits not 8 or 32, or a size that is "
+                "no multiple of the block");
+  }
+  if (s->size > 0 &&
+      (s->m == nullptr || s->v == nullptr || !AlignedTo(s->m, 16) ||
+       !AlignedTo(s->v, 16) ||
+       (s->bits == 8 && (s->m_scale == nullptr || s->v_scale == nullptr)))) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: moments or scales missing, or moments not aligned to "
+                "16 bytes");
+  }
+  return 0;
+}
+
+int CheckTensor(const scemb_adamw_tensor_t& t, int32_t i) {
+  const bool types = (t.param_type == SCEMB_F32 || t.param_type == SCEMB_BF16) &&
+                     (t.grad_type == SCEMB_F32 || t.grad_type == SCEMB_BF16);
+  if (t.numel < 0 || (t.numel > 0 && t.grad != nullptr &&
+                      (!types || t.param == nullptr))) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: tensor " + std::to_string(i) +
+                    ": parameter missing, a negative size, or a type other "
+                    "than float32 and bfloat16");
+  }
+  return 0;
+}
+
+int LaunchUpdate(const AdamArgs& a, uint32_t groups, int bits,
+                 hipStream_t stream) {
+  if (bits == 8) {
+    hipLaunchKernelGGL(AdamUpdate<8>, dim3(groups), dim3(kThreads), 0, stream,
+                       a);
+  } else {
+    hipLaunchKernelGGL(AdamUpdate<32>, dim3(groups), dim3(kThreads), 0, stream,
+                       a);
+  }
+  SCEMB_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+}  // namespace scemb
+
+extern "C" {
+
+int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
+                       int32_t num_tensors, const scemb_adamw_state_t* state,
+                       const scemb_adamw_options_t* options, void* stream) {
+  using namespace scemb;
+  const int bad = CheckState(state);
+  if (bad != 0) return bad;
+  if (num_tensors < 0 || (num_tensors > 0 && tensors == nullptr) ||
+      options == nullptr ||
+      (options->step_ptr == nullptr && options->step < 1)) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: tensors or options missing, or a step below 1");
+  }
+  int64_t blocks = 0;
+  for (int32_t i = 0; i < num_tensors; ++i) {
+    const int rc = CheckTensor(tensors[i], i);
+    if (rc != 0) return rc;
+    blocks += CeilDiv(tensors[i].numel, kQuant);
+  }
+  if (blocks * kQuant > state->size) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: the state is smaller than the tensors");
+  }
+  AdamArgs a;
+  a.moments = {state->m, state->v, state->m_scale, state->v_scale};
+  a.factors.grad_scale = static_cast<float>(options->grad_scale);
+  a.factors.beta_1 = static_cast<float>(options->beta_1);
+  a.factors.gain_1 = static_cast<float>(1.0 - options->beta_1);
+  a.factors.beta_2 = static_cast<float>(options->beta_2);
+  a.factors.gain_2 = static_cast<float>(1.0 - options->beta_2);
+  a.factors.epsilon = static_cast<float>(options->epsilon);
+  SetRates(options->learning_rate, options->beta_1, options->beta_2,
+           options->weight_decay, options->step, &a.factors);
+  a.learning_rate_ptr = options->learning_rate_ptr;
+  a.step_ptr = options->step_ptr;
+  a.grad_scale_ptr = options->grad_scale_ptr;
+  a.learning_rate = options->learning_rate;
+  a.beta_1 = options->beta_1;
+  a.beta_2 = options->beta_2;
+  a.weight_decay = options->weight_decay;
+  a.step = options->step;
+  a.n = 0;
+  uint32_t block = 0;
+  int64_t groups = 0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for (int32_t i = 0; i < num_tensors; ++i) {
+    const scemb_adamw_tensor_t& t = tensors[i];
+    if (t.grad != nullptr && t.numel > 0) {
+      const int64_t mine = CeilDiv(t.numel, kChunk);
+      if (a.n == kMaxTensors || groups + mine > 0x7fffffff) {
+        const int rc = LaunchUpdate(a, static_cast<uint32_t>(groups),
+                                    state->bits, s);
+        if (rc != 0) return rc;
+        a.n = 0;
+        groups = 0;
+      }
+      Tensor& d = a.tensors[a.n];
+      a.first[a.n] = static_cast<uint32_t>(groups);
+      d.param = t.param;
+      d.grad = t.grad;
+      d.copy = t.copy;
+      d.numel = t.numel;
+      d.block = block;
+      d.param_bf16 = t.param_type == SCEMB_BF16;
+      d.grad_bf16 = t.grad_type == SCEMB_BF16;
+      d.decay = t.decay != 0;
+      d.aligned = AlignedTo(t.param, d.param_bf16 ? 8 : 16) &&
+                  AlignedTo(t.grad, d.grad_bf16 ? 8 : 16) &&
+                  AlignedTo(t.copy, 8);
+      ++a.n;
+      groups += mine;
+    }
+    block += static_cast<uint32_t>(CeilDiv(t.numel, kQuant));
+  }
+  if (a.n == 0) return SCEMB_OK;
+  return LaunchUpdate(a, static_cast<uint32_t>(groups), state->bits, s);
+}
+
+int scemb_adamw_moments(const scemb_adamw_state_t* state, float* m, float* v,
+                        void* stream) {
+  using namespace scemb;
+  const int bad = CheckState(state);
+  if (bad != 0) return bad;
+  if (state->size == 0) return SCEMB_OK;
+  if (state->bits != 8 || m == nullptr || v == nullptr || !AlignedTo(m, 16) ||
+      !AlignedTo(v, 16)) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: moments of 32 bits are float32 already, or arrays to "
+                "write are missing or not aligned to 16 bytes");
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(
+      DecodeMoments,
+      dim3(static_cast<uint32_t>(CeilDiv(state->size, kStep))),
+      dim3(kThreads), 0, s, static_cast<const int8_t*>(state->m),
+      static_cast<const uint8_t*>(state->v), state->m_scale, state->v_scale,
+      state->size, m, v);
+  SCEMB_LAUNCH_CHECK();
+  return SCEMB_OK;
+}
+
+}  // extern "C"

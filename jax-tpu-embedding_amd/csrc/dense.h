@@ -1,0 +1,106 @@
+// Device helpers of the dense operators (layer_norm.hip, experts.hip,
+// adamw.hip): element types, vectors of them, and sums over lanes.
+#pragma once
+
+#include "../../include/scemb.h"
+#include "common.h"
+
+namespace scemb {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+// V consecutive elements, loaded and stored with one instruction of up to 16
+// bytes.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> LoadVec(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void StoreVec(T* p, const Vec<T, V>& x) {
+  *reinterpret_cast<Vec<T, V>*>(p) = x;
+}
+
+// ---------------------------------------------------------------------------
+// Sums over G neighbouring lanes (G a power of two up to 64); every lane gets
+// the sum. Steps within 16 lanes are DPP moves, the last two the lane swaps
+// of gfx950: no LDS traffic. Each step adds the same two partial sums in both
+// lanes, so all lanes hold the same bits.
+// ---------------------------------------------------------------------------
+
+template <int kCtrl>
+__device__ __forceinline__ float DppMove(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), kCtrl, 0xf,
+                                      0xf, true));
+}
+
+constexpr int kDppXor1 = 0xb1;         // quad_perm [1, 0, 3, 2]
+constexpr int kDppXor2 = 0x4e;         // quad_perm [2, 3, 0, 1]
+constexpr int kDppHalfMirror = 0x141;  // lane i of 8 <- lane 7 - i
+constexpr int kDppMirror = 0x140;      // lane i of 16 <- lane 15 - i
+
+struct LaneAdd {
+  static __device__ __forceinline__ float Of(float a, float b) {
+    return a + b;
+  }
+};
+// The larger of two values that are not negative, as bit patterns: a NaN is
+// above every number and stays.
+struct LaneMaxBits {
+  static __device__ __forceinline__ float Of(float a, float b) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, a);
+    const uint32_t y = __builtin_bit_cast(uint32_t, b);
+    return __builtin_bit_cast(float, x > y ? x : y);
+  }
+};
+
+template <typename Op, int G>
+__device__ __forceinline__ float LaneReduce(float x) {
+  static_assert(G >= 1 && G <= kWave && (G & (G - 1)) == 0, "power of two");
+  if constexpr (G >= 2) x = Op::Of(x, DppMove<kDppXor1>(x));
+  if constexpr (G >= 4) x = Op::Of(x, DppMove<kDppXor2>(x));
+  if constexpr (G >= 8) x = Op::Of(x, DppMove<kDppHalfMirror>(x));
+  if constexpr (G >= 16) x = Op::Of(x, DppMove<kDppMirror>(x));
+  if constexpr (G >= 32) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    // Copies: a bit cast of a vector's element reads element 0.
+    const uint32_t lo = r[0], hi = r[1];
+    x = Op::Of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+  }
+  if constexpr (G >= 64) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    // Copies: a bit cast of a vector's element reads element 0.
+    const uint32_t lo = r[0], hi = r[1];
+    x = Op::Of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+  }
+  return x;
+}
+
+template <int G>
+__device__ __forceinline__ float LaneSum(float x) {
+  return LaneReduce<LaneAdd, G>(x);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+
+inline int TypeBytes(int32_t type) {
+  return type == SCEMB_F32 ? 4
+         : type == SCEMB_BF16 || type == SCEMB_F16 ? 2
+                                                   : 0;
+}
+
+inline bool AlignedTo(const void* p, size_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+}  // namespace scemb
