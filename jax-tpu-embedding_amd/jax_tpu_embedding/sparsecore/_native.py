@@ -293,61 +293,6 @@ class PreprocessJob(ctypes.Structure):
   ]
 
 
-# Element types of the dense operators.
-TYPE_F32 = 0
-TYPE_BF16 = 1
-TYPE_F16 = 2
-
-MAX_EXPERTS = 1024
-ADAMW_BLOCK = 256
-
-
-class ExpertOrder(ctypes.Structure):
-  _fields_ = [
-      ("positions", ctypes.c_void_p),
-      ("offsets", ctypes.c_void_p),
-      ("tokens", ctypes.c_int64),
-      ("choices", ctypes.c_int32),
-      ("num_experts", ctypes.c_int32),
-  ]
-
-
-# scemb_adamw_tensor_t as a numpy record: an array of them is filled column by
-# column.
-ADAMW_TENSOR = np.dtype([
-    ("param", np.uint64), ("grad", np.uint64), ("copy", np.uint64),
-    ("numel", np.int64), ("param_type", np.int32), ("grad_type", np.int32),
-    ("decay", np.int32), ("reserved", np.int32)])
-assert ADAMW_TENSOR.itemsize == 48
-
-
-class AdamWState(ctypes.Structure):
-  _fields_ = [
-      ("m", ctypes.c_void_p),
-      ("v", ctypes.c_void_p),
-      ("m_scale", ctypes.c_void_p),
-      ("v_scale", ctypes.c_void_p),
-      ("size", ctypes.c_int64),
-      ("bits", ctypes.c_int32),
-      ("reserved", ctypes.c_int32),
-  ]
-
-
-class AdamWOptions(ctypes.Structure):
-  _fields_ = [
-      ("learning_rate", ctypes.c_double),
-      ("beta_1", ctypes.c_double),
-      ("beta_2", ctypes.c_double),
-      ("epsilon", ctypes.c_double),
-      ("weight_decay", ctypes.c_double),
-      ("grad_scale", ctypes.c_double),
-      ("step", ctypes.c_int64),
-      ("learning_rate_ptr", ctypes.c_void_p),
-      ("step_ptr", ctypes.c_void_p),
-      ("grad_scale_ptr", ctypes.c_void_p),
-  ]
-
-
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -465,37 +410,46 @@ def load_library() -> ctypes.CDLL:
     lib.scemb_profile_collect.argtypes = [ctypes.c_char_p,
                                           ctypes.POINTER(ctypes.c_double),
                                           ctypes.POINTER(ctypes.c_int64)]
-    order_p = ctypes.POINTER(ExpertOrder)
-    adamw_p = ctypes.POINTER(AdamWState)
-    lib.scemb_layer_norm.restype = ctypes.c_int
-    lib.scemb_layer_norm.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, f32,
-                                     vp, vp, vp, vp]
-    lib.scemb_layer_norm_grad_workspace_size.restype = sz
-    lib.scemb_layer_norm_grad_workspace_size.argtypes = [i32, i64, i64]
-    lib.scemb_layer_norm_grad.restype = ctypes.c_int
-    lib.scemb_layer_norm_grad.argtypes = [
-        vp, i64, vp, i64, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp, vp, sz,
-        vp]
-    lib.scemb_sort_by_expert_workspace_size.restype = sz
-    lib.scemb_sort_by_expert_workspace_size.argtypes = [i64, i32]
-    lib.scemb_sort_by_expert.restype = ctypes.c_int
-    lib.scemb_sort_by_expert.argtypes = [vp, i32, i64, i32, vp, vp, vp, vp, sz,
-                                         vp]
-    lib.scemb_tokens_to_experts.restype = ctypes.c_int
-    lib.scemb_tokens_to_experts.argtypes = [vp, i32, i64, i64, order_p, vp, vp]
-    lib.scemb_tokens_from_experts.restype = ctypes.c_int
-    lib.scemb_tokens_from_experts.argtypes = [vp, i32, i64, i64, vp, i32,
-                                              order_p, vp, vp]
-    lib.scemb_tokens_from_experts_grad.restype = ctypes.c_int
-    lib.scemb_tokens_from_experts_grad.argtypes = [
-        vp, i64, vp, i32, i64, i64, vp, i32, order_p, vp, vp, vp]
-    lib.scemb_adamw_update.restype = ctypes.c_int
-    lib.scemb_adamw_update.argtypes = [vp, i32, adamw_p,
-                                       ctypes.POINTER(AdamWOptions), vp]
-    lib.scemb_adamw_moments.restype = ctypes.c_int
-    lib.scemb_adamw_moments.argtypes = [adamw_p, vp, vp, vp]
     _lib = lib
     return lib
+
+
+# The functions that the dense operators' module calls, in its order.
+_DENSE_FUNCTIONS = (
+    "scemb_last_error",
+    "scemb_layer_norm",
+    "scemb_layer_norm_grad_workspace_size",
+    "scemb_layer_norm_grad",
+    "scemb_sort_by_expert_workspace_size",
+    "scemb_sort_by_expert",
+    "scemb_tokens_to_experts",
+    "scemb_tokens_from_experts",
+    "scemb_tokens_from_experts_grad",
+    "scemb_adamw_update",
+    "scemb_adamw_moments",
+)
+
+_dense_module = None
+
+
+def dense_binding():
+  """The Python module of the dense operators' calls (csrc/dense_binding.cc),
+  bound to the loaded library; raises RuntimeError when it was not built."""
+  global _dense_module
+  if _dense_module is None:
+    lib = load_library()
+    try:
+      from jax_tpu_embedding.sparsecore import _dense  # pylint: disable=g-import-not-at-top
+    except ImportError as e:
+      raise RuntimeError(
+          f"the dense operators' module is missing or does not load ({e}); "
+          "build it with `python -c 'import __graft_entry__; "
+          "__graft_entry__.build()'` or `make -C jax-tpu-embedding_amd/csrc`."
+      ) from e
+    _dense.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value
+                 for f in _DENSE_FUNCTIONS])
+    _dense_module = _dense
+  return _dense_module
 
 
 def profile_enable(on: bool) -> None:
@@ -1226,84 +1180,3 @@ def sparse_dense_matmul_grad_with_optimizer(
         stream_handle())
   del keep
   check(rc)
-
-
-# ---------------------------------------------------------------------------
-# Dense operators (lib/nn/dense.py checks what it hands over).
-# ---------------------------------------------------------------------------
-
-
-def layer_norm(x, type_code: int, rows: int, dim: int, stride: int, weight,
-               bias, weight_type: int, epsilon: float, y, mean, rstd) -> None:
-  check(load_library().scemb_layer_norm(
-      x.data_ptr(), type_code, rows, dim, stride, ptr(weight), ptr(bias),
-      weight_type, epsilon, y.data_ptr(), ptr(mean), ptr(rstd),
-      stream_handle()))
-
-
-def layer_norm_grad(y_grad, y_grad_stride: int, x, stride: int, type_code: int,
-                    rows: int, dim: int, mean, rstd, weight, weight_type: int,
-                    x_grad, weight_grad, bias_grad) -> None:
-  lib = load_library()
-  ws, size = None, 0
-  if weight_grad is not None or bias_grad is not None:
-    size = lib.scemb_layer_norm_grad_workspace_size(type_code, rows, dim)
-    if size == 0:
-      check(SCEMB_ERR_INVALID_ARGUMENT)
-    ws = WORKSPACE.get(size).data_ptr()
-  check(lib.scemb_layer_norm_grad(
-      y_grad.data_ptr(), y_grad_stride, x.data_ptr(), stride, type_code, rows,
-      dim, mean.data_ptr(), rstd.data_ptr(), ptr(weight), weight_type,
-      x_grad.data_ptr(), ptr(weight_grad), ptr(bias_grad), ws, size,
-      stream_handle()))
-
-
-def sort_by_expert(ids, id_bytes: int, num_experts: int, positions, sources,
-                   offsets) -> None:
-  lib = load_library()
-  n = ids.numel()
-  size = lib.scemb_sort_by_expert_workspace_size(n, num_experts)
-  if size == 0:
-    check(SCEMB_ERR_INVALID_ARGUMENT)
-  ws = WORKSPACE.get(size)
-  check(lib.scemb_sort_by_expert(
-      ids.data_ptr(), id_bytes, n, num_experts, positions.data_ptr(),
-      sources.data_ptr(), offsets.data_ptr(), ws.data_ptr(), size,
-      stream_handle()))
-
-
-def tokens_to_experts(x, type_code: int, stride: int, dim: int,
-                      order: ExpertOrder, rows) -> None:
-  check(load_library().scemb_tokens_to_experts(
-      x.data_ptr(), type_code, stride, dim, ctypes.byref(order),
-      rows.data_ptr(), stream_handle()))
-
-
-def tokens_from_experts(rows, type_code: int, stride: int, dim: int, weights,
-                        weights_type: int, order: ExpertOrder, y) -> None:
-  check(load_library().scemb_tokens_from_experts(
-      rows.data_ptr(), type_code, stride, dim, ptr(weights), weights_type,
-      ctypes.byref(order), y.data_ptr(), stream_handle()))
-
-
-def tokens_from_experts_grad(y_grad, y_grad_stride: int, rows, type_code: int,
-                             stride: int, dim: int, weights, weights_type: int,
-                             order: ExpertOrder, rows_grad,
-                             weights_grad) -> None:
-  check(load_library().scemb_tokens_from_experts_grad(
-      y_grad.data_ptr(), y_grad_stride, rows.data_ptr(), type_code, stride,
-      dim, ptr(weights), weights_type, ctypes.byref(order),
-      rows_grad.data_ptr(), ptr(weights_grad), stream_handle()))
-
-
-def adamw_update(tensors: np.ndarray, state: AdamWState,
-                 options: AdamWOptions) -> None:
-  """`tensors`: an array of ADAMW_TENSOR records."""
-  check(load_library().scemb_adamw_update(
-      tensors.ctypes.data, len(tensors), ctypes.byref(state),
-      ctypes.byref(options), stream_handle()))
-
-
-def adamw_moments(state: AdamWState, m, v) -> None:
-  check(load_library().scemb_adamw_moments(
-      ctypes.byref(state), m.data_ptr(), v.data_ptr(), stream_handle()))
