@@ -1,16 +1,18 @@
 // AdamW over many tensors at once, with moments in float32 or in 8 bits.
 //
 // One launch takes up to kMaxTensors tensors, whose addresses travel in the
-// kernel arguments; a work-group has kChunk consecutive values of one of them.
+// kernel arguments; a work-group has up to kSteps * kStep consecutive values of
+// one of them.
 // The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
 // bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy.
 //
 // Moments of 8 bits are decoded, moved, used and encoded in registers. A block
 // of 256 values is the four values of each lane of a wavefront, so its scale
 // is a maximum over lanes. Products and sums are rounded one by one (the file
-// is compiled without contraction) and the roots and quotients behind a code
-// are correctly rounded, so a code is a function of its block alone, whatever
-// kernel computes it.
+// is compiled without contraction) and codes are those of correctly rounded
+// roots and quotients, so a code is a function of its block alone, whatever
+// computes it. The weight's own update uses the approximate reciprocal, an ulp
+// off: against a correctly rounded division a few ulp of the update.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -23,9 +25,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPer = 4;                    // consecutive values of a lane
 constexpr int kStep = kThreads * kPer;     // values of a work-group at a time
-constexpr int kChunk = 4 * kStep;          // values of a work-group
+constexpr int kSteps = 4;                  // steps of a work-group
 constexpr int kQuant = SCEMB_ADAMW_BLOCK;  // values that share a scale
 constexpr int kMaxTensors = 64;            // a launch: a tensor a lane
+constexpr int kCus = 256;
 static_assert(kQuant == kWave * kPer, "a block is one step of a wavefront");
 
 struct Tensor {
@@ -37,7 +40,6 @@ struct Tensor {
   uint8_t param_bf16;
   uint8_t grad_bf16;
   uint8_t decay;
-  uint8_t aligned;  // four values can be loaded and stored at once
 };
 
 struct Moments {
@@ -75,6 +77,7 @@ struct AdamArgs {
   double weight_decay;
   int64_t step;
   int32_t n;
+  int32_t steps;
 };
 static_assert(sizeof(AdamArgs) <= 3584,
               "the arguments must fit the kernel argument block");
@@ -88,33 +91,34 @@ __host__ __device__ inline void SetRates(double learning_rate, double beta_1,
   f->keep = static_cast<float>(1.0 - learning_rate * weight_decay);
 }
 
+// The lane's values, of which `count` exist.
 template <typename T>
-__device__ __forceinline__ void Load4(const T* p, int64_t at, int count,
-                                      bool whole, float (&x)[kPer]) {
-  if (whole) {
-    const auto v = LoadVec<T, kPer>(p + at);
+__device__ __forceinline__ void Load4(const T* p, int count,
+                                      float (&x)[kPer]) {
+  if (count == kPer) {
+    const auto v = LoadVec<T, kPer>(p);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) x[j] = static_cast<float>(v.v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      x[j] = j < count ? static_cast<float>(p[at + j]) : 0.f;
+      x[j] = j < count ? static_cast<float>(p[j]) : 0.f;
     }
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void Store4(T* p, int64_t at, int count, bool whole,
+__device__ __forceinline__ void Store4(T* p, int count,
                                        const float (&x)[kPer]) {
-  if (whole) {
+  if (count == kPer) {
     Vec<T, kPer> v;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) v.v[j] = static_cast<T>(x[j]);
-    StoreVec<T, kPer>(p + at, v);
+    StoreVec<T, kPer>(p, v);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      if (j < count) p[at + j] = static_cast<T>(x[j]);
+      if (j < count) p[j] = static_cast<T>(x[j]);
     }
   }
 }
@@ -128,39 +132,59 @@ __device__ __forceinline__ float DecodeR(uint8_t q, float scale) {
   return x * x * scale;
 }
 
-// Rounded to nearest, ties to even. A scale of zero has only zeros below it.
-__device__ __forceinline__ int8_t EncodeM(float m, float scale) {
-  const float q = fminf(
-      rintf(sqrtf(fabsf(m) / (scale > 0.f ? scale : 1.f)) * 127.f), 127.f);
-  return static_cast<int8_t>(m < 0.f ? -q : q);
-}
-__device__ __forceinline__ uint8_t EncodeR(float r, float scale) {
-  const float q =
-      fminf(rintf(sqrtf(r / (scale > 0.f ? scale : 1.f)) * 255.f), 255.f);
-  return static_cast<uint8_t>(r > 0.f && q < 1.f ? 1.f : q);
+// The code of x >= 0 (kLevels: 127 or 255) among values up to `scale`:
+// sqrt(x / scale) * kLevels, rounded to nearest, ties to even. A scale of zero
+// has only zeros below it.
+template <int kLevels>
+__device__ __forceinline__ float CodeExact(float x, float scale) {
+  constexpr float kMost = kLevels;
+  return fminf(rintf(sqrtf(x / (scale > 0.f ? scale : 1.f)) * kMost), kMost);
 }
 
-// One chunk of one tensor: values [begin, begin + kChunk) of it.
+// The same code at a third of the instructions. With r = 1 / scale to an ulp,
+// sqrt(x * r) * kLevels by the approximate root is within 2.8e-7 of the exact
+// value (half of an ulp of r and of the product's rounding, an ulp of the
+// root, the last rounding), and what CodeExact rounds within 1.6e-7: 4.4e-7 *
+// kLevels apart, 5.6e-5 and 1.1e-4. Where the nearest half is further away
+// than twice that, both round alike; elsewhere (and for NaN) the exact one
+// decides, for one lane in 4000 to 2000.
+template <int kLevels>
+__device__ __forceinline__ float CodeOf(float x, float scale, float r) {
+  constexpr float kNear = 0.5f - kLevels * 1e-6f;
+  const float u = __builtin_amdgcn_sqrtf(x * r) * kLevels;
+  float q = rintf(u);
+  if (!(fabsf(u - q) < kNear)) q = CodeExact<kLevels>(x, scale);
+  return q;
+}
+
+// Whether r = 1 / scale may be used: below, the reciprocal could overflow.
+// Such blocks (and zero and non-finite ones) take CodeExact throughout.
+__device__ __forceinline__ bool OrdinaryScale(float scale) {
+  return scale > 0x1p-100f && scale < 0x1p100f;
+}
+
+// One chunk of one tensor: `steps` times kStep values from `begin` on.
 template <int kBits, typename P, typename G>
 __device__ __forceinline__ void UpdateChunk(const Tensor& t, const Moments& s,
-                                            const Factors& f, int64_t begin) {
+                                            const Factors& f, int64_t begin,
+                                            int steps) {
   P* param = static_cast<P*>(t.param);
   const G* grad = static_cast<const G*>(t.grad);
   bf16* copy = static_cast<bf16*>(t.copy);
   const float keep = t.decay ? f.keep : 1.f;
   const int64_t arena = static_cast<int64_t>(t.block) * kQuant;
-  for (int64_t base = begin; base < begin + kChunk; base += kStep) {
+  for (int k = 0; k < steps; ++k) {
+    const int64_t base = begin + k * kStep;
     const int64_t at = base + threadIdx.x * kPer;
     // The wavefront's 256 values: all of its lanes go on, or none.
     if (at - (threadIdx.x % kWave) * kPer >= t.numel) break;
     const int64_t left = t.numel - at;
     const int count = left < 0 ? 0 : left < kPer ? static_cast<int>(left)
                                                  : kPer;
-    const bool whole = count == kPer && t.aligned;
     const int64_t slot = arena + at;
     float p[kPer], g[kPer], m[kPer], v[kPer], r[kPer];
-    Load4<P>(param, at, count, whole, p);
-    Load4<G>(grad, at, count, whole, g);
+    Load4<P>(param + at, count, p);
+    Load4<G>(grad + at, count, g);
     if constexpr (kBits == 8) {
       const auto qm =
           LoadVec<int8_t, kPer>(static_cast<const int8_t*>(s.m) + slot);
@@ -190,11 +214,12 @@ __device__ __forceinline__ void UpdateChunk(const Tensor& t, const Moments& s,
       const float x = g[j] * f.grad_scale;
       m[j] = m[j] * f.beta_1 + x * f.gain_1;
       v[j] = v[j] * f.beta_2 + x * x * f.gain_2;
-      r[j] = sqrtf(v[j]);
-      p[j] = p[j] * keep - m[j] / (r[j] * f.root + f.epsilon) * f.rate;
+      r[j] = kBits == 8 ? sqrtf(v[j]) : __builtin_amdgcn_sqrtf(v[j]);
+      p[j] = p[j] * keep -
+             m[j] * __builtin_amdgcn_rcpf(r[j] * f.root + f.epsilon) * f.rate;
     }
-    Store4<P>(param, at, count, whole, p);
-    if (copy != nullptr) Store4<bf16>(copy, at, count, whole, p);
+    Store4<P>(param + at, count, p);
+    if (copy != nullptr) Store4<bf16>(copy + at, count, p);
     if constexpr (kBits == 8) {
       // Past the tensor's end the codes decode to zero and so do these; the
       // moments there are written back as they were.
@@ -209,10 +234,19 @@ __device__ __forceinline__ void UpdateChunk(const Tensor& t, const Moments& s,
       vs = LaneReduce<LaneMaxBits, kWave>(vs);
       Vec<int8_t, kPer> qm;
       Vec<uint8_t, kPer> qv;
+      const bool ordinary = OrdinaryScale(ms) && OrdinaryScale(vs);
+      const float mr = __builtin_amdgcn_rcpf(ms);
+      const float vr = __builtin_amdgcn_rcpf(vs);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        qm.v[j] = EncodeM(m[j], ms);
-        qv.v[j] = EncodeR(r[j], vs);
+        const float a = fabsf(m[j]);
+        const float cm = ordinary ? CodeOf<127>(a, ms, mr)
+                                  : CodeExact<127>(a, ms);
+        const float cv = ordinary ? CodeOf<255>(r[j], vs, vr)
+                                  : CodeExact<255>(r[j], vs);
+        qm.v[j] = static_cast<int8_t>(m[j] < 0.f ? -cm : cm);
+        qv.v[j] =
+            static_cast<uint8_t>(r[j] > 0.f && cv < 1.f ? 1.f : cv);
       }
       StoreVec<int8_t, kPer>(static_cast<int8_t*>(s.m) + slot, qm);
       StoreVec<uint8_t, kPer>(static_cast<uint8_t*>(s.v) + slot, qv);
@@ -251,18 +285,18 @@ __global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs a) {
              a.step_ptr != nullptr ? *a.step_ptr : a.step, &f);
   }
   if (a.grad_scale_ptr != nullptr) f.grad_scale = *a.grad_scale_ptr;
-  const int64_t begin =
-      static_cast<int64_t>(blockIdx.x - a.first[i]) * kChunk;
+  const int64_t begin = static_cast<int64_t>(blockIdx.x - a.first[i]) *
+                        (a.steps * kStep);
   if (t.param_bf16) {
     if (t.grad_bf16) {
-      UpdateChunk<kBits, bf16, bf16>(t, a.moments, f, begin);
+      UpdateChunk<kBits, bf16, bf16>(t, a.moments, f, begin, a.steps);
     } else {
-      UpdateChunk<kBits, bf16, float>(t, a.moments, f, begin);
+      UpdateChunk<kBits, bf16, float>(t, a.moments, f, begin, a.steps);
     }
   } else if (t.grad_bf16) {
-    UpdateChunk<kBits, float, bf16>(t, a.moments, f, begin);
+    UpdateChunk<kBits, float, bf16>(t, a.moments, f, begin, a.steps);
   } else {
-    UpdateChunk<kBits, float, float>(t, a.moments, f, begin);
+    UpdateChunk<kBits, float, float>(t, a.moments, f, begin, a.steps);
   }
 }
 
@@ -299,12 +333,10 @@ int CheckState(const scemb_adamw_state_t* s) {
                 "no multiple of the block");
   }
   if (s->size > 0 &&
-      (s->m == nullptr || s->v == nullptr || !AlignedTo(s->m, 16) ||
-       !AlignedTo(s->v, 16) ||
+      (s->m == nullptr || s->v == nullptr ||
        (s->bits == 8 && (s->m_scale == nullptr || s->v_scale == nullptr)))) {
     return Fail(SCEMB_ERR_INVALID_ARGUMENT,
-                "adamw: moments or scales missing, or moments not aligned to "
-                "16 bytes");
+                "adamw: moments or scales missing");
   }
   return 0;
 }
@@ -380,6 +412,11 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
   a.beta_2 = options->beta_2;
   a.weight_decay = options->weight_decay;
   a.step = options->step;
+  // Steps one after another cost their latency (2 us each) where there is not
+  // a work-group for every CU without them.
+  a.steps = blocks * kQuant > kCus * static_cast<int64_t>(kStep) * kSteps
+                ? kSteps
+                : 1;
   a.n = 0;
   uint32_t block = 0;
   int64_t groups = 0;
@@ -387,7 +424,7 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
   for (int32_t i = 0; i < num_tensors; ++i) {
     const scemb_adamw_tensor_t& t = tensors[i];
     if (t.grad != nullptr && t.numel > 0) {
-      const int64_t mine = CeilDiv(t.numel, kChunk);
+      const int64_t mine = CeilDiv(t.numel, a.steps * kStep);
       if (a.n == kMaxTensors || groups + mine > 0x7fffffff) {
         const int rc = LaunchUpdate(a, static_cast<uint32_t>(groups),
                                     state->bits, s);
@@ -405,9 +442,6 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
       d.param_bf16 = t.param_type == SCEMB_BF16;
       d.grad_bf16 = t.grad_type == SCEMB_BF16;
       d.decay = t.decay != 0;
-      d.aligned = AlignedTo(t.param, d.param_bf16 ? 8 : 16) &&
-                  AlignedTo(t.grad, d.grad_bf16 ? 8 : 16) &&
-                  AlignedTo(t.copy, 8);
       ++a.n;
       groups += mine;
     }
@@ -423,11 +457,10 @@ int scemb_adamw_moments(const scemb_adamw_state_t* state, float* m, float* v,
   const int bad = CheckState(state);
   if (bad != 0) return bad;
   if (state->size == 0) return SCEMB_OK;
-  if (state->bits != 8 || m == nullptr || v == nullptr || !AlignedTo(m, 16) ||
-      !AlignedTo(v, 16)) {
+  if (state->bits != 8 || m == nullptr || v == nullptr) {
     return Fail(SCEMB_ERR_INVALID_ARGUMENT,
                 "adamw: moments of 32 bits are float32 already, or arrays to "
-                "write are missing or not aligned to 16 bytes");
+                "write are missing");
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(

@@ -14,6 +14,7 @@ namespace scemb {
 namespace {
 
 constexpr int kCus = 256;
+constexpr int kForwardThreads = 2048;  // of a CU
 
 template <typename T>
 struct NormArgs {
@@ -46,24 +47,29 @@ struct NormGradArgs {
   bool weight_f32;
 };
 
-// V weights from `at` on as float32 (`p` NULL: `missing`).
-template <typename T, int V>
-__device__ __forceinline__ void LoadWeights(const void* p, bool f32, int at,
+// A vector's weights as float32 (`p` NULL: `missing`).
+template <Cut kCut, typename T, int V>
+__device__ __forceinline__ void LoadWeights(const void* p, bool f32,
+                                            const Span<kCut, V>& s,
                                             float missing, float (&w)[V]) {
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < V; ++j) w[j] = missing;
   } else if (f32 || sizeof(T) == 4) {
-    constexpr int kPart = V < 4 ? V : 4;
+    const float* q = static_cast<const float*>(p);
+    if constexpr (kCut == Cut::kPart) {
 #pragma unroll
-    for (int j = 0; j < V; j += kPart) {
-      const auto v = LoadVec<float, kPart>(static_cast<const float*>(p) + at +
-                                           j);
+      for (int j = 0; j < V; ++j) w[j] = j < s.hi ? q[j] : 0.f;
+    } else {
 #pragma unroll
-      for (int k = 0; k < kPart; ++k) w[j + k] = v.v[k];
+      for (int j = 0; j < V; j += 4) {
+        const auto v = LoadVec<float, 4>(q + s.at + j);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[j + k] = v.v[k];
+      }
     }
   } else {
-    const auto v = LoadVec<T, V>(static_cast<const T*>(p) + at);
+    const auto v = LoadSpan<kCut, T, V>(static_cast<const T*>(p), s);
 #pragma unroll
     for (int j = 0; j < V; ++j) w[j] = static_cast<float>(v.v[j]);
   }
@@ -94,15 +100,46 @@ __device__ __forceinline__ void RowSum(float (&x)[N], float* part) {
   }
 }
 
+// Keeps a row's 16-bit elements packed over a reduction: without it the
+// compiler holds on to their float32 values, twice the registers.
+template <typename T, int NV>
+__device__ __forceinline__ void StayPacked(Vec<T, kVec<T>> (&x)[NV]) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      Words w = __builtin_bit_cast(Words, x[i]);
+      asm volatile("" : "+v"(w));
+      x[i] = __builtin_bit_cast(Vec<T, kVec<T>>, w);
+    }
+  }
+}
+
 constexpr int BlockOf(int g) { return g > 256 ? g : 256; }
 
-template <typename T, int V, int NV, int G>
+// The G lanes of a row take every gridDim.x-th row and keep their columns'
+// weights in registers: read from the caches for every row, float32 weights of
+// 16-bit rows are twice the bytes of the row and its result together (65,536 x
+// 3328 bfloat16: 330 us that way, 169 this way).
+template <typename T, int NV, int G, Cut kCut>
 __global__ __launch_bounds__(BlockOf(G)) void NormForward(NormArgs<T> a) {
+  constexpr int V = kVec<T>;
   constexpr int kRows = BlockOf(G) / G;
   constexpr int kParts = G > kWave ? G / kWave : 1;
+  using At = Span<kCut, V>;
   __shared__ float part[2 * kParts];
   const int lane = threadIdx.x % G;
   const float scale = 1.f / static_cast<float>(a.dim);
+  float w[NV][V], b[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + lane) * V;
+    if (c < a.dim) {
+      const At s(c, a.dim);
+      LoadWeights<kCut, T, V>(a.weight, a.weight_f32, s, 1.f, w[i]);
+      LoadWeights<kCut, T, V>(a.bias, a.weight_f32, s, 0.f, b[i]);
+    }
+  }
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows +
                      threadIdx.x / G;
        row < a.rows; row += static_cast<int64_t>(gridDim.x) * kRows) {
@@ -112,29 +149,38 @@ __global__ __launch_bounds__(BlockOf(G)) void NormForward(NormArgs<T> a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
-      if (c < a.dim) x[i] = LoadVec<T, V>(src + c);
+      if (c < a.dim) x[i] = LoadSpan<kCut, T, V>(src, At(c, a.dim));
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * G + lane) * V < a.dim) {
+      const int c = (i * G + lane) * V;
+      if (c < a.dim) {
+        const At s(c, a.dim);
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] += static_cast<float>(x[i].v[j]);
+        for (int j = 0; j < V; ++j) {
+          sum[0] += s.Has(j) ? static_cast<float>(x[i].v[j]) : 0.f;
+        }
       }
     }
     RowSum<G>(sum, part);
+    StayPacked<T, NV>(x);
     const float mean = sum[0] * scale;
     float sq[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * G + lane) * V < a.dim) {
+      const int c = (i * G + lane) * V;
+      if (c < a.dim) {
+        const At s(c, a.dim);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float d = static_cast<float>(x[i].v[j]) - mean;
+          const float d =
+              s.Has(j) ? static_cast<float>(x[i].v[j]) - mean : 0.f;
           sq[0] = fmaf(d, d, sq[0]);
         }
       }
     }
     RowSum<G>(sq, part + kParts);
+    StayPacked<T, NV>(x);
     const float rstd = rsqrtf(sq[0] * scale + a.epsilon);
     if (lane == 0) {
       if (a.mean != nullptr) a.mean[row] = mean;
@@ -145,16 +191,13 @@ __global__ __launch_bounds__(BlockOf(G)) void NormForward(NormArgs<T> a) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
       if (c < a.dim) {
-        float w[V], b[V];
-        LoadWeights<T, V>(a.weight, a.weight_f32, c, 1.f, w);
-        LoadWeights<T, V>(a.bias, a.weight_f32, c, 0.f, b);
         Vec<T, V> y;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float xhat = (static_cast<float>(x[i].v[j]) - mean) * rstd;
-          y.v[j] = static_cast<T>(fmaf(xhat, w[j], b[j]));
+          y.v[j] = static_cast<T>(fmaf(xhat, w[i][j], b[i][j]));
         }
-        StoreVec<T, V>(dst + c, y);
+        StoreSpan<kCut, T, V>(dst, At(c, a.dim), y);
       }
     }
   }
@@ -162,29 +205,33 @@ __global__ __launch_bounds__(BlockOf(G)) void NormForward(NormArgs<T> a) {
 
 // Rows longer than the registers of a work-group: three passes, the last two
 // mostly from L2.
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(1024) void NormForwardLong(NormArgs<T> a) {
   constexpr int G = 1024;
+  constexpr int V = kVec<T>;
+  using At = Span<Cut::kOver, V>;
   __shared__ float part[2 * (G / kWave)];
   const float scale = 1.f / static_cast<float>(a.dim);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* src = a.x + row * a.stride;
     float sum[1] = {0.f};
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.dim;
-         c += G * V) {
-      const auto x = LoadVec<T, V>(src + c);
+    for (int c = threadIdx.x * V; c < a.dim; c += G * V) {
+      const At s(c, a.dim);
+      const auto x = LoadVec<T, V>(src + s.at);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[0] += static_cast<float>(x.v[j]);
+      for (int j = 0; j < V; ++j) {
+        sum[0] += s.Has(j) ? static_cast<float>(x.v[j]) : 0.f;
+      }
     }
     RowSum<G>(sum, part);
     const float mean = sum[0] * scale;
     float sq[1] = {0.f};
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.dim;
-         c += G * V) {
-      const auto x = LoadVec<T, V>(src + c);
+    for (int c = threadIdx.x * V; c < a.dim; c += G * V) {
+      const At s(c, a.dim);
+      const auto x = LoadVec<T, V>(src + s.at);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = static_cast<float>(x.v[j]) - mean;
+        const float d = s.Has(j) ? static_cast<float>(x.v[j]) - mean : 0.f;
         sq[0] = fmaf(d, d, sq[0]);
       }
     }
@@ -195,19 +242,19 @@ __global__ __launch_bounds__(1024) void NormForwardLong(NormArgs<T> a) {
       if (a.rstd != nullptr) a.rstd[row] = rstd;
     }
     T* dst = a.y + row * a.dim;
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.dim;
-         c += G * V) {
-      const auto x = LoadVec<T, V>(src + c);
+    for (int c = threadIdx.x * V; c < a.dim; c += G * V) {
+      const At s(c, a.dim);
+      const auto x = LoadVec<T, V>(src + s.at);
       float w[V], b[V];
-      LoadWeights<T, V>(a.weight, a.weight_f32, static_cast<int>(c), 1.f, w);
-      LoadWeights<T, V>(a.bias, a.weight_f32, static_cast<int>(c), 0.f, b);
+      LoadWeights<Cut::kOver, T, V>(a.weight, a.weight_f32, s, 1.f, w);
+      LoadWeights<Cut::kOver, T, V>(a.bias, a.weight_f32, s, 0.f, b);
       Vec<T, V> y;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xhat = (static_cast<float>(x.v[j]) - mean) * rstd;
         y.v[j] = static_cast<T>(fmaf(xhat, w[j], b[j]));
       }
-      StoreVec<T, V>(dst + c, y);
+      StoreVec<T, V>(dst + s.at, y);
     }
   }
 }
@@ -215,12 +262,16 @@ __global__ __launch_bounds__(1024) void NormForwardLong(NormArgs<T> a) {
 // The G lanes of a row take every gridDim.x-th row and keep their columns'
 // share of the weight's and the bias's gradients in registers; at the end
 // the groups of a work-group are added in LDS, in their order, and the
-// work-group's sums go to `partial`.
-template <typename T, int V, int NV, int G>
+// work-group's sums go to `partial`. kHold: the weights stay in registers too
+// (where a work-group of 1024 has 16 values a lane there is no room).
+template <typename T, int NV, int G, Cut kCut>
 __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
+  constexpr int V = kVec<T>;
   constexpr int kBlock = BlockOf(G);
   constexpr int kGroups = kBlock / G;
   constexpr int kParts = G > kWave ? 2 * (G / kWave) : 1;
+  constexpr bool kHold = sizeof(T) == 2 || NV * G < 4096;
+  using At = Span<kCut, V>;
   __shared__ float part[2 * kParts];
   const int lane = threadIdx.x % G;
   const int group = threadIdx.x / G;
@@ -231,20 +282,22 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
     const int c = (i * G + lane) * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) w[i][j] = dw[i][j] = db[i][j] = 0.f;
-    if (c < a.dim) {
-      LoadWeights<T, V>(a.weight, a.weight_f32, c, 1.f, w[i]);
+    if (kHold && c < a.dim) {
+      LoadWeights<kCut, T, V>(a.weight, a.weight_f32, At(c, a.dim), 1.f, w[i]);
     }
   }
   int turn = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
        row < a.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
+    const T* px = a.x + row * a.stride;
+    const T* pdy = a.dy + row * a.dy_stride;
     Vec<T, V> x[NV], dy[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
       if (c < a.dim) {
-        x[i] = LoadVec<T, V>(a.x + row * a.stride + c);
-        dy[i] = LoadVec<T, V>(a.dy + row * a.dy_stride + c);
+        x[i] = LoadSpan<kCut, T, V>(px, At(c, a.dim));
+        dy[i] = LoadSpan<kCut, T, V>(pdy, At(c, a.dim));
       }
     }
     const float mean = a.mean[row];
@@ -252,12 +305,17 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * G + lane) * V < a.dim) {
+      const int c = (i * G + lane) * V;
+      if (c < a.dim) {
+        const At s(c, a.dim);
+        if (!kHold) {
+          LoadWeights<kCut, T, V>(a.weight, a.weight_f32, s, 1.f, w[i]);
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float g = static_cast<float>(dy[i].v[j]);
           const float xhat = (static_cast<float>(x[i].v[j]) - mean) * rstd;
-          const float h = g * w[i][j];
+          const float h = s.Has(j) ? g * w[i][j] : 0.f;
           sum[0] += h;
           sum[1] = fmaf(h, xhat, sum[1]);
           dw[i][j] = fmaf(g, xhat, dw[i][j]);
@@ -266,6 +324,8 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
       }
     }
     RowSum<G>(sum, part + turn * kParts);
+    StayPacked<T, NV>(x);
+    StayPacked<T, NV>(dy);
     turn ^= 1;
     const float along1 = sum[0] * scale;
     const float alongx = sum[1] * scale;
@@ -273,6 +333,10 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
       if (c < a.dim) {
+        const At s(c, a.dim);
+        if (!kHold) {
+          LoadWeights<kCut, T, V>(a.weight, a.weight_f32, s, 1.f, w[i]);
+        }
         Vec<T, V> dx;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -280,7 +344,7 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
           const float h = static_cast<float>(dy[i].v[j]) * w[i][j];
           dx.v[j] = static_cast<T>((h - along1 - xhat * alongx) * rstd);
         }
-        StoreVec<T, V>(a.dx + row * a.dim + c, dx);
+        StoreSpan<kCut, T, V>(a.dx + row * a.dim, s, dx);
       }
     }
   }
@@ -293,10 +357,13 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
       if (c < a.dim) {
+        const At s(c, a.dim);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          out[0][c + j] = dw[i][j];
-          out[1][c + j] = db[i][j];
+          if (s.Has(j)) {
+            out[0][s.at + j] = dw[i][j];
+            out[1][s.at + j] = db[i][j];
+          }
         }
       }
     }
@@ -308,10 +375,15 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + lane) * V;
+        if (c < a.dim) {
+          const At s(c, a.dim);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          all[group * kCols + (i * G + lane) * V + j] =
-              which == 0 ? dw[i][j] : db[i][j];
+          for (int j = 0; j < V; ++j) {
+            if (s.Has(j)) {
+              all[group * kCols + s.at + j] = which == 0 ? dw[i][j] : db[i][j];
+            }
+          }
         }
       }
       __syncthreads();
@@ -327,10 +399,12 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
 
 // Rows longer than the registers of a work-group: the gradient of x in two
 // passes over the row.
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(1024) void NormBackwardLong(NormGradArgs<T> a) {
   constexpr int G = 1024;
+  constexpr int V = kVec<T>;
   constexpr int kParts = 2 * (G / kWave);
+  using At = Span<Cut::kOver, V>;
   __shared__ float part[2 * kParts];
   const float scale = 1.f / static_cast<float>(a.dim);
   int turn = 0;
@@ -340,16 +414,16 @@ __global__ __launch_bounds__(1024) void NormBackwardLong(NormGradArgs<T> a) {
     const float mean = a.mean[row];
     const float rstd = a.rstd[row];
     float sum[2] = {0.f, 0.f};
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.dim;
-         c += G * V) {
-      const auto x = LoadVec<T, V>(px + c);
-      const auto dy = LoadVec<T, V>(pdy + c);
+    for (int c = threadIdx.x * V; c < a.dim; c += G * V) {
+      const At s(c, a.dim);
+      const auto x = LoadVec<T, V>(px + s.at);
+      const auto dy = LoadVec<T, V>(pdy + s.at);
       float w[V];
-      LoadWeights<T, V>(a.weight, a.weight_f32, static_cast<int>(c), 1.f, w);
+      LoadWeights<Cut::kOver, T, V>(a.weight, a.weight_f32, s, 1.f, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xhat = (static_cast<float>(x.v[j]) - mean) * rstd;
-        const float h = static_cast<float>(dy.v[j]) * w[j];
+        const float h = s.Has(j) ? static_cast<float>(dy.v[j]) * w[j] : 0.f;
         sum[0] += h;
         sum[1] = fmaf(h, xhat, sum[1]);
       }
@@ -358,12 +432,12 @@ __global__ __launch_bounds__(1024) void NormBackwardLong(NormGradArgs<T> a) {
     turn ^= 1;
     const float along1 = sum[0] * scale;
     const float alongx = sum[1] * scale;
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.dim;
-         c += G * V) {
-      const auto x = LoadVec<T, V>(px + c);
-      const auto dy = LoadVec<T, V>(pdy + c);
+    for (int c = threadIdx.x * V; c < a.dim; c += G * V) {
+      const At s(c, a.dim);
+      const auto x = LoadVec<T, V>(px + s.at);
+      const auto dy = LoadVec<T, V>(pdy + s.at);
       float w[V];
-      LoadWeights<T, V>(a.weight, a.weight_f32, static_cast<int>(c), 1.f, w);
+      LoadWeights<Cut::kOver, T, V>(a.weight, a.weight_f32, s, 1.f, w);
       Vec<T, V> dx;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -371,24 +445,25 @@ __global__ __launch_bounds__(1024) void NormBackwardLong(NormGradArgs<T> a) {
         const float h = static_cast<float>(dy.v[j]) * w[j];
         dx.v[j] = static_cast<T>((h - along1 - xhat * alongx) * rstd);
       }
-      StoreVec<T, V>(a.dx + row * a.dim + c, dx);
+      StoreVec<T, V>(a.dx + row * a.dim + s.at, dx);
     }
   }
 }
 
 // Their weight's and bias's gradients: a thread has V columns (blockIdx.x)
 // and every gridDim.y-th row.
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(256) void NormColumnsLong(NormGradArgs<T> a) {
-  const int64_t c =
-      (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
+  constexpr int V = kVec<T>;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * V;
   if (c >= a.dim) return;
+  const Span<Cut::kOver, V> s(c, a.dim);
   float dw[V], db[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) dw[j] = db[j] = 0.f;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const auto x = LoadVec<T, V>(a.x + row * a.stride + c);
-    const auto dy = LoadVec<T, V>(a.dy + row * a.dy_stride + c);
+    const auto x = LoadVec<T, V>(a.x + row * a.stride + s.at);
+    const auto dy = LoadVec<T, V>(a.dy + row * a.dy_stride + s.at);
     const float mean = a.mean[row];
     const float rstd = a.rstd[row];
 #pragma unroll
@@ -399,21 +474,26 @@ __global__ __launch_bounds__(256) void NormColumnsLong(NormGradArgs<T> a) {
       db[j] += g;
     }
   }
+  float* out = a.partial + static_cast<int64_t>(blockIdx.y) * a.dim + s.at;
+  const int64_t bias = static_cast<int64_t>(gridDim.y) * a.dim;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    a.partial[static_cast<int64_t>(blockIdx.y) * a.dim + c + j] = dw[j];
-    a.partial[(static_cast<int64_t>(gridDim.y) + blockIdx.y) * a.dim + c + j] =
-        db[j];
+    if (s.Has(j)) {
+      out[j] = dw[j];
+      out[bias + j] = db[j];
+    }
   }
 }
 
 // Adds the work-groups' sums: 32 columns a work-group, the `parts` rows of
-// sums in 8 slices that LDS joins in their order.
+// sums in 32 slices that LDS joins in their order. It is latency alone (8 to
+// 16 MB at most, from L2): eight loads of a thread are in flight.
 template <typename W>
-__global__ __launch_bounds__(256) void NormReduce(const float* partial,
-                                                  int32_t parts, int32_t dim,
-                                                  W* dweight, W* dbias) {
-  __shared__ float sums[8][32];
+__global__ __launch_bounds__(1024) void NormReduce(const float* partial,
+                                                   int32_t parts, int32_t dim,
+                                                   W* dweight, W* dbias) {
+  constexpr int kSlices = 32;
+  __shared__ float sums[kSlices][33];
   W* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
   const int col = threadIdx.x % 32;
@@ -423,16 +503,17 @@ __global__ __launch_bounds__(256) void NormReduce(const float* partial,
       partial + static_cast<int64_t>(blockIdx.y) * parts * dim + c;
   float s = 0.f;
   if (c < dim) {
-#pragma unroll 4
-    for (int p = slice; p < parts; p += 8) {
+#pragma unroll 8
+    for (int p = slice; p < parts; p += kSlices) {
       s += src[static_cast<int64_t>(p) * dim];
     }
   }
   sums[slice][col] = s;
   __syncthreads();
-  if (slice == 0 && c < dim) {
+  if (threadIdx.x < 32 && c < dim) {
+    s = 0.f;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][col];
+    for (int i = 0; i < kSlices; ++i) s += sums[i][col];
     out[c] = static_cast<W>(s);
   }
 }
@@ -442,58 +523,27 @@ __global__ __launch_bounds__(256) void NormReduce(const float* partial,
 // ---------------------------------------------------------------------------
 
 // How a row is laid out over lanes: G lanes of NV vectors each. The fewest
-// lanes whose registers hold the row, G = 0 for a row that no work-group
-// holds.
+// lanes that hold the row at 16 values a lane (their weights and, backwards,
+// two sums stay in registers too); G = 0 for a row that no work-group holds.
 struct Layout {
   int g;
   int nv;
 };
 
-Layout ForwardLayout(int v, int64_t dim) {
+Layout LayoutOf(int v, int64_t dim) {
   const int64_t n = CeilDiv(dim, v);
-  if (v == 1) {
-    return n <= 64      ? Layout{16, 4}
-           : n <= 256   ? Layout{64, 4}
-           : n <= 1024  ? Layout{64, 16}
-           : n <= 4096  ? Layout{256, 16}
-           : n <= 8192  ? Layout{1024, 8}
-                        : Layout{0, 0};
-  }
-  return n <= 4      ? Layout{4, 1}
-         : n <= 16   ? Layout{16, 1}
-         : n <= 32   ? Layout{16, 2}
-         : n <= 64   ? Layout{64, 1}
-         : n <= 128  ? Layout{64, 2}
-         : n <= 256  ? Layout{64, 4}
-         : n <= 512  ? Layout{64, 8}
-         : n <= 1024 ? Layout{256, 4}
-         : n <= 2048 ? Layout{256, 8}
-         : n <= 4096 ? Layout{1024, 4}
-                     : Layout{0, 0};
-}
-
-// At most 16 values a lane: their weights and two sums stay in registers too.
-Layout BackwardLayout(int v, int64_t dim) {
-  const int64_t n = CeilDiv(dim, v);
-  if (v == 1) {
-    return n <= 64      ? Layout{16, 4}
-           : n <= 256   ? Layout{64, 4}
-           : n <= 1024  ? Layout{64, 16}
-           : n <= 4096  ? Layout{256, 16}
-           : n <= 8192  ? Layout{1024, 8}
-                        : Layout{0, 0};
-  }
   const int most = 16 / v;  // vectors a lane
-  return n <= 4              ? Layout{4, 1}
-         : n <= 16           ? Layout{16, 1}
-         : n <= 32           ? Layout{16, 2}
-         : n <= 64           ? Layout{64, 1}
-         : n <= 128          ? Layout{64, 2}
-         : n <= 64 * most    ? Layout{64, most}
-         : n <= 512          ? Layout{256, 2}
-         : n <= 256 * most   ? Layout{256, most}
-         : n <= 2048         ? Layout{1024, 2}
-                             : Layout{0, 0};
+  return n <= 4            ? Layout{4, 1}
+         : n <= 16         ? Layout{16, 1}
+         : n <= 32         ? Layout{16, 2}
+         : n <= 64         ? Layout{64, 1}
+         : n <= 128        ? Layout{64, 2}
+         : n <= 64 * most  ? Layout{64, most}
+         : n <= 512        ? Layout{256, 2}
+         : n <= 256 * most ? Layout{256, most}
+         : n <= 2048       ? Layout{1024, 2}
+         : n <= 1024 * most ? Layout{1024, most}
+                            : Layout{0, 0};
 }
 
 // Work-groups of the backward pass, and so rows of partial sums: four a CU
@@ -508,123 +558,100 @@ int64_t BackwardParts(Layout l, int type_bytes, int64_t rows) {
   return std::max<int64_t>(1, std::min({most, by_rows, by_bytes}));
 }
 
-template <typename T>
-int VectorWidth(int64_t dim, int64_t stride_a, int64_t stride_b,
-                std::initializer_list<const void*> data) {
-  constexpr int V = 16 / sizeof(T);
-  if (dim % V != 0 || stride_a % V != 0 || stride_b % V != 0) return 1;
-  for (const void* p : data) {
-    if (!AlignedTo(p, 16)) return 1;
-  }
-  return V;
-}
-
-template <typename T, int V, int NV, int G>
+template <typename T, int NV, int G, Cut kCut>
 int LaunchForward(const NormArgs<T>& a, hipStream_t stream) {
-  const int64_t blocks = CeilDiv(a.rows, BlockOf(G) / G);
-  hipLaunchKernelGGL((NormForward<T, V, NV, G>),
-                     dim3(static_cast<uint32_t>(
-                         std::min<int64_t>(blocks, 0x7fffffff))),
-                     dim3(BlockOf(G)), 0, stream, a);
+  const int64_t blocks =
+      std::min<int64_t>(CeilDiv(a.rows, BlockOf(G) / G),
+                        kCus * (kForwardThreads / BlockOf(G)));
+  hipLaunchKernelGGL((NormForward<T, NV, G, kCut>),
+                     dim3(static_cast<uint32_t>(blocks)), dim3(BlockOf(G)), 0,
+                     stream, a);
   SCEMB_LAUNCH_CHECK();
   return 0;
 }
 
-template <typename T, int V, int NV, int G>
+template <typename T, int NV, int G, Cut kCut>
 int LaunchBackward(const NormGradArgs<T>& a, int64_t parts,
                    hipStream_t stream) {
-  hipLaunchKernelGGL((NormBackward<T, V, NV, G>),
+  hipLaunchKernelGGL((NormBackward<T, NV, G, kCut>),
                      dim3(static_cast<uint32_t>(parts)), dim3(BlockOf(G)), 0,
                      stream, a);
   SCEMB_LAUNCH_CHECK();
   return 0;
 }
 
-#define SCEMB_LAYOUT(G_, NV_, CALL)    \
-  if (l.g == G_ && l.nv == NV_) {      \
-    constexpr int G = G_, NV = NV_;    \
-    return CALL;                       \
+// Returns CALL with the layout's NV and G as constants. (A row below a vector
+// has one layout, 16-bit rows have at most two vectors a lane.)
+#define SCEMB_LAYOUT(G_, NV_, CALL)                                        \
+  if constexpr (NV_ * kVec<T> <= 16 &&                                     \
+                (kCut != Cut::kPart || (G_ == 4 && NV_ == 1))) {           \
+    if (l.g == G_ && l.nv == NV_) {                                        \
+      constexpr int G = G_, NV = NV_;                                      \
+      return CALL;                                                         \
+    }                                                                      \
+  }
+#define SCEMB_LAYOUTS(CALL)   \
+  SCEMB_LAYOUT(4, 1, CALL)    \
+  SCEMB_LAYOUT(16, 1, CALL)   \
+  SCEMB_LAYOUT(16, 2, CALL)   \
+  SCEMB_LAYOUT(64, 1, CALL)   \
+  SCEMB_LAYOUT(64, 2, CALL)   \
+  SCEMB_LAYOUT(64, 4, CALL)   \
+  SCEMB_LAYOUT(256, 2, CALL)  \
+  SCEMB_LAYOUT(256, 4, CALL)  \
+  SCEMB_LAYOUT(1024, 2, CALL) \
+  SCEMB_LAYOUT(1024, 4, CALL)
+// CALL for how rows of `dim` are cut.
+#define SCEMB_CUT(CALL)                           \
+  switch (CutOf(dim, kVec<T>)) {                  \
+    case Cut::kWhole: {                           \
+      constexpr Cut kCut = Cut::kWhole;           \
+      rc = CALL;                                  \
+      break;                                      \
+    }                                             \
+    case Cut::kOver: {                            \
+      constexpr Cut kCut = Cut::kOver;            \
+      rc = CALL;                                  \
+      break;                                      \
+    }                                             \
+    default: {                                    \
+      constexpr Cut kCut = Cut::kPart;            \
+      rc = CALL;                                  \
+    }                                             \
   }
 
-template <typename T>
+template <typename T, Cut kCut>
 int Forward(const NormArgs<T>& a, hipStream_t stream) {
-  constexpr int kWide = 16 / sizeof(T);
-  const int v = VectorWidth<T>(a.dim, a.stride, a.stride,
-                               {a.x, a.y, a.weight, a.bias});
-  const Layout l = ForwardLayout(v, a.dim);
-  const dim3 grid(
-      static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff)));
-  if (v == 1) {
-    constexpr int V = 1;
-    SCEMB_LAYOUT(16, 4, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 4, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 16, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(256, 16, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(1024, 8, (LaunchForward<T, V, NV, G>(a, stream)))
-    hipLaunchKernelGGL((NormForwardLong<T, V>), grid, dim3(1024), 0, stream,
-                       a);
-  } else {
-    constexpr int V = kWide;
-    SCEMB_LAYOUT(4, 1, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(16, 1, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(16, 2, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 1, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 2, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 4, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(64, 8, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(256, 4, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(256, 8, (LaunchForward<T, V, NV, G>(a, stream)))
-    SCEMB_LAYOUT(1024, 4, (LaunchForward<T, V, NV, G>(a, stream)))
-    hipLaunchKernelGGL((NormForwardLong<T, V>), grid, dim3(1024), 0, stream,
-                       a);
-  }
+  const Layout l = LayoutOf(kVec<T>, a.dim);
+  SCEMB_LAYOUTS((LaunchForward<T, NV, G, kCut>(a, stream)))
+  hipLaunchKernelGGL(
+      NormForwardLong<T>,
+      dim3(static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff))),
+      dim3(1024), 0, stream, a);
   SCEMB_LAUNCH_CHECK();
   return 0;
 }
 
-template <typename T, int V>
-int BackwardLong(const NormGradArgs<T>& a, int64_t parts, hipStream_t stream) {
-  const dim3 grid(
-      static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff)));
-  hipLaunchKernelGGL((NormBackwardLong<T, V>), grid, dim3(1024), 0, stream, a);
+template <typename T, Cut kCut>
+int Backward(const NormGradArgs<T>& a, Layout l, int64_t parts,
+             hipStream_t stream) {
+  SCEMB_LAYOUTS((LaunchBackward<T, NV, G, kCut>(a, parts, stream)))
+  hipLaunchKernelGGL(
+      NormBackwardLong<T>,
+      dim3(static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff))),
+      dim3(1024), 0, stream, a);
   SCEMB_LAUNCH_CHECK();
   if (a.partial != nullptr) {
     hipLaunchKernelGGL(
-        (NormColumnsLong<T, V>),
-        dim3(static_cast<uint32_t>(CeilDiv(a.dim, 256 * V)),
+        NormColumnsLong<T>,
+        dim3(static_cast<uint32_t>(CeilDiv(a.dim, 256 * kVec<T>)),
              static_cast<uint32_t>(parts)),
         dim3(256), 0, stream, a);
     SCEMB_LAUNCH_CHECK();
   }
   return 0;
 }
-
-template <typename T>
-int BackwardRows(const NormGradArgs<T>& a, int v, Layout l, int64_t parts,
-                 hipStream_t stream) {
-  if (v == 1) {
-    constexpr int V = 1;
-    SCEMB_LAYOUT(16, 4, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    SCEMB_LAYOUT(64, 4, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    SCEMB_LAYOUT(64, 16, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    SCEMB_LAYOUT(256, 16, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    SCEMB_LAYOUT(1024, 8, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    return BackwardLong<T, V>(a, parts, stream);
-  }
-  constexpr int V = 16 / sizeof(T);
-  SCEMB_LAYOUT(4, 1, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(16, 1, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(16, 2, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(64, 1, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(64, 2, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(256, 2, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  SCEMB_LAYOUT(1024, 2, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  if constexpr (V == 4) {
-    SCEMB_LAYOUT(64, 4, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-    SCEMB_LAYOUT(256, 4, (LaunchBackward<T, V, NV, G>(a, parts, stream)))
-  }
-  return BackwardLong<T, V>(a, parts, stream);
-}
+#undef SCEMB_LAYOUTS
 #undef SCEMB_LAYOUT
 
 int CheckNorm(int32_t type, int32_t weight_type, int64_t rows, int64_t dim) {
@@ -658,7 +685,9 @@ int RunForward(const void* x, int64_t rows, int64_t dim, int64_t stride,
   a.dim = static_cast<int32_t>(dim);
   a.weight_f32 = weight_f32;
   a.epsilon = epsilon;
-  return Forward<T>(a, stream);
+  int rc = 0;
+  SCEMB_CUT((Forward<T, kCut>(a, stream)))
+  return rc;
 }
 
 template <typename T, typename W>
@@ -666,7 +695,7 @@ int RunReduce(const float* partial, int64_t parts, int64_t dim, void* dweight,
               void* dbias, hipStream_t stream) {
   hipLaunchKernelGGL((NormReduce<W>),
                      dim3(static_cast<uint32_t>(CeilDiv(dim, 32)), 2),
-                     dim3(256), 0, stream, partial,
+                     dim3(1024), 0, stream, partial,
                      static_cast<int32_t>(parts), static_cast<int32_t>(dim),
                      static_cast<W*>(dweight), static_cast<W*>(dbias));
   SCEMB_LAUNCH_CHECK();
@@ -691,8 +720,7 @@ int RunBackward(const void* dy, int64_t dy_stride, const void* x,
   a.stride = stride;
   a.dim = static_cast<int32_t>(dim);
   a.weight_f32 = weight_f32;
-  const int v = VectorWidth<T>(dim, stride, dy_stride, {dy, x, dx, weight});
-  const Layout l = BackwardLayout(v, dim);
+  const Layout l = LayoutOf(kVec<T>, dim);
   const int64_t parts = BackwardParts(l, sizeof(T), rows);
   Arena arena(workspace, workspace_bytes);
   a.partial = nullptr;
@@ -704,7 +732,8 @@ int RunBackward(const void* dy, int64_t dy_stride, const void* x,
     }
   }
   if (rows > 0) {
-    const int rc = BackwardRows<T>(a, v, l, parts, stream);
+    int rc = 0;
+    SCEMB_CUT((Backward<T, kCut>(a, l, parts, stream)))
     if (rc != 0) return rc;
   }
   if (a.partial == nullptr) return 0;
@@ -752,13 +781,9 @@ size_t scemb_layer_norm_grad_workspace_size(int32_t type, int64_t rows,
   using namespace scemb;
   if (CheckNorm(type, type, rows, dim) != 0) return 0;
   const int bytes = TypeBytes(type);
-  // What a call needs depends on its alignment: the larger of the two.
-  int64_t parts = 0;
-  for (const int v : {1, 16 / bytes}) {
-    parts = std::max(parts, BackwardParts(BackwardLayout(v, dim), bytes, rows));
-  }
   Arena arena(nullptr, 0);
-  arena.Take<float>(2 * parts * dim);
+  arena.Take<float>(
+      2 * dim * BackwardParts(LayoutOf(16 / bytes, dim), bytes, rows));
   return arena.used();
 }
 
