@@ -20,17 +20,51 @@ struct Vec {
   T v[V];
 };
 
+// A vector's bytes as one value, aligned to 2 bytes as the smallest elements
+// are (1 for 4 bytes, which are 8-bit codes).
+template <int kBytes>
+struct Words;
+template <>
+struct Words<16> {
+  typedef uint32_t Vector __attribute__((ext_vector_type(4)));
+  typedef Vector Type __attribute__((aligned(2)));
+};
+template <>
+struct Words<8> {
+  typedef uint32_t Vector __attribute__((ext_vector_type(2)));
+  typedef Vector Type __attribute__((aligned(2)));
+};
+template <>
+struct Words<4> {
+  typedef uint32_t Type __attribute__((aligned(1)));
+};
+
 // Elements of 16 bytes.
 template <typename T>
 constexpr int kVec = 16 / sizeof(T);
 
-template <typename T, int V>
+// kStream: memory that is not touched again soon; the access leaves other data
+// in the caches.
+template <typename T, int V, bool kStream = false>
 __device__ __forceinline__ Vec<T, V> LoadVec(const T* p) {
-  return *reinterpret_cast<const Vec<T, V>*>(p);
+  if constexpr (kStream) {
+    using W = Words<sizeof(T) * V>;
+    return __builtin_bit_cast(
+        Vec<T, V>, __builtin_nontemporal_load(
+                       reinterpret_cast<const typename W::Type*>(p)));
+  } else {
+    return *reinterpret_cast<const Vec<T, V>*>(p);
+  }
 }
-template <typename T, int V>
+template <typename T, int V, bool kStream = false>
 __device__ __forceinline__ void StoreVec(T* p, const Vec<T, V>& x) {
-  *reinterpret_cast<Vec<T, V>*>(p) = x;
+  if constexpr (kStream) {
+    using W = Words<sizeof(T) * V>;
+    __builtin_nontemporal_store(__builtin_bit_cast(typename W::Type, x),
+                                reinterpret_cast<typename W::Type*>(p));
+  } else {
+    *reinterpret_cast<Vec<T, V>*>(p) = x;
+  }
 }
 
 // How rows of a length are cut into vectors of V elements.
@@ -117,9 +151,8 @@ struct LaneAdd {
 // above every number and stays.
 struct LaneMaxBits {
   static __device__ __forceinline__ float Of(float a, float b) {
-    const uint32_t x = __builtin_bit_cast(uint32_t, a);
-    const uint32_t y = __builtin_bit_cast(uint32_t, b);
-    return __builtin_bit_cast(float, x > y ? x : y);
+    return __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, a),
+                                         __builtin_bit_cast(uint32_t, b)));
   }
 };
 

@@ -14,7 +14,7 @@ namespace scemb {
 namespace {
 
 constexpr int kCus = 256;
-constexpr int kForwardThreads = 2048;  // of a CU
+constexpr int kForwardThreads = 4096;  // of a CU, about twice what it holds
 
 template <typename T>
 struct NormArgs {
@@ -546,12 +546,12 @@ Layout LayoutOf(int v, int64_t dim) {
                             : Layout{0, 0};
 }
 
-// Work-groups of the backward pass, and so rows of partial sums: four a CU
+// Work-groups of the backward pass, and so rows of partial sums: three a CU
 // (two of 1024 threads), each group of lanes at least one row, and no more
 // bytes of sums written and read than a quarter of what the rows are.
 int64_t BackwardParts(Layout l, int type_bytes, int64_t rows) {
   const int groups = l.g == 0 ? 1 : BlockOf(l.g) / l.g;
-  const int64_t most = l.g == 1024 || l.g == 0 ? kCus : 4 * kCus;
+  const int64_t most = l.g == 1024 || l.g == 0 ? kCus : 3 * kCus;
   const int64_t by_rows = CeilDiv(rows, groups);
   const int64_t by_bytes =
       std::max<int64_t>(rows * type_bytes * 3 / (4 * 16), 32);

@@ -143,9 +143,13 @@ def _blocks(x):
   return out.reshape(-1, 256)
 
 
-@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("offset,size", [(0, 1.0), (1, 1.0), (0, 1e-33),
+                                         (0, 1e-18), (0, 1e-12), (0, 1e-6),
+                                         (0, 1e9), (0, 1e17)])
 @pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16], ids=str)
-def test_8_bit_moments(gtype, offset):
+def test_8_bit_moments(gtype, offset, size):
+  """size: of the gradients; second moments from none (they underflow) to near
+  the largest float32."""
   params = _tensors(SIZES, torch.float32, 2, offset=offset)
   state = dense.init_adamw_state(params, state_bits=8)
   host = [(np.zeros(n, F), np.zeros(n, F)) for n in SIZES]  # m, root of v
@@ -156,6 +160,7 @@ def test_8_bit_moments(gtype, offset):
       g *= torch.exp(3 * torch.sin(torch.arange(g.numel(), device="cuda"))).to(
           gtype)
       g[g.abs() < 0.05] = 0
+      g *= size
     before = [_cpu(p).astype(F) for p in params]
     dense.adamw_update(params, grads, state, grad_scale=0.5, **HYPER)
     for i, n in enumerate(SIZES):
