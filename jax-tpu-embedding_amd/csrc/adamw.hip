@@ -26,11 +26,6 @@ constexpr int kPer = 4;                    // consecutive values of a lane
 constexpr int kStep = kThreads * kPer;     // values of a work-group
 constexpr int kQuant = SCEMB_ADAMW_BLOCK;  // values that share a scale
 constexpr int kMaxTensors = 64;            // a launch: a tensor a lane
-// Tensors of more than the last cache (256 MB) are streamed past it: 176M
-// float32 values 915 us through the caches, 829 past them; 79M with 8-bit
-// moments (whose codes stay) 255 and 212; but 4.9M values, which it holds, 22
-// and 24.
-constexpr int64_t kCacheBytes = 256 << 20;
 static_assert(kQuant == kWave * kPer, "a block is one step of a wavefront");
 
 struct Tensor {
@@ -455,6 +450,10 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto launch = [&]() {
     const uint32_t n = static_cast<uint32_t>(groups);
+    // Read and written past the caches where they cannot hold it until the
+    // next step: 176M float32 values 915 us through them, 829 past them; 79M
+    // with 8-bit moments (whose codes stay) 255 and 212; but 4.9M values 22 and
+    // 24.
     const bool past = bytes > kCacheBytes;
     return state->bits == 8 ? LaunchUpdate<8>(a, n, past, s)
                             : LaunchUpdate<32>(a, n, past, s);

@@ -285,7 +285,7 @@ struct Order {
 };
 
 // E: an unsigned type of the elements' size; they are only moved.
-template <typename E, int G, Cut kCut>
+template <typename E, int G, Cut kCut, bool kStream>
 __global__ __launch_bounds__(kRowBlock) void ToExperts(const E* x,
                                                        int64_t stride,
                                                        int32_t dim,
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kRowBlock) void ToExperts(const E* x,
     const int32_t* places = order.positions + t * order.choices;
     for (int32_t c = lane * V; c < dim; c += G * V) {
       const Span<kCut, V> s(c, dim);
-      const auto v = LoadSpan<kCut, E, V>(x + t * stride, s);
+      const auto v = LoadSpan<kCut, E, V, kStream>(x + t * stride, s);
       for (int k = 0; k < order.choices; ++k) {
         const uint32_t p = static_cast<uint32_t>(places[k]);
         if (p < all) {
@@ -320,7 +320,7 @@ __device__ __forceinline__ float WeightAt(const void* w, bool f32, int64_t i) {
                       : static_cast<float>(static_cast<const T*>(w)[i]);
 }
 
-template <typename T, int G, Cut kCut>
+template <typename T, int G, Cut kCut, bool kStream>
 __global__ __launch_bounds__(kRowBlock) void FromExperts(
     const T* rows, int64_t stride, int32_t dim, const void* weights,
     bool weights_f32, Order order, T* y) {
@@ -342,7 +342,8 @@ __global__ __launch_bounds__(kRowBlock) void FromExperts(
         const uint32_t p = static_cast<uint32_t>(order.positions[first + k]);
         if (p < kept) {
           const float w = WeightAt<T>(weights, weights_f32, first + k);
-          const auto v = LoadSpan<kCut, T, V>(rows + p * stride, s);
+          const auto v =
+              LoadSpan<kCut, T, V, kStream>(rows + p * stride, s);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             sum[j] = fmaf(w, static_cast<float>(v.v[j]), sum[j]);
@@ -475,12 +476,23 @@ int CheckOrder(const scemb_expert_order_t* o, int32_t type, int64_t dim) {
   return 0;
 }
 
+// Whether the tokens' and the choices' rows are more than the last cache.
+bool PastCache(const Order& o, int64_t dim, int64_t bytes) {
+  return o.tokens * (o.choices + 1) * dim * bytes > kCacheBytes;
+}
+
 template <typename E>
 int RunToExperts(const void* x, int64_t stride, int64_t dim, const Order& o,
                  void* rows, hipStream_t stream) {
-  SCEMB_LANES(kVec<E>, (ToExperts<E, G, kCut>),
-              static_cast<const E*>(x), stride, static_cast<int32_t>(dim), o,
-              static_cast<E*>(rows))
+  const E* from = static_cast<const E*>(x);
+  E* to = static_cast<E*>(rows);
+  const int32_t d = static_cast<int32_t>(dim);
+  if (PastCache(o, dim, sizeof(E))) {
+    SCEMB_LANES(kVec<E>, (ToExperts<E, G, kCut, true>), from, stride, d, o, to)
+  } else {
+    SCEMB_LANES(kVec<E>, (ToExperts<E, G, kCut, false>), from, stride, d, o,
+                to)
+  }
   return 0;
 }
 
@@ -488,9 +500,16 @@ template <typename T>
 int RunFromExperts(const void* rows, int64_t stride, int64_t dim,
                    const void* weights, bool f32, const Order& o, void* y,
                    hipStream_t stream) {
-  SCEMB_LANES(kVec<T>, (FromExperts<T, G, kCut>),
-              static_cast<const T*>(rows), stride, static_cast<int32_t>(dim),
-              weights, f32, o, static_cast<T*>(y))
+  const T* from = static_cast<const T*>(rows);
+  T* to = static_cast<T*>(y);
+  const int32_t d = static_cast<int32_t>(dim);
+  if (PastCache(o, dim, sizeof(T))) {
+    SCEMB_LANES(kVec<T>, (FromExperts<T, G, kCut, true>), from, stride, d,
+                weights, f32, o, to)
+  } else {
+    SCEMB_LANES(kVec<T>, (FromExperts<T, G, kCut, false>), from, stride, d,
+                weights, f32, o, to)
+  }
   return 0;
 }
 

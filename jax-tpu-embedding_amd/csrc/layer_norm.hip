@@ -264,7 +264,7 @@ __global__ __launch_bounds__(1024) void NormForwardLong(NormArgs<T> a) {
 // the groups of a work-group are added in LDS, in their order, and the
 // work-group's sums go to `partial`. kHold: the weights stay in registers too
 // (where a work-group of 1024 has 16 values a lane there is no room).
-template <typename T, int NV, int G, Cut kCut>
+template <typename T, int NV, int G, Cut kCut, bool kStream>
 __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
   constexpr int V = kVec<T>;
   constexpr int kBlock = BlockOf(G);
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(BlockOf(G)) void NormBackward(NormGradArgs<T> a) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
       if (c < a.dim) {
-        x[i] = LoadSpan<kCut, T, V>(px, At(c, a.dim));
-        dy[i] = LoadSpan<kCut, T, V>(pdy, At(c, a.dim));
+        x[i] = LoadSpan<kCut, T, V, kStream>(px, At(c, a.dim));
+        dy[i] = LoadSpan<kCut, T, V, kStream>(pdy, At(c, a.dim));
       }
     }
     const float mean = a.mean[row];
@@ -573,9 +573,14 @@ int LaunchForward(const NormArgs<T>& a, hipStream_t stream) {
 template <typename T, int NV, int G, Cut kCut>
 int LaunchBackward(const NormGradArgs<T>& a, int64_t parts,
                    hipStream_t stream) {
-  hipLaunchKernelGGL((NormBackward<T, NV, G, kCut>),
-                     dim3(static_cast<uint32_t>(parts)), dim3(BlockOf(G)), 0,
-                     stream, a);
+  const dim3 grid(static_cast<uint32_t>(parts));
+  if (a.rows * a.dim * 3 * static_cast<int64_t>(sizeof(T)) > kCacheBytes) {
+    hipLaunchKernelGGL((NormBackward<T, NV, G, kCut, true>), grid,
+                       dim3(BlockOf(G)), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((NormBackward<T, NV, G, kCut, false>), grid,
+                       dim3(BlockOf(G)), 0, stream, a);
+  }
   SCEMB_LAUNCH_CHECK();
   return 0;
 }
