@@ -21,9 +21,15 @@ constexpr int kTileWaves = 4;        // work-group of a tile
 constexpr int kSingleWaves = 16;     // work-group of a sort in one launch
 constexpr int64_t kTile = 1024;      // ids of a tile, or a multiple of it
 constexpr int64_t kMaxTiles = 4096;  // counts of all tiles are scanned
-// Up to here one work-group sorts by itself, in one launch instead of three
-// (where its counts fit 64 KB of LDS).
+// Up to here one work-group sorts by itself in one launch, where its counts fit
+// 64 KB of LDS (6000 ids 9.1 us against 10.9 in two launches, 8000 10.9 and
+// 11.0, 12,000 14.7 and 10.9).
 constexpr int64_t kSingle = 8192;
+// Counts of all tiles up to which every tile adds them up itself, in two
+// launches instead of three (131,072 ids of 64 experts, 8192 counts: 11.0 us
+// against 13.9; 60,000 of 256, 15,104 counts: 12.9 and 14.2; 300,000 of 64,
+// 18,752 counts: 14.6 and 13.9).
+constexpr int64_t kOwnSumsMost = 16384;
 constexpr int kKeyBits = 11;  // 0..SCEMB_MAX_EXPERTS
 static_assert(SCEMB_MAX_EXPERTS < (1 << kKeyBits), "keys of kKeyBits bits");
 
@@ -136,8 +142,9 @@ __global__ __launch_bounds__(kSingleWaves* kWave) void SortSingle(
              counts + (threadIdx.x / kWave) * row, positions, sources);
 }
 
-// Counts of each tile: hist[key][tile].
-template <typename I>
+// Counts of each tile: hist[tile][key] where the tiles add them up themselves
+// (kOwnSums), hist[key][tile] for ScanTiles.
+template <typename I, bool kOwnSums>
 __global__ __launch_bounds__(kTileWaves* kWave) void CountTiles(
     const I* ids, int64_t n, int32_t experts, int64_t tile, uint32_t* hist) {
   constexpr int kBlock = kTileWaves * kWave;
@@ -152,7 +159,10 @@ __global__ __launch_bounds__(kTileWaves* kWave) void CountTiles(
   }
   __syncthreads();
   for (int i = threadIdx.x; i < row; i += kBlock) {
-    hist[static_cast<int64_t>(i) * gridDim.x + blockIdx.x] = counts[i];
+    const int64_t at = kOwnSums ? static_cast<int64_t>(blockIdx.x) * row + i
+                                : static_cast<int64_t>(i) * gridDim.x +
+                                      blockIdx.x;
+    hist[at] = counts[i];
   }
 }
 
@@ -176,6 +186,18 @@ __global__ __launch_bounds__(256) void ScanTiles(uint32_t* hist, int32_t tiles,
   if (lane == 0) totals[key] = run;
 }
 
+// Turns the counts of a tile's wavefronts for key e into the places of their
+// first choices; `place` is the tile's.
+__device__ __forceinline__ void PlacesOf(uint32_t* counts, int row, int e,
+                                         uint32_t place) {
+#pragma unroll
+  for (int w = 0; w < kTileWaves; ++w) {
+    const uint32_t c = counts[w * row + e];
+    counts[w * row + e] = place;
+    place += c;
+  }
+}
+
 // Places each tile's choices. Every work-group sums the keys' totals itself.
 template <typename I>
 __global__ __launch_bounds__(kTileWaves* kWave) void PlaceTiles(
@@ -193,21 +215,81 @@ __global__ __launch_bounds__(kTileWaves* kWave) void PlaceTiles(
   uint32_t run = 0;
   for (int at = 0; at < row; at += kBlock) {
     const int e = at + threadIdx.x;
-    const uint32_t total = e < row ? totals[e] : 0u;
     uint32_t sum = 0;
     const uint32_t before =
-        run + BlockExclusiveScan<uint32_t, kBlock>(total, scan, &sum);
+        run + BlockExclusiveScan<uint32_t, kBlock>(e < row ? totals[e] : 0u,
+                                                   scan, &sum);
     run += sum;
     if (e < row) {
       if (blockIdx.x == 0) offsets[e] = static_cast<int32_t>(before);
-      uint32_t place =
-          before + hist[static_cast<int64_t>(e) * gridDim.x + blockIdx.x];
-      for (int w = 0; w < kTileWaves; ++w) {
-        const uint32_t c = counts[w * row + e];
-        counts[w * row + e] = place;
-        place += c;
+      PlacesOf(counts, row, e,
+               before +
+                   hist[static_cast<int64_t>(e) * gridDim.x + blockIdx.x]);
+    }
+  }
+  __syncthreads();
+  PlaceShare(ids, experts, s.first, s.last,
+             counts + (threadIdx.x / kWave) * row, positions, sources);
+}
+
+// The same without ScanTiles: every work-group adds up the counts of all tiles
+// itself, 2^lanes_log threads (at least the experts) a slice of the tiles. The
+// dropped choices before a tile are those that are left.
+template <typename I>
+__global__ __launch_bounds__(kTileWaves* kWave) void SumAndPlaceTiles(
+    const I* ids, int64_t n, int32_t experts, int32_t lanes_log, int64_t tile,
+    const uint32_t* hist, int32_t* positions, int32_t* sources,
+    int32_t* offsets) {
+  constexpr int kBlock = kTileWaves * kWave;
+  extern __shared__ uint32_t counts[];
+  __shared__ uint32_t scan[kTileWaves + 1];
+  __shared__ uint32_t before_of[kBlock], total_of[kBlock];
+  const int row = experts + 1;
+  const int64_t begin = blockIdx.x * tile;
+  const int64_t end = begin + tile < n ? begin + tile : n;
+  const Share s = ShareOf<kTileWaves>(begin, end);
+  const int e = threadIdx.x & ((1 << lanes_log) - 1);
+  const uint32_t slices = kBlock >> lanes_log;
+  uint32_t before = 0, total = 0;
+  if (e < experts) {
+    constexpr int kLoads = 8;  // in flight
+    for (uint32_t t = threadIdx.x >> lanes_log; t < gridDim.x;
+         t += kLoads * slices) {
+      uint32_t c[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t u = t + i * slices;
+        c[i] = u < gridDim.x ? hist[u * row + e] : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        total += c[i];
+        before += t + i * slices < blockIdx.x ? c[i] : 0u;
       }
     }
+  }
+  before_of[threadIdx.x] = before;
+  total_of[threadIdx.x] = total;
+  CountShares<I, kTileWaves>(ids, experts, s.first, s.last, counts);
+  before = total = 0;
+  if (threadIdx.x < experts) {
+    for (int i = threadIdx.x; i < kBlock; i += 1 << lanes_log) {
+      before += before_of[i];
+      total += total_of[i];
+    }
+  }
+  uint32_t kept = 0, kept_before = 0;
+  const uint32_t first =
+      BlockExclusiveScan<uint32_t, kBlock>(total, scan, &kept);
+  BlockExclusiveScan<uint32_t, kBlock>(before, scan, &kept_before);
+  if (threadIdx.x < experts) {
+    if (blockIdx.x == 0) offsets[threadIdx.x] = static_cast<int32_t>(first);
+    PlacesOf(counts, row, threadIdx.x, first + before);
+  }
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) offsets[experts] = static_cast<int32_t>(kept);
+    PlacesOf(counts, row, experts,
+             kept + static_cast<uint32_t>(begin) - kept_before);
   }
   __syncthreads();
   PlaceShare(ids, experts, s.first, s.last,
@@ -251,14 +333,27 @@ int Sort(const void* ids, int64_t n, int32_t experts, int32_t* positions,
     return Fail(SCEMB_ERR_WORKSPACE,
                 "sort by expert: workspace missing or too small");
   }
-  hipLaunchKernelGGL(CountTiles<I>, dim3(tiles), dim3(kTileWaves * kWave), row,
-                     stream, in, n, experts, tile, hist);
+  const dim3 block(kTileWaves * kWave);
+  const int lanes_log = BitWidth(experts - 1);
+  if ((1 << lanes_log) <= kTileWaves * kWave &&
+      (static_cast<int64_t>(tiles) << lanes_log) <= kOwnSumsMost) {
+    hipLaunchKernelGGL((CountTiles<I, true>), dim3(tiles), block, row, stream,
+                       in, n, experts, tile, hist);
+    SCEMB_LAUNCH_CHECK();
+    hipLaunchKernelGGL(SumAndPlaceTiles<I>, dim3(tiles), block,
+                       kTileWaves * row, stream, in, n, experts, lanes_log, tile,
+                       hist, positions, sources, offsets);
+    SCEMB_LAUNCH_CHECK();
+    return 0;
+  }
+  hipLaunchKernelGGL((CountTiles<I, false>), dim3(tiles), block, row, stream,
+                     in, n, experts, tile, hist);
   SCEMB_LAUNCH_CHECK();
   hipLaunchKernelGGL(ScanTiles, dim3((experts + 4) / 4), dim3(256), 0, stream,
                      hist, static_cast<int32_t>(tiles), experts + 1, totals);
   SCEMB_LAUNCH_CHECK();
-  hipLaunchKernelGGL(PlaceTiles<I>, dim3(tiles), dim3(kTileWaves * kWave),
-                     kTileWaves * row, stream, in, n, experts, tile, hist,
+  hipLaunchKernelGGL(PlaceTiles<I>, dim3(tiles), block, kTileWaves * row,
+                     stream, in, n, experts, tile, hist,
                      totals, positions, sources, offsets);
   SCEMB_LAUNCH_CHECK();
   return 0;

@@ -289,6 +289,34 @@ def test_not_finite_gradients(bits):
   assert not m[300].isfinite() and not v[301].isfinite()
 
 
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32),
+                                   (torch.float32, torch.bfloat16),
+                                   (torch.bfloat16, torch.bfloat16)], ids=str)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_than_the_caches(bits, types):
+  """Steps of more than 256 MB go past the caches: the same bits as in parts."""
+  ptype, gtype = types
+  n, parts = 64_000_513, 8
+  p = _tensors([n], ptype, 1)[0]
+  g = _tensors([n], gtype, 2)[0]
+  step = 8_000_000
+  assert step % 256 == 0 and step * parts < n
+  q = p.clone()
+  cuts = [slice(i * step, (i + 1) * step if i < parts else n)
+          for i in range(parts + 1)]
+  copy = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+  whole = dense.init_adamw_state([p], state_bits=bits)
+  states = [dense.init_adamw_state([q[c]], state_bits=bits) for c in cuts]
+  for _ in range(2):
+    dense.adamw_update([p], [g], whole, copies=[copy], **HYPER)
+    for c, s in zip(cuts, states):
+      dense.adamw_update([q[c]], [g[c]], s, **HYPER)
+  assert torch.equal(p, q) and torch.equal(copy, p.bfloat16())
+  for name in ("m", "v") + (("m_scale", "v_scale") if bits == 8 else ()):
+    assert torch.equal(getattr(whole, name),
+                       torch.cat([getattr(s, name) for s in states])), name
+
+
 def test_large_tensor():
   """More than 2^31 bytes in one tensor, checked at both ends."""
   n = 600_000_007

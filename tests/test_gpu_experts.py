@@ -274,6 +274,28 @@ def test_offsets_past_32_bits():
   assert torch.allclose(dw.double(), exact, rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.parametrize("dim", [1024, 1023])
+def test_more_than_the_caches(dim):
+  """Calls of more than 256 MB read their rows past the caches."""
+  tokens = 50000
+  order, x, rows, _, weights = _case(tokens, 2, 16, dim, torch.bfloat16,
+                                     dropped=0.05)
+  got = dense.tokens_to_experts(x, order)
+  expected = x[order.sources.long() // 2]
+  expected[int(order.offsets[-1]):] = 0
+  assert torch.equal(got, expected)
+  y = dense.tokens_from_experts(rows, weights, order)
+  for at in range(0, tokens, 10000):
+    part = dense.ExpertOrder(order.positions[at:at + 10000], None,
+                             order.offsets)
+    picked, kept = _picked(rows, part)
+    parts = picked * torch.where(kept, weights[at:at + 10000].double(),
+                                 0.0).unsqueeze(2)
+    exact = parts.sum(1)
+    tol = ROUND[torch.bfloat16] * exact.abs() + 3 * U * parts.abs().sum(1)
+    assert ((y[at:at + 10000].double() - exact).abs() <= tol).all()
+
+
 def test_refusals():
   order, x, rows, dy, weights = _case(20, 2, 4, 16, torch.float32)
   ids = torch.zeros((20, 2), dtype=torch.int64, device="cuda")

@@ -257,6 +257,32 @@ def test_many_rows_and_offsets_past_32_bits():
   _check_backward(values, w, dy, mean, rstd, got)
 
 
+@pytest.mark.parametrize("dim", [1024, 1001])
+def test_more_than_the_caches(dim):
+  """Calls of more than 256 MB read their rows past the caches: the same bits
+  as calls on parts of the rows, and sums over all of them."""
+  rows = 50000
+  x, w, b, dy = _inputs(rows, dim, torch.bfloat16)
+  y, mean, rstd = dense.layer_norm(x, w, b, epsilon=EPS, return_stats=True)
+  dx, dw, db = dense.layer_norm_grad(dy, x, mean, rstd, w)
+  sums = torch.zeros((2, dim), dtype=torch.float64, device="cuda")
+  size = torch.zeros((2, dim), dtype=torch.float64, device="cuda")
+  for at in range(0, rows, 10000):
+    cut = slice(at, at + 10000)
+    part = dense.layer_norm(x[cut], w, b, epsilon=EPS)
+    assert torch.equal(part, y[cut])
+    part = dense.layer_norm_grad(dy[cut], x[cut], mean[cut], rstd[cut], w)
+    assert torch.equal(part[0], dx[cut])
+    xhat = (x[cut].double() - mean[cut, None].double()) * rstd[cut, None].double()
+    for i, v in enumerate((dy[cut].double() * xhat, dy[cut].double())):
+      sums[i] += v.sum(0)
+      size[i] += v.abs().sum(0)
+  # A lane adds a row at a time, 3 work-groups of 4 rows a CU: 17 rows of it,
+  # then 4 and 768 / 32 sums; and xhat is off by 4 u (|x| + |mean|) rstd < 32 u.
+  assert ((dw - sums[0]).abs() <= 64 * U * size[0] + 32 * U * size[1]).all()
+  assert ((db - sums[1]).abs() <= 64 * U * size[1]).all()
+
+
 def test_refusals():
   x, w, b, dy = _inputs(4, 16, torch.bfloat16)
   y, mean, rstd = dense.layer_norm(x, w, b, return_stats=True)
