@@ -661,7 +661,8 @@ int scemb_layer_norm_grad(const void* y_grad, int64_t y_grad_stride,
  * own order. ids (id_bytes 4: int32, 8: int64) outside [0, num_experts) are
  * dropped choices and go to the end. positions[i] is choice i's place,
  * sources[p] the choice at place p, offsets[e] the first place of expert e
- * (offsets[num_experts]: the number of choices that are not dropped). */
+ * (offsets[num_experts]: the number of choices that are not dropped). The
+ * workspace size is 0 where none is needed (and for what the call refuses). */
 #define SCEMB_MAX_EXPERTS 1024
 size_t scemb_sort_by_expert_workspace_size(int64_t n, int32_t num_experts);
 int scemb_sort_by_expert(const void* ids, int32_t id_bytes, int64_t n,

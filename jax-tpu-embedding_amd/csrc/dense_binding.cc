@@ -195,9 +195,10 @@ PyObject* Tuple(std::initializer_list<Tensor> tensors) {
 
 // A workspace of at least `bytes`, from the caller's function of a size.
 void* Workspace(PyObject* get, size_t bytes) {
-  if (bytes == 0) Refuse(lib.last_error());
-  PyObject* o = PyObject_CallFunction(
-      get, "n", static_cast<Py_ssize_t>(bytes));
+  PyObject* size = PyLong_FromSize_t(bytes);
+  if (size == nullptr) throw Raised();
+  PyObject* o = PyObject_CallOneArg(get, size);
+  Py_DECREF(size);
   if (o == nullptr) throw Raised();
   // The pool keeps it.
   void* p = THPVariable_Check(o) ? THPVariable_Unpack(o).data_ptr() : nullptr;
@@ -313,6 +314,7 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     size_t bytes = 0;
     if (dw.defined() || db.defined()) {
       bytes = lib.layer_norm_grad_workspace(code, r.n, dim);
+      if (bytes == 0) Check(SCEMB_ERR_INVALID_ARGUMENT);
       ws = Workspace(a[8], bytes);
     }
     Check(lib.layer_norm_grad(
@@ -353,7 +355,7 @@ PyObject* SortByExpert(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor offsets = New({experts + 1}, at::kInt, ids);
     const int32_t e = static_cast<int32_t>(experts);
     const size_t bytes = lib.sort_by_expert_workspace(count, e);
-    void* ws = Workspace(a[2], bytes);
+    void* ws = bytes > 0 ? Workspace(a[2], bytes) : nullptr;
     Check(lib.sort_by_expert(
         in.data_ptr(), static_cast<int32_t>(in.element_size()), count, e,
         static_cast<int32_t*>(positions.data_ptr()),

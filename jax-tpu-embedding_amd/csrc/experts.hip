@@ -63,9 +63,10 @@ __device__ __forceinline__ void CountShares(const I* ids, int32_t experts,
 // Places a wavefront's share: next[key] is the place of its next choice of
 // that key. 64 choices at a time, equal keys ranked by lane.
 template <typename I>
-__device__ __forceinline__ void PlaceShare(const I* ids, int32_t experts,
-                                           int64_t first, int64_t last,
-                                           uint32_t* next, int32_t* positions,
+__device__ __forceinline__ void PlaceShare(const I* ids, int64_t n,
+                                           int32_t experts, int64_t first,
+                                           int64_t last, uint32_t* next,
+                                           int32_t* positions,
                                            int32_t* sources) {
   const int lane = threadIdx.x % kWave;
   for (int64_t at = first; at < last; at += kWave) {
@@ -83,7 +84,8 @@ __device__ __forceinline__ void PlaceShare(const I* ids, int32_t experts,
     if (in) {
       const uint32_t place = base + __popcll(same & LaneMaskLt());
       positions[i] = static_cast<int32_t>(place);
-      sources[place] = static_cast<int32_t>(i);
+      // Always, unless the ids changed since they were counted.
+      if (place < n) sources[place] = static_cast<int32_t>(i);
     }
   }
 }
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(kSingleWaves* kWave) void SortSingle(
     }
   }
   __syncthreads();
-  PlaceShare(ids, experts, s.first, s.last,
+  PlaceShare(ids, n, experts, s.first, s.last,
              counts + (threadIdx.x / kWave) * row, positions, sources);
 }
 
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(kTileWaves* kWave) void PlaceTiles(
     }
   }
   __syncthreads();
-  PlaceShare(ids, experts, s.first, s.last,
+  PlaceShare(ids, n, experts, s.first, s.last,
              counts + (threadIdx.x / kWave) * row, positions, sources);
 }
 
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(kTileWaves* kWave) void SumAndPlaceTiles(
              kept + static_cast<uint32_t>(begin) - kept_before);
   }
   __syncthreads();
-  PlaceShare(ids, experts, s.first, s.last,
+  PlaceShare(ids, n, experts, s.first, s.last,
              counts + (threadIdx.x / kWave) * row, positions, sources);
 }
 
@@ -371,11 +373,11 @@ struct Order {
   int64_t tokens;
   int32_t choices;
 
-  // Choices that are kept, at most as many as there are.
+  // Choices that are kept, within what there are whatever the order says.
   __device__ __forceinline__ uint32_t Kept() const {
     const int64_t n = tokens * choices;
     const int64_t k = *kept;
-    return static_cast<uint32_t>(k < n ? k : n);
+    return static_cast<uint32_t>(k < 0 ? 0 : k < n ? k : n);
   }
 };
 
@@ -629,14 +631,13 @@ size_t scemb_sort_by_expert_workspace_size(int64_t n, int32_t num_experts) {
   using namespace scemb;
   if (n < 0 || n > 0x7fffffff || num_experts < 1 ||
       num_experts > SCEMB_MAX_EXPERTS) {
-    SetError("sort by expert: choices or experts out of range");
     return 0;
   }
   Arena arena(nullptr, 0);
   if (!SortsSingle(n, num_experts)) {
     arena.Take<uint32_t>((num_experts + 1) * TilesOf(n));
+    arena.Take<uint32_t>(num_experts + 1);
   }
-  arena.Take<uint32_t>(num_experts + 1);
   return arena.used();
 }
 

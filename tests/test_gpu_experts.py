@@ -212,8 +212,16 @@ def test_wrong_positions_are_dropped():
   assert dw[3, 1] == 0 and dw[4, 0] == 0 and lost >= 0
   many = order.offsets.clone()
   many[-1] = 2**31 - 1
-  dense.tokens_from_experts(
-      rows, weights, dense.ExpertOrder(order.positions, order.sources, many))
+  got = dense.tokens_from_experts(rows, weights,
+                                  dense.ExpertOrder(pos, None, many))
+  assert torch.equal(got, dense.tokens_from_experts(rows, weights, bad))
+  # No choices are kept, by a count that no sort gives either.
+  many[-1] = -3
+  none = dense.ExpertOrder(order.positions, order.sources, many)
+  assert (dense.tokens_from_experts(rows, weights, none) == 0).all()
+  assert (dense.tokens_to_experts(x, none) == 0).all()
+  drows, dw = dense.tokens_from_experts_grad(dy, rows, weights, none)
+  assert (drows == 0).all() and (dw == 0).all()
 
 
 def test_autograd_and_differences():
