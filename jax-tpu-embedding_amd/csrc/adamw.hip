@@ -1,7 +1,7 @@
 // AdamW over many tensors at once, with moments in float32 or in 8 bits.
 //
-// One launch takes up to kMaxTensors tensors, whose addresses travel in the
-// kernel arguments; a work-group has kStep consecutive values of one of them.
+// One launch takes up to 104 tensors, whose addresses travel in the kernel
+// arguments; a work-group has kStep consecutive values of one of them.
 // The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
 // bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy.
 //
@@ -25,19 +25,24 @@ constexpr int kThreads = 256;
 constexpr int kPer = 4;                    // consecutive values of a lane
 constexpr int kStep = kThreads * kPer;     // values of a work-group
 constexpr int kQuant = SCEMB_ADAMW_BLOCK;  // values that share a scale
-constexpr int kMaxTensors = 64;            // a launch: a tensor a lane
 static_assert(kQuant == kWave * kPer, "a block is one step of a wavefront");
 
 struct Tensor {
   void* param;
   const void* grad;
-  void* copy;
-  int64_t numel;
+  uint64_t numel : 48;
+  uint64_t param_bf16 : 1;
+  uint64_t grad_bf16 : 1;
+  uint64_t decay : 1;
   uint32_t block;  // its first block of moments
-  uint8_t param_bf16;
-  uint8_t grad_bf16;
-  uint8_t decay;
+  uint32_t first;  // its first work-group
 };
+static_assert(sizeof(Tensor) == 32, "four words");
+
+// Tensors of a launch: what the kernel's arguments hold, two lanes' worth at
+// most (a launch of 64 small tensors takes 5 us, and so does one of 104).
+template <bool kCopies>
+constexpr int kMaxTensors = kCopies ? 83 : 104;
 
 struct Moments {
   void* m;
@@ -59,9 +64,15 @@ struct Factors {
   float keep;    // 1 - learning_rate * weight_decay
 };
 
-struct AdamArgs {
-  uint32_t first[kMaxTensors];  // first work-group of each tensor
-  Tensor tensors[kMaxTensors];
+template <bool kCopies>
+struct Tensors {
+  Tensor tensors[kMaxTensors<kCopies>];
+  // Every tensor's bfloat16 copy (NULL: none).
+  void* copies[kCopies ? kMaxTensors<kCopies> : 1];
+};
+
+template <bool kCopies>
+struct AdamArgs : Tensors<kCopies> {
   Moments moments;
   Factors factors;
   // Device scalars and what the factors are then made of.
@@ -75,7 +86,8 @@ struct AdamArgs {
   int64_t step;
   int32_t n;
 };
-static_assert(sizeof(AdamArgs) <= 3584,
+static_assert(sizeof(AdamArgs<false>) <= 3584 &&
+                  sizeof(AdamArgs<true>) <= 3584,
               "the arguments must fit the kernel argument block");
 
 __host__ __device__ inline void SetRates(double learning_rate, double beta_1,
@@ -182,10 +194,11 @@ __device__ __forceinline__ void Roots(const float (&v)[kPer],
 
 // A work-group's values of one tensor: kStep from `begin` on.
 template <int kBits, typename P, typename G, bool kStream>
-__device__ __forceinline__ void UpdateStep(const Tensor& t, const Moments& s,
-                                           const Factors& f, int64_t begin) {
+__device__ __forceinline__ void UpdateStep(const Tensor& t, bf16* copy,
+                                           const Moments& s, const Factors& f,
+                                           int64_t begin) {
   const int64_t at = begin + threadIdx.x * kPer;
-  const int64_t left = t.numel - at;
+  const int64_t left = static_cast<int64_t>(t.numel) - at;
   // The wavefront's block of 256 values: all of its lanes go on, or none.
   if (left + (threadIdx.x % kWave) * kPer <= 0) return;
   const int count = left < 0 ? 0 : left < kPer ? static_cast<int>(left) : kPer;
@@ -224,9 +237,7 @@ __device__ __forceinline__ void UpdateStep(const Tensor& t, const Moments& s,
            m[j] * __builtin_amdgcn_rcpf(r[j] * f.root + f.epsilon) * f.rate;
   }
   Store4<P, kStream>(static_cast<P*>(t.param) + at, count, p);
-  if (t.copy != nullptr) {
-    Store4<bf16, kStream>(static_cast<bf16*>(t.copy) + at, count, p);
-  }
+  if (copy != nullptr) Store4<bf16, kStream>(copy + at, count, p);
   if constexpr (kBits == 8) {
     // Codes past the tensor's end are zeros and stay so.
     if (count < kPer) {
@@ -292,13 +303,18 @@ __device__ __forceinline__ void UpdateStep(const Tensor& t, const Moments& s,
   }
 }
 
-template <int kBits, bool kStream>
-__global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs a) {
-  const int lane = threadIdx.x % kWave;
-  const uint64_t before =
-      __ballot(lane < a.n && a.first[lane] <= blockIdx.x);
-  const int i = __builtin_amdgcn_readfirstlane(__popcll(before) - 1);
+template <int kBits, bool kStream, bool kCopies>
+__global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs<kCopies> a) {
+  static_assert(kMaxTensors<kCopies> <= 2 * kWave, "two tensors a lane");
+  int i = -1;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int at = threadIdx.x % kWave + k * kWave;
+    i += __popcll(__ballot(at < a.n && a.tensors[at].first <= blockIdx.x));
+  }
+  i = __builtin_amdgcn_readfirstlane(i);
   const Tensor t = a.tensors[i];
+  bf16* copy = kCopies ? static_cast<bf16*>(a.copies[i]) : nullptr;
   Factors f = a.factors;
   if (a.learning_rate_ptr != nullptr || a.step_ptr != nullptr) {
     SetRates(a.learning_rate_ptr != nullptr
@@ -308,18 +324,17 @@ __global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs a) {
              a.step_ptr != nullptr ? *a.step_ptr : a.step, &f);
   }
   if (a.grad_scale_ptr != nullptr) f.grad_scale = *a.grad_scale_ptr;
-  const int64_t begin =
-      static_cast<int64_t>(blockIdx.x - a.first[i]) * kStep;
+  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.first) * kStep;
   if (t.param_bf16) {
     if (t.grad_bf16) {
-      UpdateStep<kBits, bf16, bf16, kStream>(t, a.moments, f, begin);
+      UpdateStep<kBits, bf16, bf16, kStream>(t, copy, a.moments, f, begin);
     } else {
-      UpdateStep<kBits, bf16, float, kStream>(t, a.moments, f, begin);
+      UpdateStep<kBits, bf16, float, kStream>(t, copy, a.moments, f, begin);
     }
   } else if (t.grad_bf16) {
-    UpdateStep<kBits, float, bf16, kStream>(t, a.moments, f, begin);
+    UpdateStep<kBits, float, bf16, kStream>(t, copy, a.moments, f, begin);
   } else {
-    UpdateStep<kBits, float, float, kStream>(t, a.moments, f, begin);
+    UpdateStep<kBits, float, float, kStream>(t, copy, a.moments, f, begin);
   }
 }
 
@@ -380,18 +395,79 @@ int CheckTensor(const scemb_adamw_tensor_t& t, int32_t i) {
   return 0;
 }
 
-template <int kBits>
-int LaunchUpdate(const AdamArgs& a, uint32_t groups, bool stream_data,
+template <int kBits, bool kCopies>
+int LaunchUpdate(const AdamArgs<kCopies>& a, uint32_t groups, bool past_cache,
                  hipStream_t stream) {
-  if (stream_data) {
-    hipLaunchKernelGGL((AdamUpdate<kBits, true>), dim3(groups), dim3(kThreads),
-                       0, stream, a);
+  if (past_cache) {
+    hipLaunchKernelGGL((AdamUpdate<kBits, true, kCopies>), dim3(groups),
+                       dim3(kThreads), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((AdamUpdate<kBits, false>), dim3(groups),
+    hipLaunchKernelGGL((AdamUpdate<kBits, false, kCopies>), dim3(groups),
                        dim3(kThreads), 0, stream, a);
   }
   SCEMB_LAUNCH_CHECK();
   return 0;
+}
+
+// Launches of up to kMaxTensors tensors with a gradient each.
+template <bool kCopies>
+int UpdateAll(const scemb_adamw_tensor_t* tensors, int32_t num_tensors,
+              const scemb_adamw_state_t& state,
+              const scemb_adamw_options_t& o, bool past_cache,
+              hipStream_t stream) {
+  AdamArgs<kCopies> a;
+  a.moments = {state.m, state.v, state.m_scale, state.v_scale};
+  a.factors.grad_scale = static_cast<float>(o.grad_scale);
+  a.factors.beta_1 = static_cast<float>(o.beta_1);
+  a.factors.gain_1 = static_cast<float>(1.0 - o.beta_1);
+  a.factors.beta_2 = static_cast<float>(o.beta_2);
+  a.factors.gain_2 = static_cast<float>(1.0 - o.beta_2);
+  a.factors.epsilon = static_cast<float>(o.epsilon);
+  SetRates(o.learning_rate, o.beta_1, o.beta_2, o.weight_decay, o.step,
+           &a.factors);
+  a.learning_rate_ptr = o.learning_rate_ptr;
+  a.step_ptr = o.step_ptr;
+  a.grad_scale_ptr = o.grad_scale_ptr;
+  a.learning_rate = o.learning_rate;
+  a.beta_1 = o.beta_1;
+  a.beta_2 = o.beta_2;
+  a.weight_decay = o.weight_decay;
+  a.step = o.step;
+  a.n = 0;
+  uint32_t block = 0;
+  int64_t groups = 0;
+  const auto launch = [&]() {
+    const uint32_t n = static_cast<uint32_t>(groups);
+    return state.bits == 8
+               ? LaunchUpdate<8, kCopies>(a, n, past_cache, stream)
+               : LaunchUpdate<32, kCopies>(a, n, past_cache, stream);
+  };
+  for (int32_t i = 0; i < num_tensors; ++i) {
+    const scemb_adamw_tensor_t& t = tensors[i];
+    if (t.grad != nullptr && t.numel > 0) {
+      const int64_t mine = CeilDiv(t.numel, kStep);
+      if (a.n == kMaxTensors<kCopies> || groups + mine > 0x7fffffff) {
+        const int rc = launch();
+        if (rc != 0) return rc;
+        a.n = 0;
+        groups = 0;
+      }
+      Tensor& d = a.tensors[a.n];
+      d.param = t.param;
+      d.grad = t.grad;
+      d.numel = static_cast<uint64_t>(t.numel);
+      d.param_bf16 = t.param_type == SCEMB_BF16;
+      d.grad_bf16 = t.grad_type == SCEMB_BF16;
+      d.decay = t.decay != 0;
+      d.block = block;
+      d.first = static_cast<uint32_t>(groups);
+      if constexpr (kCopies) a.copies[a.n] = t.copy;
+      ++a.n;
+      groups += mine;
+    }
+    block += static_cast<uint32_t>(CeilDiv(t.numel, kQuant));
+  }
+  return a.n == 0 ? 0 : launch();
 }
 
 }  // namespace
@@ -412,78 +488,31 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
                 "adamw: tensors or options missing, or a step below 1");
   }
   int64_t blocks = 0, bytes = 0;
+  bool copies = false;
   for (int32_t i = 0; i < num_tensors; ++i) {
     const scemb_adamw_tensor_t& t = tensors[i];
     const int rc = CheckTensor(t, i);
     if (rc != 0) return rc;
-    blocks += CeilDiv(t.numel, kQuant);
+    blocks += CeilDiv(std::min(t.numel, state->size + 1), kQuant);
     if (t.grad != nullptr) {
       bytes += t.numel * (TypeBytes(t.param_type) + TypeBytes(t.grad_type) +
                           (t.copy != nullptr ? 2 : 0) + state->bits / 4);
+      copies = copies || t.copy != nullptr;
     }
   }
   if (blocks * kQuant > state->size) {
     return Fail(SCEMB_ERR_INVALID_ARGUMENT,
                 "adamw: the state is smaller than the tensors");
   }
-  AdamArgs a;
-  a.moments = {state->m, state->v, state->m_scale, state->v_scale};
-  a.factors.grad_scale = static_cast<float>(options->grad_scale);
-  a.factors.beta_1 = static_cast<float>(options->beta_1);
-  a.factors.gain_1 = static_cast<float>(1.0 - options->beta_1);
-  a.factors.beta_2 = static_cast<float>(options->beta_2);
-  a.factors.gain_2 = static_cast<float>(1.0 - options->beta_2);
-  a.factors.epsilon = static_cast<float>(options->epsilon);
-  SetRates(options->learning_rate, options->beta_1, options->beta_2,
-           options->weight_decay, options->step, &a.factors);
-  a.learning_rate_ptr = options->learning_rate_ptr;
-  a.step_ptr = options->step_ptr;
-  a.grad_scale_ptr = options->grad_scale_ptr;
-  a.learning_rate = options->learning_rate;
-  a.beta_1 = options->beta_1;
-  a.beta_2 = options->beta_2;
-  a.weight_decay = options->weight_decay;
-  a.step = options->step;
-  a.n = 0;
-  uint32_t block = 0;
-  int64_t groups = 0;
+  // Read and written past the caches where they cannot hold it until the next
+  // step: 176M float32 values 915 us through them, 829 past them; 79M with
+  // 8-bit moments (whose codes stay) 255 and 212; but 4.9M values 22 and 24.
+  const bool past_cache = bytes > kCacheBytes;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto launch = [&]() {
-    const uint32_t n = static_cast<uint32_t>(groups);
-    // Read and written past the caches where they cannot hold it until the
-    // next step: 176M float32 values 915 us through them, 829 past them; 79M
-    // with 8-bit moments (whose codes stay) 255 and 212; but 4.9M values 22 and
-    // 24.
-    const bool past = bytes > kCacheBytes;
-    return state->bits == 8 ? LaunchUpdate<8>(a, n, past, s)
-                            : LaunchUpdate<32>(a, n, past, s);
-  };
-  for (int32_t i = 0; i < num_tensors; ++i) {
-    const scemb_adamw_tensor_t& t = tensors[i];
-    if (t.grad != nullptr && t.numel > 0) {
-      const int64_t mine = CeilDiv(t.numel, kStep);
-      if (a.n == kMaxTensors || groups + mine > 0x7fffffff) {
-        const int rc = launch();
-        if (rc != 0) return rc;
-        a.n = 0;
-        groups = 0;
-      }
-      Tensor& d = a.tensors[a.n];
-      a.first[a.n] = static_cast<uint32_t>(groups);
-      d.param = t.param;
-      d.grad = t.grad;
-      d.copy = t.copy;
-      d.numel = t.numel;
-      d.block = block;
-      d.param_bf16 = t.param_type == SCEMB_BF16;
-      d.grad_bf16 = t.grad_type == SCEMB_BF16;
-      d.decay = t.decay != 0;
-      ++a.n;
-      groups += mine;
-    }
-    block += static_cast<uint32_t>(CeilDiv(t.numel, kQuant));
-  }
-  return a.n == 0 ? SCEMB_OK : launch();
+  return copies ? UpdateAll<true>(tensors, num_tensors, *state, *options,
+                                  past_cache, s)
+                : UpdateAll<false>(tensors, num_tensors, *state, *options,
+                                   past_cache, s);
 }
 
 int scemb_adamw_moments(const scemb_adamw_state_t* state, float* m, float* v,

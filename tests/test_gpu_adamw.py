@@ -231,6 +231,33 @@ def test_many_tensors(bits):
   assert torch.equal(together[0], _tensors(sizes, torch.float32, 6)[0])
 
 
+@pytest.mark.parametrize("count", [63, 64, 65, 83, 84, 104, 105, 129, 209])
+def test_numbers_of_tensors(count):
+  """On both sides of what a launch and a lane take, with and without copies,
+  against one tensor that holds them all."""
+  sizes = [256 * (1 + i % 5) for i in range(count)]
+  for with_copies in (False, True):
+    flat, grad = _tensors([sum(sizes)], torch.float32, 1)[0], _tensors(
+        [sum(sizes)], torch.bfloat16, 2)[0]
+    other = flat.clone()
+    copy = torch.zeros_like(grad)
+    params, grads, copies = (list(x.split(sizes)) for x in (flat, grad, copy))
+    if with_copies:
+      copies[count // 2] = None
+    state = dense.init_adamw_state(params, state_bits=8)
+    one = dense.init_adamw_state([other], state_bits=8)
+    dense.adamw_update(params, grads, state, **HYPER,
+                       copies=copies if with_copies else None)
+    dense.adamw_update([other], [grad], one, **HYPER)
+    assert torch.equal(flat, other)
+    for name in ("m", "v", "m_scale", "v_scale"):
+      assert torch.equal(getattr(state, name), getattr(one, name))
+    for i, c in enumerate(copy.split(sizes)):
+      written = with_copies and i != count // 2
+      assert torch.equal(c, params[i].bfloat16() if written else
+                         torch.zeros_like(c))
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_hyperparameters_on_the_gpu(bits):
   """Device scalars give what host values give; their factors are made in 64
