@@ -197,23 +197,28 @@ template <int kBits, typename P, typename G, bool kStream>
 __device__ __forceinline__ void UpdateStep(const Tensor& t, bf16* copy,
                                            const Moments& s, const Factors& f,
                                            int64_t begin) {
-  const int64_t at = begin + threadIdx.x * kPer;
-  const int64_t left = static_cast<int64_t>(t.numel) - at;
+  // The work-group's part is uniform: lanes only add 32-bit offsets to it.
+  const int64_t slot = static_cast<int64_t>(t.block) * kQuant + begin;
+  const int64_t left = static_cast<int64_t>(t.numel) - begin;
+  const int here = left < kStep ? static_cast<int>(left) : kStep;
+  const uint32_t own = threadIdx.x * kPer;
   // The wavefront's block of 256 values: all of its lanes go on, or none.
-  if (left + (threadIdx.x % kWave) * kPer <= 0) return;
-  const int count = left < 0 ? 0 : left < kPer ? static_cast<int>(left) : kPer;
-  const int64_t slot = static_cast<int64_t>(t.block) * kQuant + at;
+  const uint32_t block =
+      __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (static_cast<int>(block) * kQuant >= here) return;
+  const int count = min(max(here - static_cast<int>(own), 0), kPer);
+  P* param = static_cast<P*>(t.param) + begin;
   const float keep = t.decay ? f.keep : 1.f;
   float p[kPer], g[kPer], m[kPer], v[kPer], r[kPer];
-  Load4<P, kStream>(static_cast<const P*>(t.param) + at, count, p);
-  Load4<G, kStream>(static_cast<const G*>(t.grad) + at, count, g);
+  Load4<P, kStream>(param + own, count, p);
+  Load4<G, kStream>(static_cast<const G*>(t.grad) + begin + own, count, g);
   if constexpr (kBits == 8) {
     const auto qm =
-        LoadVec<int8_t, kPer>(static_cast<const int8_t*>(s.m) + slot);
+        LoadVec<int8_t, kPer>(static_cast<const int8_t*>(s.m) + slot + own);
     const auto qv =
-        LoadVec<uint8_t, kPer>(static_cast<const uint8_t*>(s.v) + slot);
-    const float ms = s.m_scale[slot / kQuant];
-    const float vs = s.v_scale[slot / kQuant];
+        LoadVec<uint8_t, kPer>(static_cast<const uint8_t*>(s.v) + slot + own);
+    const float ms = s.m_scale[slot / kQuant + block];
+    const float vs = s.v_scale[slot / kQuant + block];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       m[j] = DecodeM(qm.v[j], ms);
@@ -221,8 +226,10 @@ __device__ __forceinline__ void UpdateStep(const Tensor& t, bf16* copy,
       v[j] = root * root;
     }
   } else {
-    Load4<float, kStream>(static_cast<const float*>(s.m) + slot, kPer, m);
-    Load4<float, kStream>(static_cast<const float*>(s.v) + slot, kPer, v);
+    Load4<float, kStream>(static_cast<const float*>(s.m) + slot + own, kPer,
+                          m);
+    Load4<float, kStream>(static_cast<const float*>(s.v) + slot + own, kPer,
+                          v);
   }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -236,8 +243,8 @@ __device__ __forceinline__ void UpdateStep(const Tensor& t, bf16* copy,
     p[j] = p[j] * keep -
            m[j] * __builtin_amdgcn_rcpf(r[j] * f.root + f.epsilon) * f.rate;
   }
-  Store4<P, kStream>(static_cast<P*>(t.param) + at, count, p);
-  if (copy != nullptr) Store4<bf16, kStream>(copy + at, count, p);
+  Store4<P, kStream>(param + own, count, p);
+  if (copy != nullptr) Store4<bf16, kStream>(copy + begin + own, count, p);
   if constexpr (kBits == 8) {
     // Codes past the tensor's end are zeros and stay so.
     if (count < kPer) {
@@ -289,17 +296,17 @@ __device__ __forceinline__ void UpdateStep(const Tensor& t, bf16* copy,
       qv.v[j] = static_cast<uint8_t>(
           max(static_cast<uint32_t>(static_cast<int32_t>(cv[j])), low));
     }
-    StoreVec<int8_t, kPer>(static_cast<int8_t*>(s.m) + slot, qm);
-    StoreVec<uint8_t, kPer>(static_cast<uint8_t*>(s.v) + slot, qv);
+    StoreVec<int8_t, kPer>(static_cast<int8_t*>(s.m) + slot + own, qm);
+    StoreVec<uint8_t, kPer>(static_cast<uint8_t*>(s.v) + slot + own, qv);
     if (threadIdx.x % kWave == 0) {
-      s.m_scale[slot / kQuant] = ms;
-      s.v_scale[slot / kQuant] = vs;
+      s.m_scale[slot / kQuant + block] = ms;
+      s.v_scale[slot / kQuant + block] = vs;
     }
   } else {
     // Slots past the tensor's end belong to no value: their gradient was
     // read as zero, so zeros stay zeros.
-    Store4<float, kStream>(static_cast<float*>(s.m) + slot, kPer, m);
-    Store4<float, kStream>(static_cast<float*>(s.v) + slot, kPer, v);
+    Store4<float, kStream>(static_cast<float*>(s.m) + slot + own, kPer, m);
+    Store4<float, kStream>(static_cast<float*>(s.v) + slot + own, kPer, v);
   }
 }
 
