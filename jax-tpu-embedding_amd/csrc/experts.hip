@@ -42,6 +42,40 @@ __device__ __forceinline__ uint32_t KeyOf(const I* ids, int64_t i,
                                                  : experts;
 }
 
+// The keys of choices i, i + step, ... (kNoKey from `last` > 0 on), kKeys loads
+// in flight: one by one, each waits for memory.
+constexpr int kKeys = 4;
+constexpr uint32_t kNoKey = ~0u;
+template <typename I>
+__device__ __forceinline__ void LoadKeys(const I* ids, int32_t experts,
+                                         int64_t i, int64_t step, int64_t last,
+                                         uint32_t (&keys)[kKeys]) {
+#pragma unroll
+  for (int k = 0; k < kKeys; ++k) {
+    const int64_t at = i + k * step;
+    keys[k] = KeyOf(ids, at < last ? at : last - 1, experts);
+  }
+#pragma unroll
+  for (int k = 0; k < kKeys; ++k) {
+    if (i + k * step >= last) keys[k] = kNoKey;
+  }
+}
+
+// Adds the keys of choices i, i + step, ... to `counts` in LDS.
+template <typename I>
+__device__ __forceinline__ void CountKeys(const I* ids, int32_t experts,
+                                          int64_t i, int64_t step,
+                                          int64_t last, uint32_t* counts) {
+  for (; i < last; i += kKeys * step) {
+    uint32_t keys[kKeys];
+    LoadKeys(ids, experts, i, step, last, keys);
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) {
+      if (keys[k] != kNoKey) atomicAdd(&counts[keys[k]], 1u);
+    }
+  }
+}
+
 // Counts the keys of each wavefront's share [first, last) of a tile into its
 // row of `counts` ([waves][experts + 1] in LDS, cleared here).
 template <typename I, int kWaves>
@@ -53,10 +87,8 @@ __device__ __forceinline__ void CountShares(const I* ids, int32_t experts,
     counts[i] = 0;
   }
   __syncthreads();
-  uint32_t* mine = counts + (threadIdx.x / kWave) * row;
-  for (int64_t i = first + threadIdx.x % kWave; i < last; i += kWave) {
-    atomicAdd(&mine[KeyOf(ids, i, experts)], 1u);
-  }
+  CountKeys(ids, experts, first + threadIdx.x % kWave, kWave, last,
+            counts + (threadIdx.x / kWave) * row);
   __syncthreads();
 }
 
@@ -69,23 +101,29 @@ __device__ __forceinline__ void PlaceShare(const I* ids, int64_t n,
                                            int32_t* positions,
                                            int32_t* sources) {
   const int lane = threadIdx.x % kWave;
-  for (int64_t at = first; at < last; at += kWave) {
-    const int64_t i = at + lane;
-    const bool in = i < last;
-    const uint32_t key = in ? KeyOf(ids, i, experts) : 0u;
-    const uint64_t same = MatchLanes<kKeyBits>(__ballot(in), key);
-    const int leader = in ? __ffsll(static_cast<unsigned long long>(same)) - 1
-                          : lane;
-    uint32_t base = 0;
-    if (in && lane == leader) {
-      base = atomicAdd(&next[key], static_cast<uint32_t>(__popcll(same)));
-    }
-    base = __shfl(base, leader, kWave);
-    if (in) {
-      const uint32_t place = base + __popcll(same & LaneMaskLt());
-      positions[i] = static_cast<int32_t>(place);
-      // Always, unless the ids changed since they were counted.
-      if (place < n) sources[place] = static_cast<int32_t>(i);
+  for (int64_t at = first; at < last; at += kKeys * kWave) {
+    uint32_t keys[kKeys];
+    LoadKeys(ids, experts, at + lane, kWave, last, keys);
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) {
+      if (at + k * kWave >= last) break;  // uniform
+      const uint32_t key = keys[k];
+      const bool in = key != kNoKey;
+      const uint64_t same = MatchLanes<kKeyBits>(__ballot(in), key);
+      const int leader =
+          in ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
+      uint32_t base = 0;
+      if (in && lane == leader) {
+        base = atomicAdd(&next[key], static_cast<uint32_t>(__popcll(same)));
+      }
+      base = __shfl(base, leader, kWave);
+      if (in) {
+        const int64_t i = at + k * kWave + lane;
+        const uint32_t place = base + __popcll(same & LaneMaskLt());
+        positions[i] = static_cast<int32_t>(place);
+        // Always, unless the ids changed since they were counted.
+        if (place < n) sources[place] = static_cast<int32_t>(i);
+      }
     }
   }
 }
@@ -156,9 +194,7 @@ __global__ __launch_bounds__(kTileWaves* kWave) void CountTiles(
   __syncthreads();
   const int64_t begin = blockIdx.x * tile;
   const int64_t end = begin + tile < n ? begin + tile : n;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kBlock) {
-    atomicAdd(&counts[KeyOf(ids, i, experts)], 1u);
-  }
+  CountKeys(ids, experts, begin + threadIdx.x, kBlock, end, counts);
   __syncthreads();
   for (int i = threadIdx.x; i < row; i += kBlock) {
     const int64_t at = kOwnSums ? static_cast<int64_t>(blockIdx.x) * row + i
