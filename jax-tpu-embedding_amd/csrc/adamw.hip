@@ -3,7 +3,12 @@
 // One launch takes up to 104 tensors, whose addresses travel in the kernel
 // arguments; a work-group has kStep consecutive values of one of them.
 // The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
-// bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy.
+// bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy. A
+// work-group has one value vector a lane and ends: with four of them in a loop,
+// or read ahead of the computation, large tensors took 3% longer. Measured,
+// 176M values with float32 throughout 790 us, 6.2 TB/s (a device copy moves 4.9);
+// 79M with 8-bit moments, bfloat16 gradients and copies 245 us, 5.2 TB/s, where
+// the vector units are busy 0.73 of the time.
 //
 // Moments of 8 bits are decoded, moved, used and encoded in registers. A block
 // of 256 values is the four values of each lane of a wavefront, so its scale

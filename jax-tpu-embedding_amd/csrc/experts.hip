@@ -5,7 +5,14 @@
 // The sort knows both where a choice goes (positions) and where it came from
 // (sources), so every kernel works token by token: it reads a token's row
 // once however many choices it has, writes whole rows, and sums in the order
-// of the choices. Nothing is added atomically.
+// of the choices. Nothing is added atomically. (Row by row of the experts'
+// order, a token's row would be read once for each choice, from anywhere.)
+//
+// The sort is latency: 131,072 choices are 3 MB, and take 5 us to count and 7
+// to place. The rows are HBM-bound. Measured, 65,536 tokens with two of 64
+// experts each and 1024 bfloat16 columns: to the experts 76 us (5.3 TB/s) after
+// 11 us of sorting, back 67 us (6.0 TB/s); the gradient of four choices of
+// 16,384 tokens with 512 columns 30 us (5.1 TB/s).
 #include <algorithm>
 
 #include "dense.h"
