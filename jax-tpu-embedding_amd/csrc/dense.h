@@ -21,7 +21,7 @@ struct Vec {
 };
 
 // A vector's bytes as one value, aligned to 2 bytes as the smallest elements
-// are (1 for 4 bytes, which are 8-bit codes).
+// are.
 template <int kBytes>
 struct Words;
 template <>
@@ -33,10 +33,6 @@ template <>
 struct Words<8> {
   typedef uint32_t Vector __attribute__((ext_vector_type(2)));
   typedef Vector Type __attribute__((aligned(2)));
-};
-template <>
-struct Words<4> {
-  typedef uint32_t Type __attribute__((aligned(1)));
 };
 
 // Elements of 16 bytes.

@@ -42,6 +42,7 @@ struct Library {
   decltype(&scemb_adamw_moments) adamw_moments;
 };
 Library lib = {};
+PyObject* raw_stream = nullptr;  // the handle of a device's current stream
 
 // A Python exception that is already set.
 struct Raised {};
@@ -95,6 +96,18 @@ double Float(PyObject* o) {
 }
 void* Address(PyObject* o) {
   return o == Py_None ? nullptr : reinterpret_cast<void*>(Int(o));
+}
+
+void* Stream(int device) {
+  PyObject* index = PyLong_FromLong(device);
+  if (index == nullptr) throw Raised();
+  PyObject* o = PyObject_CallOneArg(raw_stream, index);
+  Py_DECREF(index);
+  if (o == nullptr) throw Raised();
+  void* stream = PyLong_AsVoidPtr(o);
+  Py_DECREF(o);
+  if (stream == nullptr && PyErr_Occurred()) throw Raised();
+  return stream;
 }
 
 constexpr uint32_t Bit(at::ScalarType t) {
@@ -242,10 +255,10 @@ Affine AffineOf(const Tensor& x, PyObject* weight, PyObject* bias, int dev) {
   return a;
 }
 
-// layer_norm(x, weight, bias, epsilon, stats, stream) -> y or (y, mean, rstd)
+// layer_norm(x, weight, bias, epsilon, stats) -> y or (y, mean, rstd)
 PyObject* LayerNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 6) Refuse("layer_norm takes 6 arguments");
+    if (n != 5) Refuse("layer_norm takes 5 arguments");
     const int dev = CurrentDevice();
     const Tensor& x = TensorOf(a[0], "x", dev, kRowTypes);
     const Affine p = AffineOf(x, a[1], a[2], dev);
@@ -269,18 +282,18 @@ PyObject* LayerNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Data(p.weight), Data(p.bias),
         w.defined() ? Code(w.scalar_type()) : SCEMB_F32,
         static_cast<float>(epsilon), y.data_ptr(), FloatData(mean),
-        FloatData(rstd), Address(a[5])));
+        FloatData(rstd), Stream(dev)));
     return stats ? Tuple({y, mean, rstd}) : Wrap(y);
   });
 }
 
 // layer_norm_grad(y_grad, x, mean, rstd, weight, want_weight, want_bias,
-//                 bias_f32, workspace, stream) -> (dx, dweight, dbias)
+//                 bias_f32, workspace) -> (dx, dweight, dbias)
 // bias_f32: the bias's type where there is no weight to say it (float32 or
 // x's).
 PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 10) Refuse("layer_norm_grad takes 10 arguments");
+    if (n != 9) Refuse("layer_norm_grad takes 9 arguments");
     const int dev = CurrentDevice();
     const Tensor& x = TensorOf(a[1], "x", dev, kRowTypes);
     const Affine p = AffineOf(x, a[4], Py_None, dev);
@@ -320,7 +333,7 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Check(lib.layer_norm_grad(
         g.t.data_ptr(), g.stride, r.t.data_ptr(), r.stride, code, r.n, dim,
         FloatData(stats[0]), FloatData(stats[1]), Data(p.weight), Code(type),
-        dx.data_ptr(), Data(dw), Data(db), ws, bytes, Address(a[9])));
+        dx.data_ptr(), Data(dw), Data(db), ws, bytes, Stream(dev)));
     return Tuple({dx, dw, db});
   });
 }
@@ -329,11 +342,11 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // Tokens and experts.
 // ---------------------------------------------------------------------------
 
-// sort_by_expert(ids, num_experts, workspace, stream)
+// sort_by_expert(ids, num_experts, workspace)
 //   -> (positions, sources, offsets)
 PyObject* SortByExpert(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 4) Refuse("sort_by_expert takes 4 arguments");
+    if (n != 3) Refuse("sort_by_expert takes 3 arguments");
     const int dev = CurrentDevice();
     const Tensor& ids = TensorOf(a[0], "expert_ids", dev, kI32 | kI64);
     if (ids.dim() != 1 && ids.dim() != 2) {
@@ -360,7 +373,7 @@ PyObject* SortByExpert(PyObject*, PyObject* const* a, Py_ssize_t n) {
         in.data_ptr(), static_cast<int32_t>(in.element_size()), count, e,
         static_cast<int32_t*>(positions.data_ptr()),
         static_cast<int32_t*>(sources.data_ptr()),
-        static_cast<int32_t*>(offsets.data_ptr()), ws, bytes, Address(a[3])));
+        static_cast<int32_t*>(offsets.data_ptr()), ws, bytes, Stream(dev)));
     return Tuple({positions, sources, offsets});
   });
 }
@@ -419,10 +432,10 @@ int32_t WeightsCode(const Tensor& w) {
   return w.defined() ? Code(w.scalar_type()) : SCEMB_F32;
 }
 
-// tokens_to_experts(x, positions, offsets, stream) -> rows
+// tokens_to_experts(x, positions, offsets) -> rows
 PyObject* TokensToExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 4) Refuse("tokens_to_experts takes 4 arguments");
+    if (n != 3) Refuse("tokens_to_experts takes 3 arguments");
     const int dev = CurrentDevice();
     const OrderOf o(a[1], a[2], dev);
     const Tensor& x = RowsArg(a[0], "x", o.positions.size(0), dev, kRowTypes);
@@ -431,18 +444,18 @@ PyObject* TokensToExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor rows = New({o.positions.numel(), dim}, x.scalar_type(), x);
     Check(lib.tokens_to_experts(r.t.data_ptr(), Code(x.scalar_type()),
                                 r.stride, dim, &o.order, rows.data_ptr(),
-                                Address(a[3])));
+                                Stream(dev)));
     return Wrap(rows);
   });
 }
 
-// tokens_from_experts(rows, weights, positions, offsets, stream, name) -> y
+// tokens_from_experts(rows, weights, positions, offsets, name) -> y
 PyObject* TokensFromExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 6) Refuse("tokens_from_experts takes 6 arguments");
+    if (n != 5) Refuse("tokens_from_experts takes 5 arguments");
     const int dev = CurrentDevice();
     const OrderOf o(a[2], a[3], dev);
-    const char* name = PyUnicode_AsUTF8(a[5]);
+    const char* name = PyUnicode_AsUTF8(a[4]);
     if (name == nullptr) throw Raised();
     const Tensor& rows =
         RowsArg(a[0], name, o.positions.numel(), dev, kRowTypes);
@@ -453,16 +466,16 @@ PyObject* TokensFromExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
         New({o.positions.size(0), dim}, rows.scalar_type(), rows);
     Check(lib.tokens_from_experts(r.t.data_ptr(), Code(rows.scalar_type()),
                                   r.stride, dim, Data(w), WeightsCode(w),
-                                  &o.order, y.data_ptr(), Address(a[4])));
+                                  &o.order, y.data_ptr(), Stream(dev)));
     return Wrap(y);
   });
 }
 
-// tokens_from_experts_grad(y_grad, rows, weights, positions, offsets, stream)
+// tokens_from_experts_grad(y_grad, rows, weights, positions, offsets)
 //   -> (drows, dweights)
 PyObject* TokensFromExpertsGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 6) Refuse("tokens_from_experts_grad takes 6 arguments");
+    if (n != 5) Refuse("tokens_from_experts_grad takes 5 arguments");
     const int dev = CurrentDevice();
     const OrderOf o(a[3], a[4], dev);
     const Tensor& rows =
@@ -483,7 +496,7 @@ PyObject* TokensFromExpertsGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Check(lib.tokens_from_experts_grad(
         g.t.data_ptr(), g.stride, r.t.data_ptr(), Code(rows.scalar_type()),
         r.stride, dim, Data(w), WeightsCode(w), &o.order, drows.data_ptr(),
-        Data(dweights), Address(a[5])));
+        Data(dweights), Stream(dev)));
     return Tuple({drows, dweights});
   });
 }
@@ -600,12 +613,11 @@ void CheckApart(const std::vector<scemb_adamw_tensor_t>& tensors) {
 
 // adamw_update(params, grads, copies, layout, m, v, m_scale, v_scale,
 //              learning_rate, beta_1, beta_2, epsilon, weight_decay,
-//              grad_scale, step, learning_rate_ptr, step_ptr, grad_scale_ptr,
-//              stream)
+//              grad_scale, step, learning_rate_ptr, step_ptr, grad_scale_ptr)
 // layout: bytes of scemb_adamw_tensor_t, of which numel and decay are set.
 PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 19) Refuse("adamw_update takes 19 arguments");
+    if (n != 18) Refuse("adamw_update takes 18 arguments");
     const int dev = CurrentDevice();
     const Sequence params(a[0], "params must be a sequence of tensors");
     const Sequence grads(a[1], "grads must be a sequence of tensors");
@@ -678,22 +690,22 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     o.step_ptr = static_cast<const int64_t*>(Address(a[16]));
     o.grad_scale_ptr = static_cast<const float*>(Address(a[17]));
     Check(lib.adamw_update(tensors.data(), static_cast<int32_t>(count), &state,
-                           &o, Address(a[18])));
+                           &o, Stream(dev)));
     Py_RETURN_NONE;
   });
 }
 
-// adamw_moments(m, v, m_scale, v_scale, stream) -> (m, v)
+// adamw_moments(m, v, m_scale, v_scale) -> (m, v)
 PyObject* AdamwMoments(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 5) Refuse("adamw_moments takes 5 arguments");
+    if (n != 4) Refuse("adamw_moments takes 4 arguments");
     const int dev = CurrentDevice();
     const scemb_adamw_state_t state = StateOf(a[0], a[1], a[2], a[3], dev);
     const Tensor& like = THPVariable_Unpack(a[0]);
     const Tensor m = New({state.size}, at::kFloat, like);
     const Tensor v = New({state.size}, at::kFloat, like);
     Check(lib.adamw_moments(&state, FloatData(m), FloatData(v),
-                            Address(a[4])));
+                            Stream(dev)));
     return Tuple({m, v});
   });
 }
@@ -702,10 +714,15 @@ PyObject* AdamwMoments(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // The module.
 // ---------------------------------------------------------------------------
 
-// bind(addresses): the library's functions, in the order of Library.
-PyObject* Bind(PyObject*, PyObject* addresses) {
+// bind(addresses, raw_stream): the library's functions, in the order of
+// Library, and a function from a device's index to its current stream's handle.
+PyObject* Bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
-    const Sequence s(addresses, "bind takes a sequence of addresses");
+    if (n != 2 || !PyCallable_Check(a[1])) {
+      PyErr_SetString(PyExc_ValueError, "bind takes addresses and a function");
+      return nullptr;
+    }
+    const Sequence s(a[0], "bind takes a sequence of addresses");
     constexpr Py_ssize_t kCount = sizeof(Library) / sizeof(void*);
     void* p[kCount];
     if (s.n != kCount) {
@@ -714,6 +731,8 @@ PyObject* Bind(PyObject*, PyObject* addresses) {
     }
     for (Py_ssize_t i = 0; i < kCount; ++i) p[i] = Address(s[i]);
     static_assert(sizeof(p) == sizeof(Library), "pointers only");
+    Py_INCREF(a[1]);
+    Py_XSETREF(raw_stream, a[1]);
     std::memcpy(&lib, p, sizeof(lib));
     Py_RETURN_NONE;
   } catch (const Raised&) {
@@ -737,7 +756,7 @@ PyObject* WantsGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define SCEMB_METHOD(name, f) \
   {name, reinterpret_cast<PyCFunction>(f), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
-    {"bind", Bind, METH_O, nullptr},
+    SCEMB_METHOD("bind", Bind),
     SCEMB_METHOD("wants_grad", WantsGrad),
     SCEMB_METHOD("layer_norm", LayerNorm),
     SCEMB_METHOD("layer_norm_grad", LayerNormGrad),

@@ -446,8 +446,9 @@ def dense_binding():
           "build it with `python -c 'import __graft_entry__; "
           "__graft_entry__.build()'` or `make -C jax-tpu-embedding_amd/csrc`."
       ) from e
+    raw = getattr(torch()._C, "_cuda_getCurrentRawStream", _raw_stream)  # pylint: disable=protected-access
     _dense.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value
-                 for f in _DENSE_FUNCTIONS])
+                 for f in _DENSE_FUNCTIONS], raw)
     _dense_module = _dense
   return _dense_module
 

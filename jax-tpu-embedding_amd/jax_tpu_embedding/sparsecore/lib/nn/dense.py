@@ -45,7 +45,6 @@ def _calls():
   return _binding
 
 
-_stream = _native.stream_handle
 _workspace = _native.WORKSPACE.get
 
 _functions = {}
@@ -61,8 +60,7 @@ def _function(name: str):
 
       @staticmethod
       def forward(ctx, x, weight, bias, epsilon):
-        y, mean, rstd = _calls().layer_norm(x, weight, bias, epsilon, True,
-                                            _stream())
+        y, mean, rstd = _calls().layer_norm(x, weight, bias, epsilon, True)
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.bias_f32 = bias is not None and bias.dtype == t.float32
         ctx.mark_non_differentiable(mean, rstd)
@@ -75,7 +73,7 @@ def _function(name: str):
         need = ctx.needs_input_grad
         dx, dw, db = _calls().layer_norm_grad(
             y_grad, x, mean, rstd, weight, need[1], need[2], ctx.bias_f32,
-            _workspace, _stream())
+            _workspace)
         return dx if need[0] else None, dw, db, None
 
     class ToExperts(t.autograd.Function):
@@ -83,13 +81,13 @@ def _function(name: str):
       @staticmethod
       def forward(ctx, x, positions, offsets):
         ctx.save_for_backward(positions, offsets)
-        return _calls().tokens_to_experts(x, positions, offsets, _stream())
+        return _calls().tokens_to_experts(x, positions, offsets)
 
       @staticmethod
       @once
       def backward(ctx, rows_grad):
         dx = _calls().tokens_from_experts(rows_grad, None, *ctx.saved_tensors,
-                                          _stream(), "rows_grad")
+                                          "rows_grad")
         return dx, None, None
 
     class FromExperts(t.autograd.Function):
@@ -98,14 +96,14 @@ def _function(name: str):
       def forward(ctx, rows, weights, positions, offsets):
         ctx.save_for_backward(rows, weights, positions, offsets)
         return _calls().tokens_from_experts(rows, weights, positions, offsets,
-                                            _stream(), "rows")
+                                            "rows")
 
       @staticmethod
       @once
       def backward(ctx, y_grad):
         need = ctx.needs_input_grad
-        drows, dw = _calls().tokens_from_experts_grad(
-            y_grad, *ctx.saved_tensors, _stream())
+        drows, dw = _calls().tokens_from_experts_grad(y_grad,
+                                                      *ctx.saved_tensors)
         return (drows if need[0] else None, dw if need[1] else None, None,
                 None)
 
@@ -136,8 +134,7 @@ def layer_norm(x, weight=None, bias=None, *, epsilon: float = 1e-6,
   if calls.wants_grad(x, weight, bias):
     out = _function("norm").apply(x, weight, bias, epsilon)
     return out if return_stats else out[0]
-  return calls.layer_norm(x, weight, bias, epsilon, bool(return_stats),
-                          _stream())
+  return calls.layer_norm(x, weight, bias, epsilon, bool(return_stats))
 
 
 def layer_norm_grad(y_grad, x, mean, rstd, weight=None, *,
@@ -153,7 +150,7 @@ def layer_norm_grad(y_grad, x, mean, rstd, weight=None, *,
   in float32 in an order that the shapes decide.
   """
   return _calls().layer_norm_grad(y_grad, x, mean, rstd, weight, True,
-                                  bool(with_bias), True, _workspace, _stream())
+                                  bool(with_bias), True, _workspace)
 
 
 # ---------------------------------------------------------------------------
@@ -188,7 +185,7 @@ def sort_by_expert(expert_ids, num_experts: int) -> ExpertOrder:
   Choices of one expert keep their order.
   """
   return ExpertOrder(*_calls().sort_by_expert(expert_ids, num_experts,
-                                              _workspace, _stream()))
+                                              _workspace))
 
 
 def tokens_to_experts(x, order: ExpertOrder):
@@ -200,7 +197,7 @@ def tokens_to_experts(x, order: ExpertOrder):
   calls = _calls()
   if calls.wants_grad(x):
     return _function("to").apply(x, order.positions, order.offsets)
-  return calls.tokens_to_experts(x, order.positions, order.offsets, _stream())
+  return calls.tokens_to_experts(x, order.positions, order.offsets)
 
 
 def tokens_to_experts_grad(rows_grad, order: ExpertOrder):
@@ -208,7 +205,7 @@ def tokens_to_experts_grad(rows_grad, order: ExpertOrder):
   choices' rows, in float32, rounded once. Rows of dropped choices are not
   read."""
   return _calls().tokens_from_experts(rows_grad, None, order.positions,
-                                      order.offsets, _stream(), "rows_grad")
+                                      order.offsets, "rows_grad")
 
 
 def tokens_from_experts(rows, weights, order: ExpertOrder):
@@ -224,7 +221,7 @@ def tokens_from_experts(rows, weights, order: ExpertOrder):
     return _function("back").apply(rows, weights, order.positions,
                                    order.offsets)
   return calls.tokens_from_experts(rows, weights, order.positions,
-                                   order.offsets, _stream(), "rows")
+                                   order.offsets, "rows")
 
 
 def tokens_from_experts_grad(y_grad, rows, weights, order: ExpertOrder):
@@ -233,8 +230,8 @@ def tokens_from_experts_grad(y_grad, rows, weights, order: ExpertOrder):
   Rows of dropped choices get zeros, and so do their weights. The second is
   None without weights.
   """
-  return _calls().tokens_from_experts_grad(
-      y_grad, rows, weights, order.positions, order.offsets, _stream())
+  return _calls().tokens_from_experts_grad(y_grad, rows, weights,
+                                           order.positions, order.offsets)
 
 
 # ---------------------------------------------------------------------------
@@ -357,7 +354,7 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   _calls().adamw_update(
       params, grads, copies, state._layout, state.m, state.v,  # pylint: disable=protected-access
       state.m_scale, state.v_scale, float(rate), beta_1, beta_2, epsilon,
-      weight_decay, float(scale), at, rate_at, step_at, scale_at, _stream())
+      weight_decay, float(scale), at, rate_at, step_at, scale_at)
   del keep_rate, keep_scale, keep_step
   if step_at is None:
     state.step = at
@@ -370,4 +367,4 @@ def adamw_moments(state: AdamWState):
   if state.bits == 32:
     return state.m, state.v
   return _calls().adamw_moments(state.m, state.v, state.m_scale,
-                                state.v_scale, _stream())
+                                state.v_scale)
