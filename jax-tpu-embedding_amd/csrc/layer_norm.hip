@@ -493,36 +493,54 @@ __global__ __launch_bounds__(256) void NormColumnsLong(NormGradArgs<T> a) {
   }
 }
 
-// Adds the work-groups' sums: 32 columns a work-group, the `parts` rows of
-// sums in 32 slices that LDS joins in their order. It is latency alone (8 to
-// 16 MB at most, from L2): eight loads of a thread are in flight.
-template <typename W>
+// Adds the work-groups' sums: kReduceColumns columns a work-group, the `parts`
+// rows of sums in slices that LDS joins in their order. It is latency alone (12
+// MB at most, from L2): all of a thread's loads are in flight at once. 16
+// columns up to 1024 (100 columns 3.6 us, with 32 a work-group 4.2), then 32
+// (4096 columns 5.8 us, with 16 8.9).
+template <typename W, int kReduceColumns>
 __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
                                                    int32_t parts, int32_t dim,
                                                    W* dweight, W* dbias) {
-  constexpr int kSlices = 32;
-  __shared__ float sums[kSlices][33];
+  constexpr int kSlices = 1024 / kReduceColumns;
+  __shared__ float sums[kSlices][kReduceColumns + 1];
   W* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
-  const int col = threadIdx.x % 32;
-  const int slice = threadIdx.x / 32;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col;
+  const int col = threadIdx.x % kReduceColumns;
+  const int slice = threadIdx.x / kReduceColumns;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kReduceColumns + col;
   const float* src =
       partial + static_cast<int64_t>(blockIdx.y) * parts * dim + c;
   float s = 0.f;
   if (c < dim) {
-#pragma unroll 8
-    for (int p = slice; p < parts; p += kSlices) {
-      s += src[static_cast<int64_t>(p) * dim];
+    constexpr int kLoads = 3 * kCus / kSlices;
+    for (int p = slice; p < parts; p += kLoads * kSlices) {
+      float x[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = p + i * kSlices;
+        x[i] = src[static_cast<int64_t>(at < parts ? at : p) * dim];
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (p + i * kSlices < parts) s += x[i];
+      }
     }
   }
   sums[slice][col] = s;
   __syncthreads();
-  if (threadIdx.x < 32 && c < dim) {
+  // Joined by 4 lanes a column, a quarter of the slices each.
+  if (threadIdx.x < 4 * kReduceColumns) {
+    const int quarter = threadIdx.x % 4;
+    const int k = threadIdx.x / 4;
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) s += sums[i][col];
-    out[c] = static_cast<W>(s);
+    for (int i = 0; i < kSlices / 4; ++i) {
+      s += sums[quarter * (kSlices / 4) + i][k];
+    }
+    s = LaneSum<4>(s);
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * kReduceColumns + k;
+    if (quarter == 0 && to < dim) out[to] = static_cast<W>(s);
   }
 }
 
@@ -542,6 +560,7 @@ Layout LayoutOf(int v, int64_t dim) {
   const int64_t n = CeilDiv(dim, v);
   const int most = 16 / v;  // vectors a lane
   return n <= 4            ? Layout{4, 1}
+         : n <= 8          ? Layout{8, 1}
          : n <= 16         ? Layout{16, 1}
          : n <= 32         ? Layout{16, 2}
          : n <= 64         ? Layout{64, 1}
@@ -605,6 +624,7 @@ int LaunchBackward(const NormGradArgs<T>& a, int64_t parts,
   }
 #define SCEMB_LAYOUTS(CALL)   \
   SCEMB_LAYOUT(4, 1, CALL)    \
+  SCEMB_LAYOUT(8, 1, CALL)    \
   SCEMB_LAYOUT(16, 1, CALL)   \
   SCEMB_LAYOUT(16, 2, CALL)   \
   SCEMB_LAYOUT(64, 1, CALL)   \
@@ -703,16 +723,26 @@ int RunForward(const void* x, int64_t rows, int64_t dim, int64_t stride,
   return rc;
 }
 
-template <typename T, typename W>
-int RunReduce(const float* partial, int64_t parts, int64_t dim, void* dweight,
-              void* dbias, hipStream_t stream) {
-  hipLaunchKernelGGL((NormReduce<W>),
-                     dim3(static_cast<uint32_t>(CeilDiv(dim, 32)), 2),
-                     dim3(1024), 0, stream, partial,
-                     static_cast<int32_t>(parts), static_cast<int32_t>(dim),
-                     static_cast<W*>(dweight), static_cast<W*>(dbias));
+template <typename W, int kReduceColumns>
+int LaunchReduce(const float* partial, int64_t parts, int64_t dim,
+                 void* dweight, void* dbias, hipStream_t stream) {
+  hipLaunchKernelGGL(
+      (NormReduce<W, kReduceColumns>),
+      dim3(static_cast<uint32_t>(CeilDiv(dim, kReduceColumns)), 2),
+      dim3(1024), 0, stream, partial, static_cast<int32_t>(parts),
+      static_cast<int32_t>(dim), static_cast<W*>(dweight),
+      static_cast<W*>(dbias));
   SCEMB_LAUNCH_CHECK();
   return 0;
+}
+
+template <typename W>
+int RunReduce(const float* partial, int64_t parts, int64_t dim, void* dweight,
+              void* dbias, hipStream_t stream) {
+  return dim <= 1024 ? LaunchReduce<W, 16>(partial, parts, dim, dweight, dbias,
+                                           stream)
+                     : LaunchReduce<W, 32>(partial, parts, dim, dweight, dbias,
+                                           stream);
 }
 
 template <typename T>
@@ -752,9 +782,8 @@ int RunBackward(const void* dy, int64_t dy_stride, const void* x,
   if (a.partial == nullptr) return 0;
   const int64_t sums = rows > 0 ? parts : 0;
   return weight_f32
-             ? RunReduce<T, float>(a.partial, sums, dim, dweight, dbias,
-                                   stream)
-             : RunReduce<T, T>(a.partial, sums, dim, dweight, dbias, stream);
+             ? RunReduce<float>(a.partial, sums, dim, dweight, dbias, stream)
+             : RunReduce<T>(a.partial, sums, dim, dweight, dbias, stream);
 }
 
 }  // namespace
