@@ -22,7 +22,10 @@ namespace scemb {
 namespace {
 
 constexpr int kCus = 256;
-constexpr int kForwardThreads = 4096;  // of a CU, about twice what it holds
+// Threads of a CU forwards, about twice what it holds: from 1024 to 8192 times
+// differ by 2 to 8%, wide rows gaining from more and 262,144 x 64 losing 20%
+// below 1536.
+constexpr int kForwardThreads = 4096;
 
 template <typename T>
 struct NormArgs {
@@ -550,7 +553,10 @@ __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
 
 // How a row is laid out over lanes: G lanes of NV vectors each. The fewest
 // lanes that hold the row at 16 values a lane (their weights and, backwards,
-// two sums stay in registers too); G = 0 for a row that no work-group holds.
+// two sums stay in registers too): lanes past a row's end do nothing (262,144 x
+// 64 bfloat16 backwards 29 us on 16 lanes, 23 on 8). G = 0 for a row that no
+// work-group holds; in passes, 10,000 rows of 16,384 float32 took 406 us
+// forwards and 620 backwards, in registers 230 and 315.
 struct Layout {
   int g;
   int nv;
@@ -574,8 +580,9 @@ Layout LayoutOf(int v, int64_t dim) {
 }
 
 // Work-groups of the backward pass, and so rows of partial sums: three a CU
-// (two of 1024 threads), each group of lanes at least one row, and no more
-// bytes of sums written and read than a quarter of what the rows are.
+// (65,536 x 1024 bfloat16: two 94 us, three 80, four 81; one of 1024 threads),
+// each group of lanes at least one row, and no more bytes of sums written and
+// read than a quarter of what the rows are.
 int64_t BackwardParts(Layout l, int type_bytes, int64_t rows) {
   const int groups = l.g == 0 ? 1 : BlockOf(l.g) / l.g;
   const int64_t most = l.g == 1024 || l.g == 0 ? kCus : 3 * kCus;

@@ -72,6 +72,48 @@ def test_example_learns(bits):
   assert np.mean(losses[-10:]) < 0.9 * np.mean(losses[:3])
 
 
+def test_two_streams():
+  """Steps on two streams at once, each with its own data and workspace."""
+  tokens, dim, experts = 20_000, 264, 40
+
+  def make(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((tokens, dim), device="cuda", generator=g)
+    ids = torch.randint(-1, experts, (tokens, 2), device="cuda", generator=g)
+    gates = torch.rand((tokens, 2), device="cuda", generator=g)
+    p = [torch.ones(dim, device="cuda"), torch.zeros(dim, device="cuda")]
+    return x, ids, gates, p, dense.init_adamw_state(p, state_bits=8)
+
+  def step(x, ids, gates, p, state):
+    y, mean, rstd = dense.layer_norm(x, *p, return_stats=True)
+    order = dense.sort_by_expert(ids, experts)
+    rows = dense.tokens_to_experts(y, order)
+    out = dense.tokens_from_experts(rows, gates, order)
+    drows, _ = dense.tokens_from_experts_grad(out, rows, gates, order)
+    dy = dense.tokens_to_experts_grad(drows, order)
+    _, dw, db = dense.layer_norm_grad(dy, x, mean, rstd, p[0])
+    dense.adamw_update(p, [dw, db], state, learning_rate=0.01)
+    return out
+
+  alone = [make(i) for i in (1, 2)]
+  expected = [[step(*a) for _ in range(5)][-1] for a in alone]
+  torch.cuda.synchronize()
+  both = [make(i) for i in (1, 2)]
+  streams = [torch.cuda.Stream() for _ in both]
+  torch.cuda.synchronize()
+  outs = [None, None]
+  for _ in range(5):
+    for i, s in enumerate(streams):
+      with torch.cuda.stream(s):
+        outs[i] = step(*both[i])
+  torch.cuda.synchronize()
+  for i in range(2):
+    assert torch.equal(outs[i], expected[i])
+    for a, b in zip(alone[i][3], both[i][3]):
+      assert torch.equal(a, b)
+    assert torch.equal(alone[i][4].m, both[i][4].m)
+
+
 def test_captured_step():
   """Norm, experts and AdamW with a step counter on the GPU, captured once and
   replayed with other work in between: each replay as the eager step."""

@@ -194,6 +194,30 @@ def test_strides(dtype):
   _check_all(order, x[:1].expand(x.shape), rows, one, weights)
 
 
+def test_what_dropped_choices_hold_is_not_read():
+  """Infinite and undefined weights, rows and tokens of dropped choices."""
+  order, x, rows, dy, weights = _case(40, 3, 6, 24, torch.float32, dropped=0.4)
+  gone = order.positions >= order.offsets[-1]
+  clean = (dense.tokens_from_experts(rows, weights, order),
+           dense.tokens_from_experts_grad(dy, rows, weights, order))
+  for bad in (float("nan"), float("inf"), -float("inf"),
+              torch.finfo(torch.float32).min):
+    w, r = weights.clone(), rows.clone()
+    w[gone] = bad
+    r[int(order.offsets[-1]):] = bad
+    assert torch.equal(dense.tokens_from_experts(r, w, order), clean[0])
+    got = dense.tokens_from_experts_grad(dy, r, w, order)
+    assert torch.equal(got[0], clean[1][0]) and torch.equal(got[1],
+                                                            clean[1][1])
+    t = x.clone()
+    t[gone.all(1)] = bad
+    assert torch.equal(dense.tokens_to_experts(t, order),
+                       dense.tokens_to_experts(x, order))
+  none = dense.sort_by_expert(torch.full((40, 3), -1, device="cuda"), 6)
+  assert (dense.tokens_from_experts(rows, weights, none) == 0).all()
+  assert (dense.tokens_to_experts_grad(rows, none) == 0).all()
+
+
 def test_wrong_positions_are_dropped():
   """Positions that no sort gives neither fault nor touch other rows."""
   order, x, rows, dy, weights = _case(20, 2, 4, 16, torch.float32, dropped=0.0)
