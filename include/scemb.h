@@ -743,6 +743,8 @@ typedef struct scemb_adamw_state {
   int64_t size;   /* a multiple of SCEMB_ADAMW_BLOCK */
   int32_t bits;   /* 8 or 32 */
   int32_t reserved;
+  float* scratch; /* [4] for steps with a learning rate or step on the device
+                     (NULL: no such steps) */
 } scemb_adamw_state_t;
 typedef struct scemb_adamw_options {
   double learning_rate;

@@ -1,6 +1,6 @@
 // AdamW over many tensors at once, with moments in float32 or in 8 bits.
 //
-// One launch takes up to 104 tensors, whose addresses travel in the kernel
+// One launch takes up to 108 tensors, whose addresses travel in the kernel
 // arguments; a work-group has kStep consecutive values of one of them.
 // The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
 // bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy. A
@@ -45,9 +45,9 @@ struct Tensor {
 static_assert(sizeof(Tensor) == 32, "four words");
 
 // Tensors of a launch: what the kernel's arguments hold, two lanes' worth at
-// most (a launch of 64 small tensors takes 5 us, and so does one of 104).
+// most (a launch of 64 small tensors takes 5 us, and so does one of 108).
 template <bool kCopies>
-constexpr int kMaxTensors = kCopies ? 83 : 104;
+constexpr int kMaxTensors = kCopies ? 87 : 108;
 
 struct Moments {
   void* m;
@@ -80,15 +80,8 @@ template <bool kCopies>
 struct AdamArgs : Tensors<kCopies> {
   Moments moments;
   Factors factors;
-  // Device scalars and what the factors are then made of.
-  const float* learning_rate_ptr;
-  const int64_t* step_ptr;
+  const float* rates;  // rate, root and keep made on the device, or NULL
   const float* grad_scale_ptr;
-  double learning_rate;
-  double beta_1;
-  double beta_2;
-  double weight_decay;
-  int64_t step;
   int32_t n;
 };
 static_assert(sizeof(AdamArgs<false>) <= 3584 &&
@@ -102,6 +95,22 @@ __host__ __device__ inline void SetRates(double learning_rate, double beta_1,
   f->rate = static_cast<float>(learning_rate / (1.0 - pow(beta_1, t)));
   f->root = static_cast<float>(1.0 / sqrt(1.0 - pow(beta_2, t)));
   f->keep = static_cast<float>(1.0 - learning_rate * weight_decay);
+}
+
+// The same from device scalars, once a step: in every work-group of it, two
+// powers in 64 bits would be three times the step's own operations.
+__global__ void MakeRates(scemb_adamw_options_t o, float* rates) {
+  Factors f;
+  SetRates(o.learning_rate_ptr != nullptr
+               ? static_cast<double>(*o.learning_rate_ptr)
+               : o.learning_rate,
+           o.beta_1, o.beta_2, o.weight_decay,
+           o.step_ptr != nullptr ? *o.step_ptr : o.step, &f);
+  if (threadIdx.x == 0) {
+    rates[0] = f.rate;
+    rates[1] = f.root;
+    rates[2] = f.keep;
+  }
 }
 
 // The lane's values, of which `count` exist (zeros past them).
@@ -328,12 +337,10 @@ __global__ __launch_bounds__(kThreads) void AdamUpdate(AdamArgs<kCopies> a) {
   const Tensor t = a.tensors[i];
   bf16* copy = kCopies ? static_cast<bf16*>(a.copies[i]) : nullptr;
   Factors f = a.factors;
-  if (a.learning_rate_ptr != nullptr || a.step_ptr != nullptr) {
-    SetRates(a.learning_rate_ptr != nullptr
-                 ? static_cast<double>(*a.learning_rate_ptr)
-                 : a.learning_rate,
-             a.beta_1, a.beta_2, a.weight_decay,
-             a.step_ptr != nullptr ? *a.step_ptr : a.step, &f);
+  if (a.rates != nullptr) {
+    f.rate = a.rates[0];
+    f.root = a.rates[1];
+    f.keep = a.rates[2];
   }
   if (a.grad_scale_ptr != nullptr) f.grad_scale = *a.grad_scale_ptr;
   const int64_t begin = static_cast<int64_t>(blockIdx.x - t.first) * kStep;
@@ -437,14 +444,14 @@ int UpdateAll(const scemb_adamw_tensor_t* tensors, int32_t num_tensors,
   a.factors.epsilon = static_cast<float>(o.epsilon);
   SetRates(o.learning_rate, o.beta_1, o.beta_2, o.weight_decay, o.step,
            &a.factors);
-  a.learning_rate_ptr = o.learning_rate_ptr;
-  a.step_ptr = o.step_ptr;
   a.grad_scale_ptr = o.grad_scale_ptr;
-  a.learning_rate = o.learning_rate;
-  a.beta_1 = o.beta_1;
-  a.beta_2 = o.beta_2;
-  a.weight_decay = o.weight_decay;
-  a.step = o.step;
+  a.rates = nullptr;
+  if (o.learning_rate_ptr != nullptr || o.step_ptr != nullptr) {
+    a.rates = state.scratch;
+    hipLaunchKernelGGL(MakeRates, dim3(1), dim3(kWave), 0, stream, o,
+                       state.scratch);
+    SCEMB_LAUNCH_CHECK();
+  }
   a.n = 0;
   uint32_t block = 0;
   int64_t groups = 0;
@@ -498,6 +505,12 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
       (options->step_ptr == nullptr && options->step < 1)) {
     return Fail(SCEMB_ERR_INVALID_ARGUMENT,
                 "adamw: tensors or options missing, or a step below 1");
+  }
+  if ((options->learning_rate_ptr != nullptr || options->step_ptr != nullptr) &&
+      state->scratch == nullptr) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "adamw: a state without scratch takes no learning rate or "
+                "step on the device");
   }
   int64_t blocks = 0, bytes = 0;
   bool copies = false;

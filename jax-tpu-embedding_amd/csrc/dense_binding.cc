@@ -566,7 +566,7 @@ PyObject* AdamwSizes(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 scemb_adamw_state_t StateOf(PyObject* m, PyObject* v, PyObject* m_scale,
-                            PyObject* v_scale, int dev) {
+                            PyObject* v_scale, PyObject* scratch, int dev) {
   const bool bits8 = m_scale != Py_None;
   const auto one = [&](PyObject* o, const char* name,
                        at::ScalarType type) -> const Tensor& {
@@ -590,6 +590,11 @@ scemb_adamw_state_t StateOf(PyObject* m, PyObject* v, PyObject* m_scale,
     sizes = sizes && ms.numel() * SCEMB_ADAMW_BLOCK == s.size &&
             vs.numel() == ms.numel();
   }
+  if (scratch != Py_None) {
+    const Tensor& t = one(scratch, "state.scratch", at::kFloat);
+    sizes = sizes && t.numel() >= 4;
+    s.scratch = FloatData(t);
+  }
   if (!sizes) Refuse("the state's tensors are not of matching sizes");
   return s;
 }
@@ -611,13 +616,13 @@ void CheckApart(const std::vector<scemb_adamw_tensor_t>& tensors) {
   }
 }
 
-// adamw_update(params, grads, copies, layout, m, v, m_scale, v_scale,
+// adamw_update(params, grads, copies, layout, m, v, m_scale, v_scale, scratch,
 //              learning_rate, beta_1, beta_2, epsilon, weight_decay,
 //              grad_scale, step, learning_rate_ptr, step_ptr, grad_scale_ptr)
 // layout: bytes of scemb_adamw_tensor_t, of which numel and decay are set.
 PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 18) Refuse("adamw_update takes 18 arguments");
+    if (n != 19) Refuse("adamw_update takes 19 arguments");
     const int dev = CurrentDevice();
     const Sequence params(a[0], "params must be a sequence of tensors");
     const Sequence grads(a[1], "grads must be a sequence of tensors");
@@ -677,18 +682,19 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
     }
     CheckApart(tensors);
-    const scemb_adamw_state_t state = StateOf(a[4], a[5], a[6], a[7], dev);
+    const scemb_adamw_state_t state =
+        StateOf(a[4], a[5], a[6], a[7], a[8], dev);
     scemb_adamw_options_t o = {};
-    o.learning_rate = Float(a[8]);
-    o.beta_1 = Float(a[9]);
-    o.beta_2 = Float(a[10]);
-    o.epsilon = Float(a[11]);
-    o.weight_decay = Float(a[12]);
-    o.grad_scale = Float(a[13]);
-    o.step = Int(a[14]);
-    o.learning_rate_ptr = static_cast<const float*>(Address(a[15]));
-    o.step_ptr = static_cast<const int64_t*>(Address(a[16]));
-    o.grad_scale_ptr = static_cast<const float*>(Address(a[17]));
+    o.learning_rate = Float(a[9]);
+    o.beta_1 = Float(a[10]);
+    o.beta_2 = Float(a[11]);
+    o.epsilon = Float(a[12]);
+    o.weight_decay = Float(a[13]);
+    o.grad_scale = Float(a[14]);
+    o.step = Int(a[15]);
+    o.learning_rate_ptr = static_cast<const float*>(Address(a[16]));
+    o.step_ptr = static_cast<const int64_t*>(Address(a[17]));
+    o.grad_scale_ptr = static_cast<const float*>(Address(a[18]));
     Check(lib.adamw_update(tensors.data(), static_cast<int32_t>(count), &state,
                            &o, Stream(dev)));
     Py_RETURN_NONE;
@@ -700,7 +706,8 @@ PyObject* AdamwMoments(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
     if (n != 4) Refuse("adamw_moments takes 4 arguments");
     const int dev = CurrentDevice();
-    const scemb_adamw_state_t state = StateOf(a[0], a[1], a[2], a[3], dev);
+    const scemb_adamw_state_t state =
+        StateOf(a[0], a[1], a[2], a[3], Py_None, dev);
     const Tensor& like = THPVariable_Unpack(a[0]);
     const Tensor m = New({state.size}, at::kFloat, like);
     const Tensor v = New({state.size}, at::kFloat, like);

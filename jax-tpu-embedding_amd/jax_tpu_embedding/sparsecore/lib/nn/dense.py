@@ -277,6 +277,8 @@ class AdamWState:
     else:
       self.m, self.v = new(total, t.float32), new(total, t.float32)
       self.m_scale = self.v_scale = None
+    # What steps with hyperparameters on the GPU make of them.
+    self._scratch = new(4, t.float32)
     layout = np.zeros(len(sizes), _TENSOR)
     layout["numel"] = sizes
     layout["decay"] = decay
@@ -351,10 +353,12 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   at = int(at)
   if step_at is None and at < 1:
     raise ValueError(f"the first step is 1, got {at}")
+  # pylint: disable=protected-access
   _calls().adamw_update(
-      params, grads, copies, state._layout, state.m, state.v,  # pylint: disable=protected-access
-      state.m_scale, state.v_scale, float(rate), beta_1, beta_2, epsilon,
-      weight_decay, float(scale), at, rate_at, step_at, scale_at)
+      params, grads, copies, state._layout, state.m, state.v,
+      state.m_scale, state.v_scale, state._scratch, float(rate), beta_1,
+      beta_2, epsilon, weight_decay, float(scale), at, rate_at, step_at,
+      scale_at)
   del keep_rate, keep_scale, keep_step
   if step_at is None:
     state.step = at

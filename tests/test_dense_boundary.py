@@ -25,7 +25,8 @@ class Order(ctypes.Structure):
 
 class State(ctypes.Structure):
   _fields_ = [("m", VP), ("v", VP), ("m_scale", VP), ("v_scale", VP),
-              ("size", I64), ("bits", I32), ("reserved", I32)]
+              ("size", I64), ("bits", I32), ("reserved", I32),
+              ("scratch", VP)]
 
 
 class Options(ctypes.Structure):
@@ -149,7 +150,9 @@ def test_adamw():
       dict(state=dict(bits=16)), dict(state=dict(size=500)),
       dict(state=dict(size=-256)), dict(state=dict(m=0)),
       dict(state=dict(v=0)), dict(state=dict(bits=8)),
-      dict(options=dict(step=0)), dict(n=-1)]
+      dict(options=dict(step=0)), dict(n=-1),
+      dict(options=dict(step_ptr=SOME)),
+      dict(options=dict(learning_rate_ptr=SOME))]
   for b in bad:
     assert call(**b) == INVALID, b
   # Nothing to do: no tensors, none with a gradient, none with values.

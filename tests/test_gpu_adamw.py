@@ -231,7 +231,8 @@ def test_many_tensors(bits):
   assert torch.equal(together[0], _tensors(sizes, torch.float32, 6)[0])
 
 
-@pytest.mark.parametrize("count", [63, 64, 65, 83, 84, 104, 105, 129, 209])
+@pytest.mark.parametrize("count", [63, 64, 65, 83, 84, 87, 88, 104, 105, 108,
+                                   109, 129, 217])
 def test_numbers_of_tensors(count):
   """On both sides of what a launch and a lane take, with and without copies,
   against one tensor that holds them all."""
