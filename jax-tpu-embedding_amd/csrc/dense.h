@@ -196,6 +196,9 @@ __device__ __forceinline__ float LaneSum(float x) {
 // Host side.
 // ---------------------------------------------------------------------------
 
+// Work-groups of a launch at most: a grid has fewer than 2^32 threads.
+constexpr int64_t MostGroups(int threads) { return 0xffffffffll / threads; }
+
 inline int TypeBytes(int32_t type) {
   return type == SCEMB_F32 ? 4
          : type == SCEMB_BF16 || type == SCEMB_F16 ? 2

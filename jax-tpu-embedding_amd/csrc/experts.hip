@@ -559,7 +559,7 @@ __global__ __launch_bounds__(kRowBlock) void FromExpertsGrad(
 
 uint32_t RowGrid(int64_t tokens, int g) {
   return static_cast<uint32_t>(
-      std::min<int64_t>(CeilDiv(tokens, kRowBlock / g), 0x7fffffff));
+      std::min(CeilDiv(tokens, kRowBlock / g), MostGroups(kRowBlock)));
 }
 
 // Launches `kernel` with the fewest lanes a token, from 8 to a wavefront, that

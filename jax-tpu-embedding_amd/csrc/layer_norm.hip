@@ -497,21 +497,25 @@ __global__ __launch_bounds__(256) void NormColumnsLong(NormGradArgs<T> a) {
 }
 
 // Adds the work-groups' sums: kReduceColumns columns a work-group, the `parts`
-// rows of sums in slices that LDS joins in their order. It is latency alone (12
+// rows of sums in slices that LDS joins in their order, from column `first`
+// on. It is latency alone (12
 // MB at most, from L2): all of a thread's loads are in flight at once. 16
 // columns up to 1024 (100 columns 3.6 us, with 32 a work-group 4.2), then 32
 // (4096 columns 5.8 us, with 16 8.9).
 template <typename W, int kReduceColumns>
 __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
                                                    int32_t parts, int32_t dim,
-                                                   W* dweight, W* dbias) {
+                                                   int32_t first, W* dweight,
+                                                   W* dbias) {
   constexpr int kSlices = 1024 / kReduceColumns;
   __shared__ float sums[kSlices][kReduceColumns + 1];
   W* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
   const int col = threadIdx.x % kReduceColumns;
   const int slice = threadIdx.x / kReduceColumns;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kReduceColumns + col;
+  const int64_t begin =
+      first + static_cast<int64_t>(blockIdx.x) * kReduceColumns;
+  const int64_t c = begin + col;
   const float* src =
       partial + static_cast<int64_t>(blockIdx.y) * parts * dim + c;
   float s = 0.f;
@@ -542,7 +546,7 @@ __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
       s += sums[quarter * (kSlices / 4) + i][k];
     }
     s = LaneSum<4>(s);
-    const int64_t to = static_cast<int64_t>(blockIdx.x) * kReduceColumns + k;
+    const int64_t to = begin + k;
     if (quarter == 0 && to < dim) out[to] = static_cast<W>(s);
   }
 }
@@ -666,7 +670,7 @@ int Forward(const NormArgs<T>& a, hipStream_t stream) {
   SCEMB_LAYOUTS((LaunchForward<T, NV, G, kCut>(a, stream)))
   hipLaunchKernelGGL(
       NormForwardLong<T>,
-      dim3(static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff))),
+      dim3(static_cast<uint32_t>(std::min(a.rows, MostGroups(1024)))),
       dim3(1024), 0, stream, a);
   SCEMB_LAUNCH_CHECK();
   return 0;
@@ -678,7 +682,7 @@ int Backward(const NormGradArgs<T>& a, Layout l, int64_t parts,
   SCEMB_LAYOUTS((LaunchBackward<T, NV, G, kCut>(a, parts, stream)))
   hipLaunchKernelGGL(
       NormBackwardLong<T>,
-      dim3(static_cast<uint32_t>(std::min<int64_t>(a.rows, 0x7fffffff))),
+      dim3(static_cast<uint32_t>(std::min(a.rows, MostGroups(1024)))),
       dim3(1024), 0, stream, a);
   SCEMB_LAUNCH_CHECK();
   if (a.partial != nullptr) {
@@ -733,13 +737,17 @@ int RunForward(const void* x, int64_t rows, int64_t dim, int64_t stride,
 template <typename W, int kReduceColumns>
 int LaunchReduce(const float* partial, int64_t parts, int64_t dim,
                  void* dweight, void* dbias, hipStream_t stream) {
-  hipLaunchKernelGGL(
-      (NormReduce<W, kReduceColumns>),
-      dim3(static_cast<uint32_t>(CeilDiv(dim, kReduceColumns)), 2),
-      dim3(1024), 0, stream, partial, static_cast<int32_t>(parts),
-      static_cast<int32_t>(dim), static_cast<W*>(dweight),
-      static_cast<W*>(dbias));
-  SCEMB_LAUNCH_CHECK();
+  constexpr int64_t kGroups = MostGroups(1024);
+  for (int64_t first = 0; first < dim; first += kGroups * kReduceColumns) {
+    const int64_t groups =
+        std::min(CeilDiv(dim - first, kReduceColumns), kGroups);
+    hipLaunchKernelGGL((NormReduce<W, kReduceColumns>),
+                       dim3(static_cast<uint32_t>(groups), 2), dim3(1024), 0,
+                       stream, partial, static_cast<int32_t>(parts),
+                       static_cast<int32_t>(dim), static_cast<int32_t>(first),
+                       static_cast<W*>(dweight), static_cast<W*>(dbias));
+    SCEMB_LAUNCH_CHECK();
+  }
   return 0;
 }
 
