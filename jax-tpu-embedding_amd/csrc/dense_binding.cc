@@ -137,9 +137,13 @@ std::string TypeNames(uint32_t types) {
   return s;
 }
 
+// Whether the tensor's memory holds its values: views that are negated when
+// they are read, and zeros that were never written, have others.
+bool HoldsValues(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
+
 // The tensor of an argument, on GPU `device` and of one of `types`.
-const Tensor& TensorOf(PyObject* o, const std::string& name, int device,
-                       uint32_t types) {
+const Tensor& AnyTensorOf(PyObject* o, const std::string& name, int device,
+                          uint32_t types) {
   if (!THPVariable_Check(o)) {
     Refuse(name + " must be a torch tensor, got " + Py_TYPE(o)->tp_name);
   }
@@ -150,6 +154,24 @@ const Tensor& TensorOf(PyObject* o, const std::string& name, int device,
   if (!(types & Bit(t.scalar_type()))) {
     Refuse(name + " must be one of " + TypeNames(types) + ", got " +
            Text(t.scalar_type()));
+  }
+  if (t.layout() != at::kStrided) Refuse(name + " must be a dense tensor");
+  return t;
+}
+
+// The same with its values in memory, for arguments that are read.
+Tensor TensorOf(PyObject* o, const std::string& name, int device,
+                uint32_t types) {
+  const Tensor& t = AnyTensorOf(o, name, device, types);
+  return HoldsValues(t) ? t : t.clone();
+}
+
+// The same for arguments that are written.
+const Tensor& PlaceOf(PyObject* o, const std::string& name, int device,
+                      uint32_t types) {
+  const Tensor& t = AnyTensorOf(o, name, device, types);
+  if (!HoldsValues(t) || !t.is_contiguous()) {
+    Refuse(name + " must be contiguous and hold its values");
   }
   return t;
 }
@@ -260,7 +282,7 @@ PyObject* LayerNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
     if (n != 5) Refuse("layer_norm takes 5 arguments");
     const int dev = CurrentDevice();
-    const Tensor& x = TensorOf(a[0], "x", dev, kRowTypes);
+    const Tensor x = TensorOf(a[0], "x", dev, kRowTypes);
     const Affine p = AffineOf(x, a[1], a[2], dev);
     const double epsilon = Float(a[3]);
     if (!(epsilon >= 0)) {
@@ -295,9 +317,9 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
     if (n != 9) Refuse("layer_norm_grad takes 9 arguments");
     const int dev = CurrentDevice();
-    const Tensor& x = TensorOf(a[1], "x", dev, kRowTypes);
+    const Tensor x = TensorOf(a[1], "x", dev, kRowTypes);
     const Affine p = AffineOf(x, a[4], Py_None, dev);
-    const Tensor& dy = TensorOf(a[0], "y_grad", dev, Bit(x.scalar_type()));
+    const Tensor dy = TensorOf(a[0], "y_grad", dev, Bit(x.scalar_type()));
     if (dy.sizes() != x.sizes()) {
       Refuse("y_grad must have x's shape " + Text(x.sizes()) + ", got " +
              Text(dy.sizes()));
@@ -306,7 +328,7 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor stats[2];
     for (int i = 0; i < 2; ++i) {
       const char* name = i == 0 ? "mean" : "rstd";
-      const Tensor& s = TensorOf(a[2 + i], name, dev, kF32);
+      const Tensor s = TensorOf(a[2 + i], name, dev, kF32);
       if (s.numel() * dim != x.numel()) {
         Refuse(std::string(name) + " must have a value for each row of x, got "
                "shape " + Text(s.sizes()));
@@ -348,7 +370,7 @@ PyObject* SortByExpert(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
     if (n != 3) Refuse("sort_by_expert takes 3 arguments");
     const int dev = CurrentDevice();
-    const Tensor& ids = TensorOf(a[0], "expert_ids", dev, kI32 | kI64);
+    const Tensor ids = TensorOf(a[0], "expert_ids", dev, kI32 | kI64);
     if (ids.dim() != 1 && ids.dim() != 2) {
       Refuse("expert_ids must have shape [tokens, choices] or [tokens], got " +
              Text(ids.sizes()));
@@ -407,9 +429,9 @@ struct OrderOf {
   }
 };
 
-const Tensor& RowsArg(PyObject* o, const char* name, int64_t n, int dev,
+Tensor RowsArg(PyObject* o, const char* name, int64_t n, int dev,
                       uint32_t types) {
-  const Tensor& x = TensorOf(o, name, dev, types);
+  const Tensor x = TensorOf(o, name, dev, types);
   if (x.dim() != 2 || x.size(0) != n || x.size(1) < 1) {
     Refuse(std::string(name) + " must have shape [" + std::to_string(n) +
            ", dim], got " + Text(x.sizes()));
@@ -438,7 +460,7 @@ PyObject* TokensToExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 3) Refuse("tokens_to_experts takes 3 arguments");
     const int dev = CurrentDevice();
     const OrderOf o(a[1], a[2], dev);
-    const Tensor& x = RowsArg(a[0], "x", o.positions.size(0), dev, kRowTypes);
+    const Tensor x = RowsArg(a[0], "x", o.positions.size(0), dev, kRowTypes);
     const int64_t dim = x.size(1);
     const Rows r = RowsOf(x, dim);
     const Tensor rows = New({o.positions.numel(), dim}, x.scalar_type(), x);
@@ -457,7 +479,7 @@ PyObject* TokensFromExperts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const OrderOf o(a[2], a[3], dev);
     const char* name = PyUnicode_AsUTF8(a[4]);
     if (name == nullptr) throw Raised();
-    const Tensor& rows =
+    const Tensor rows =
         RowsArg(a[0], name, o.positions.numel(), dev, kRowTypes);
     const Tensor w = WeightsArg(a[1], o, rows, dev);
     const int64_t dim = rows.size(1);
@@ -478,11 +500,11 @@ PyObject* TokensFromExpertsGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 5) Refuse("tokens_from_experts_grad takes 5 arguments");
     const int dev = CurrentDevice();
     const OrderOf o(a[3], a[4], dev);
-    const Tensor& rows =
+    const Tensor rows =
         RowsArg(a[1], "rows", o.positions.numel(), dev, kRowTypes);
     const Tensor w = WeightsArg(a[2], o, rows, dev);
     const int64_t dim = rows.size(1);
-    const Tensor& dy = TensorOf(a[0], "y_grad", dev, Bit(rows.scalar_type()));
+    const Tensor dy = TensorOf(a[0], "y_grad", dev, Bit(rows.scalar_type()));
     if (dy.dim() != 2 || dy.size(0) != o.positions.size(0) ||
         dy.size(1) != dim) {
       Refuse("y_grad must have shape [" + std::to_string(o.positions.size(0)) +
@@ -525,23 +547,24 @@ std::string At(const char* name, Py_ssize_t i) {
   return std::string(name) + "[" + std::to_string(i) + "]";
 }
 
-// TensorOf of an element, whose name is only made where it is refused.
+// Whether an element is a contiguous tensor that fits. If not, TensorOf and
+// PlaceOf say why, or make one, with a name that is only made for them.
+bool Fits(PyObject* o, int dev, uint32_t types) {
+  if (!THPVariable_Check(o)) return false;
+  const Tensor& t = THPVariable_Unpack(o);
+  return t.is_cuda() && t.get_device() == dev &&
+         (types & Bit(t.scalar_type())) && t.layout() == at::kStrided &&
+         HoldsValues(t) && t.is_contiguous();
+}
+
 const Tensor& ElementOf(PyObject* o, const char* name, Py_ssize_t i, int dev,
                         uint32_t types) {
-  if (THPVariable_Check(o)) {
-    const Tensor& t = THPVariable_Unpack(o);
-    if (t.is_cuda() && t.get_device() == dev &&
-        (types & Bit(t.scalar_type()))) {
-      return t;
-    }
-  }
-  return TensorOf(o, At(name, i), dev, types);
+  return Fits(o, dev, types) ? THPVariable_Unpack(o)
+                             : PlaceOf(o, At(name, i), dev, types);
 }
 
 const Tensor& ParamOf(PyObject* o, Py_ssize_t i, int dev) {
-  const Tensor& p = ElementOf(o, "params", i, dev, kF32 | kBf16);
-  if (!p.is_contiguous()) Refuse(At("params", i) + " must be contiguous");
-  return p;
+  return ElementOf(o, "params", i, dev, kF32 | kBf16);
 }
 
 // adamw_sizes(params) -> list of their numbers of values
@@ -570,9 +593,7 @@ scemb_adamw_state_t StateOf(PyObject* m, PyObject* v, PyObject* m_scale,
   const bool bits8 = m_scale != Py_None;
   const auto one = [&](PyObject* o, const char* name,
                        at::ScalarType type) -> const Tensor& {
-    const Tensor& t = TensorOf(o, name, dev, Bit(type));
-    if (!t.is_contiguous()) Refuse(std::string(name) + " must be contiguous");
-    return t;
+    return PlaceOf(o, name, dev, Bit(type));
   };
   const Tensor& tm = one(m, "state.m", bits8 ? at::kChar : at::kFloat);
   const Tensor& tv = one(v, "state.v", bits8 ? at::kByte : at::kFloat);
@@ -650,18 +671,19 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
       t.param = p.data_ptr();
       t.param_type = Code(p.scalar_type());
       if (grads[i] != Py_None) {
-        const Tensor& g = ElementOf(grads[i], "grads", i, dev, kF32 | kBf16);
+        constexpr uint32_t kTypes = kF32 | kBf16;
+        const bool fits = Fits(grads[i], dev, kTypes);
+        if (!fits) {
+          keep.push_back(
+              TensorOf(grads[i], At("grads", i), dev, kTypes).contiguous());
+        }
+        const Tensor& g = fits ? THPVariable_Unpack(grads[i]) : keep.back();
         if (g.sizes() != p.sizes()) {
           Refuse(At("grads", i) + " must have the shape " + Text(p.sizes()) +
                  " of its weight, got " + Text(g.sizes()));
         }
         t.grad_type = Code(g.scalar_type());
-        if (g.is_contiguous()) {
-          t.grad = g.data_ptr();
-        } else {
-          keep.push_back(g.contiguous());
-          t.grad = keep.back().data_ptr();
-        }
+        t.grad = g.data_ptr();
       }
     }
     if (a[2] != Py_None) {
@@ -674,9 +696,9 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (copies[i] == Py_None) continue;
         const Tensor& c = ElementOf(copies[i], "copies", i, dev, kBf16);
         const Tensor& p = THPVariable_Unpack(params[i]);
-        if (!c.is_contiguous() || c.sizes() != p.sizes()) {
-          Refuse(At("copies", i) + " must be contiguous and have the shape " +
-                 Text(p.sizes()) + " of its weight, got " + Text(c.sizes()));
+        if (c.sizes() != p.sizes()) {
+          Refuse(At("copies", i) + " must have the shape " + Text(p.sizes()) +
+                 " of its weight, got " + Text(c.sizes()));
         }
         tensors[i].copy = c.data_ptr();
       }
