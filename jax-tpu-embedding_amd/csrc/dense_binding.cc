@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <optional>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -620,21 +621,31 @@ scemb_adamw_state_t StateOf(PyObject* m, PyObject* v, PyObject* m_scale,
   return s;
 }
 
-// Two weights that share memory would be updated by two work-groups at once.
+// Two weights or copies that share memory would be written by two work-groups
+// at once.
 void CheckApart(const std::vector<scemb_adamw_tensor_t>& tensors) {
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  spans.reserve(tensors.size());
+  spans.reserve(2 * tensors.size());
+  const auto add = [&](const void* p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    spans.emplace_back(at, at + static_cast<uintptr_t>(bytes));
+  };
   for (const auto& t : tensors) {
     if (t.numel == 0) continue;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.param);
-    spans.emplace_back(
-        at, at + static_cast<uintptr_t>(t.numel) *
-                     (t.param_type == SCEMB_F32 ? 4 : 2));
+    add(t.param, t.numel * (t.param_type == SCEMB_F32 ? 4 : 2));
+    if (t.copy != nullptr) add(t.copy, t.numel * 2);
   }
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i) {
-    if (spans[i].first < spans[i - 1].second) Refuse("two params share memory");
+    if (spans[i].first < spans[i - 1].second) {
+      Refuse("two params or copies share memory");
+    }
   }
+}
+
+// Autograd is told of a write: a backward pass that needs the old values raises.
+void Written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // adamw_update(params, grads, copies, layout, m, v, m_scale, v_scale, scratch,
@@ -686,21 +697,26 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
         t.grad = g.data_ptr();
       }
     }
+    std::optional<Sequence> copies;
     if (a[2] != Py_None) {
-      const Sequence copies(a[2], "copies must be a sequence of tensors");
-      if (copies.n != count) {
-        Refuse(std::to_string(copies.n) + " copies for " +
+      copies.emplace(a[2], "copies must be a sequence of tensors");
+      if (copies->n != count) {
+        Refuse(std::to_string(copies->n) + " copies for " +
                std::to_string(count) + " params");
       }
       for (Py_ssize_t i = 0; i < count; ++i) {
-        if (copies[i] == Py_None) continue;
-        const Tensor& c = ElementOf(copies[i], "copies", i, dev, kBf16);
+        if ((*copies)[i] == Py_None) continue;
+        const Tensor& c = ElementOf((*copies)[i], "copies", i, dev, kBf16);
         const Tensor& p = THPVariable_Unpack(params[i]);
         if (c.sizes() != p.sizes()) {
           Refuse(At("copies", i) + " must have the shape " + Text(p.sizes()) +
                  " of its weight, got " + Text(c.sizes()));
         }
-        tensors[i].copy = c.data_ptr();
+        // A bfloat16 weight's own tensor is its copy already.
+        if (p.scalar_type() == at::kFloat ||
+            c.data_ptr() != tensors[i].param) {
+          tensors[i].copy = c.data_ptr();
+        }
       }
     }
     CheckApart(tensors);
@@ -719,6 +735,13 @@ PyObject* AdamwUpdate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     o.grad_scale_ptr = static_cast<const float*>(Address(a[18]));
     Check(lib.adamw_update(tensors.data(), static_cast<int32_t>(count), &state,
                            &o, Stream(dev)));
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      if (tensors[i].grad == nullptr) continue;
+      Written(THPVariable_Unpack(params[i]));
+      if (tensors[i].copy != nullptr) {
+        Written(THPVariable_Unpack((*copies)[i]));
+      }
+    }
     Py_RETURN_NONE;
   });
 }

@@ -339,7 +339,8 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   learning_rate, grad_scale: floats, or single values on the GPU (a schedule's
     or a clipping factor that nobody waits for).
   copies: None, or a bfloat16 tensor of each weight's shape (or None) that gets
-    the rounded weight: the working copies of float32 weights.
+    the rounded weight: the working copies of float32 weights. Params and
+    copies may not share memory, but a bfloat16 weight may be its own copy.
   step: None (state.step + 1), an int, or a single int64 on the GPU, which a
     captured graph advances itself. The first step is 1.
   """

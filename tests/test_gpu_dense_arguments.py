@@ -1,6 +1,7 @@
 """What a tensor's memory does not say: the dense operators (lib/nn/dense.py) on
-views that are negated when read, zeros that were never written, and tensors
-that are not dense."""
+views that are negated when read, zeros that were never written, tensors that
+are not dense, tensors that share memory, and autograd's view of weights that
+were written."""
 
 import pytest
 
@@ -107,3 +108,48 @@ def test_sparse_tensors_are_refused():
                                           learning_rate=0.1)):
     with pytest.raises(ValueError):
       call()
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_autograd_knows_of_updated_weights(inference):
+  with torch.inference_mode(inference):
+    p, other, copy = _rand(300), _rand(300), _rand(300).bfloat16()
+  state = dense.init_adamw_state([p, other])
+  if inference:
+    dense.adamw_update([p, other], [_rand(300), None], state,
+                       learning_rate=0.1, copies=[copy, None])
+    assert torch.equal(copy, p.bfloat16())
+    return
+  x = _rand(300).requires_grad_()
+  stale, fresh = (x * p).sum(), (x * other).sum()
+  stale_copy = (x * copy).sum()
+  dense.adamw_update([p, other], [_rand(300), None], state, learning_rate=0.1,
+                     copies=[copy, None])
+  fresh.backward()
+  assert torch.equal(x.grad, other)
+  for y in (stale, stale_copy):
+    with pytest.raises(RuntimeError):
+      y.backward()
+
+
+def test_copies_share_no_memory():
+  p, q = _rand(300), _rand(300, seed=1)
+  half = _rand(300, seed=2).bfloat16()
+  room = torch.zeros(400, dtype=torch.bfloat16, device="cuda")
+  g = _rand(300, seed=3)
+  for params, copies in (([p, q], [room[:300], room[100:]]),
+                         ([p, half], [half, None]),
+                         ([p, q], [q.view(torch.bfloat16)[:300], None]),
+                         ([p], [p.view(torch.bfloat16)[:300]])):
+    before = [x.clone() for x in params]
+    state = dense.init_adamw_state(params)
+    with pytest.raises(ValueError):
+      dense.adamw_update(params, [g] * len(params), state, learning_rate=0.1,
+                         copies=copies)
+    _same(params, before)
+  # A bfloat16 weight is its own copy.
+  expected = half.clone()
+  for w, copies in ((half, [half]), (expected, None)):
+    dense.adamw_update([w], [g], dense.init_adamw_state([w]),
+                       learning_rate=0.1, copies=copies)
+  assert torch.equal(half, expected)
