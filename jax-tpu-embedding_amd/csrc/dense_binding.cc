@@ -229,17 +229,17 @@ PyObject* Tuple(std::initializer_list<Tensor> tensors) {
   return out;
 }
 
-// A workspace of at least `bytes`, from the caller's function of a size.
-void* Workspace(PyObject* get, size_t bytes) {
+// A workspace of at least `bytes`, from the caller's function of a size. It is
+// held until the work on it is enqueued.
+Tensor Workspace(PyObject* get, size_t bytes) {
   PyObject* size = PyLong_FromSize_t(bytes);
   if (size == nullptr) throw Raised();
   PyObject* o = PyObject_CallOneArg(get, size);
   Py_DECREF(size);
   if (o == nullptr) throw Raised();
-  // The pool keeps it.
-  void* p = THPVariable_Check(o) ? THPVariable_Unpack(o).data_ptr() : nullptr;
+  const Tensor t = THPVariable_Check(o) ? THPVariable_Unpack(o) : Tensor();
   Py_DECREF(o);
-  return p;
+  return t;
 }
 
 // ---------------------------------------------------------------------------
@@ -346,7 +346,7 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[5] == Py_True && p.weight.defined()) dw = New({dim}, type, x);
     if (a[6] == Py_True) db = New({dim}, type, x);
     const int32_t code = Code(x.scalar_type());
-    void* ws = nullptr;
+    Tensor ws;
     size_t bytes = 0;
     if (dw.defined() || db.defined()) {
       bytes = lib.layer_norm_grad_workspace(code, r.n, dim);
@@ -356,7 +356,7 @@ PyObject* LayerNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Check(lib.layer_norm_grad(
         g.t.data_ptr(), g.stride, r.t.data_ptr(), r.stride, code, r.n, dim,
         FloatData(stats[0]), FloatData(stats[1]), Data(p.weight), Code(type),
-        dx.data_ptr(), Data(dw), Data(db), ws, bytes, Stream(dev)));
+        dx.data_ptr(), Data(dw), Data(db), Data(ws), bytes, Stream(dev)));
     return Tuple({dx, dw, db});
   });
 }
@@ -391,12 +391,13 @@ PyObject* SortByExpert(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor offsets = New({experts + 1}, at::kInt, ids);
     const int32_t e = static_cast<int32_t>(experts);
     const size_t bytes = lib.sort_by_expert_workspace(count, e);
-    void* ws = bytes > 0 ? Workspace(a[2], bytes) : nullptr;
+    const Tensor ws = bytes > 0 ? Workspace(a[2], bytes) : Tensor();
     Check(lib.sort_by_expert(
         in.data_ptr(), static_cast<int32_t>(in.element_size()), count, e,
         static_cast<int32_t*>(positions.data_ptr()),
         static_cast<int32_t*>(sources.data_ptr()),
-        static_cast<int32_t*>(offsets.data_ptr()), ws, bytes, Stream(dev)));
+        static_cast<int32_t*>(offsets.data_ptr()), Data(ws), bytes,
+        Stream(dev)));
     return Tuple({positions, sources, offsets});
   });
 }

@@ -870,34 +870,33 @@ class _Workspace:
   side_streams), so preprocessing on one stream may overlap a step or
   another preprocessing on another.
 
-  A buffer that a call used while its stream was being captured into a graph
-  stays allocated after it has been outgrown: the graph's replays still
-  address it."""
+  Calls that are being captured into a graph use no such buffer: graphs
+  captured on one stream (torch's default capture stream, mostly) may be
+  replayed on several at once. They get memory of the graph's own pool, which
+  lives as long as the graph, and which later calls of the capture use again
+  once the caller lets go of it."""
 
   def __init__(self):
     self._buf = {}
-    self._captured = set()
-    self._retired = []
 
   def get(self, nbytes: int, stream=None):
-    """The buffer of `stream` (default: the current stream), at least
-    `nbytes` long. A new buffer is allocated on that stream, so that the
-    allocator hands its memory to no other stream before the stream's work
-    on it is done."""
+    """A buffer for work on `stream` (default: the current stream), at least
+    `nbytes` long, to be held until that work is enqueued. A new buffer is
+    allocated on that stream, so that the allocator hands its memory to no
+    other stream before the stream's work on it is done."""
     t = torch()
+    if stream is not None:
+      with t.cuda.stream(stream):
+        return self.get(nbytes)
     dev = device()
-    key = (dev.index, _raw_stream(dev.index) if stream is None else
-           stream.cuda_stream)
+    if t.cuda.is_current_stream_capturing():
+      return t.empty(max(int(nbytes), 1), dtype=t.uint8, device=dev)
+    key = (dev.index, _raw_stream(dev.index))
     buf = self._buf.get(key)
     if buf is None or buf.numel() < nbytes:
-      if buf is not None and key in self._captured:
-        self._retired.append(buf)
-      with t.cuda.stream(stream or t.cuda.current_stream(dev)):
-        buf = t.empty(max(int(nbytes * 1.25), 1 << 20), dtype=t.uint8,
-                      device=dev)
+      buf = t.empty(max(int(nbytes * 1.25), 1 << 20), dtype=t.uint8,
+                    device=dev)
       self._buf[key] = buf
-    if t.cuda.is_current_stream_capturing():
-      self._captured.add(key)
     return buf
 
 
