@@ -127,8 +127,10 @@ def layer_norm(x, weight=None, bias=None, *, epsilon: float = 1e-6,
   return_stats: also return the float32 mean and reciprocal deviation of every
     row ([...]), which layer_norm_grad takes.
 
-  Statistics and products are float32; the result is rounded once. A row that
-  holds an infinity or a NaN gives a row of NaN.
+  Statistics and products are float32; the result is rounded once. The mean's
+  own rounding is taken out of the result, so a row of one value gives the bias
+  whatever that value is. A row that holds an infinity or a NaN gives a row of
+  NaN.
   """
   calls = _calls()
   if calls.wants_grad(x, weight, bias):
