@@ -671,8 +671,11 @@ int scemb_sort_by_expert(const void* ids, int32_t id_bytes, int64_t n,
                          size_t workspace_bytes, void* stream);
 
 /* Such an order of tokens * choices choices, choice t * choices + k being
- * token t's k-th. A position outside [0, tokens * choices) counts as
- * dropped. */
+ * token t's k-th. positions is a permutation of [0, tokens * choices), as
+ * scemb_sort_by_expert writes it: choices are dropped by their ids there. Other
+ * positions are not supported. They reach no memory past the rows (a position
+ * out of range adds nothing where rows are read, and its weight's gradient is
+ * zero), but a row that no choice has is not written and holds what it held. */
 typedef struct scemb_expert_order {
   const int32_t* positions; /* [tokens * choices] */
   const int32_t* offsets;   /* [num_experts + 1] */
@@ -681,8 +684,8 @@ typedef struct scemb_expert_order {
   int32_t num_experts;
 } scemb_expert_order_t;
 
-/* rows[positions[t, k]] = x[t], zero for dropped choices: every row of
- * `rows` ([tokens * choices, dim] contiguous) is written. */
+/* rows[positions[t, k]] = x[t], zero for dropped choices; `rows` is
+ * [tokens * choices, dim] contiguous. */
 int scemb_tokens_to_experts(const void* x, int32_t type, int64_t x_stride,
                             int64_t dim, const scemb_expert_order_t* order,
                             void* rows, void* stream);
@@ -698,7 +701,7 @@ int scemb_tokens_from_experts(const void* rows, int32_t type,
                               void* stream);
 
 /* Its gradients: rows_grad[positions[t, k]] = weights[t, k] * y_grad[t]
- * (every row written, zero for dropped choices) and weights_grad[t, k] =
+ * (zero for dropped choices) and weights_grad[t, k] =
  * the inner product of y_grad[t] and rows[positions[t, k]] (zero for dropped
  * choices). */
 int scemb_tokens_from_experts_grad(

@@ -446,7 +446,7 @@ __global__ __launch_bounds__(kRowBlock) void ToExperts(const E* x,
       const auto v = LoadSpan<kCut, E, V, kStream>(x + t * stride, s);
       for (int k = 0; k < order.choices; ++k) {
         const uint32_t p = static_cast<uint32_t>(places[k]);
-        if (p < all) {
+        if (p < all) {  // always, in an order that a sort made
           StoreSpan<kCut, E, V>(rows + static_cast<int64_t>(p) * dim, s,
                                 p < kept ? v : Vec<E, V>{});
         }

@@ -161,7 +161,11 @@ def layer_norm_grad(y_grad, x, mean, rstd, weight=None, *,
 
 
 class ExpertOrder(NamedTuple):
-  """The order of tokens' choices by expert, int32 tensors on the GPU.
+  """The order of tokens' choices by expert, int32 tensors on the GPU, as
+  sort_by_expert makes it. To drop a choice, sort with an id out of range:
+  positions that are changed afterwards leave a row without a choice, and what
+  is written row by row (tokens_to_experts, the gradient of
+  tokens_from_experts's rows) is undefined there.
 
   positions: of the shape of the ids: the row of each choice among all,
     expert by expert, dropped choices at the end.
