@@ -12,6 +12,7 @@
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
 #include <algorithm>
@@ -142,7 +143,14 @@ std::string TypeNames(uint32_t types) {
 // they are read, and zeros that were never written, have others.
 bool HoldsValues(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
 
-// The tensor of an argument, on GPU `device` and of one of `types`.
+// Whether the tensor carries a tangent of forward-mode differentiation.
+bool HasTangent(const Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         t._fw_grad(/*level=*/0).defined();
+}
+
+// The tensor of an argument, on GPU `device` and of one of `types`. The kernels
+// know no tangents: a result without one would be taken for a constant.
 const Tensor& AnyTensorOf(PyObject* o, const std::string& name, int device,
                           uint32_t types) {
   if (!THPVariable_Check(o)) {
@@ -157,6 +165,10 @@ const Tensor& AnyTensorOf(PyObject* o, const std::string& name, int device,
            Text(t.scalar_type()));
   }
   if (t.layout() != at::kStrided) Refuse(name + " must be a dense tensor");
+  if (HasTangent(t)) {
+    Refuse(name + " carries a tangent: the dense operators have no forward-mode "
+           "derivatives");
+  }
   return t;
 }
 
@@ -556,7 +568,7 @@ bool Fits(PyObject* o, int dev, uint32_t types) {
   const Tensor& t = THPVariable_Unpack(o);
   return t.is_cuda() && t.get_device() == dev &&
          (types & Bit(t.scalar_type())) && t.layout() == at::kStrided &&
-         HoldsValues(t) && t.is_contiguous();
+         HoldsValues(t) && t.is_contiguous() && !HasTangent(t);
 }
 
 const Tensor& ElementOf(PyObject* o, const char* name, Py_ssize_t i, int dev,

@@ -17,7 +17,8 @@ Arrays are torch tensors on the current GPU, work is enqueued on the current
 stream and nothing waits for it; arguments that do not fit raise ValueError.
 layer_norm, tokens_to_experts and tokens_from_experts take part in torch's
 autograd; the _grad functions are the same gradients for callers that keep
-their own tape, as embedding.tpu_sparse_dense_matmul_grad's are.
+their own tape, as embedding.tpu_sparse_dense_matmul_grad's are. Nothing here
+has forward-mode derivatives: tensors that carry a tangent are refused.
 """
 
 from __future__ import annotations
