@@ -8,6 +8,7 @@
 // is the same code against torch's tensors directly. The library's functions
 // are handed over by bind(), so there is one copy of it in the process.
 #include <Python.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/grad_mode.h>
@@ -72,8 +73,9 @@ PyObject* Guarded(F f) {
   } catch (const Raised&) {
   } catch (const std::invalid_argument& e) {
     PyErr_SetString(PyExc_ValueError, e.what());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    // torch's own, running out of memory among them, stay what callers catch.
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }
