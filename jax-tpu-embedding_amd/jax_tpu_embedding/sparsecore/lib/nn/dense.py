@@ -261,11 +261,13 @@ class AdamWState:
     uint8 with 8 bits, whose values adamw_moments returns.
   m_scale, v_scale: with 8 bits, a float32 for each ADAMW_BLOCK values; else
     None.
-  step: updates made so far.
+  step: updates made so far, where the host counts them. Updates whose step is a
+    value on the GPU are not in it: that value is the count.
   bits: 8 or 32.
 
-  A checkpoint keeps these tensors and the step; a state made for the same
-  weights takes them back with copy_().
+  A checkpoint keeps these tensors and the step (the value on the GPU, where that
+  counts); a state made for the same weights takes them back with copy_() and
+  `state.step = ...`.
   """
 
   def __init__(self, sizes, decay, bits: int):
@@ -290,6 +292,17 @@ class AdamWState:
     layout["numel"] = sizes
     layout["decay"] = decay
     self._layout = layout.tobytes()
+
+  @property
+  def step(self) -> int:
+    return self._step
+
+  @step.setter
+  def step(self, value: int):
+    self._step = value
+    # Whether the last update's step was a value on the GPU: the host cannot
+    # count on from `step` then.
+    self._counted_on_gpu = False
 
 
 def init_adamw_state(params, *, state_bits: int = 32,
@@ -349,11 +362,17 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
     the rounded weight: the working copies of float32 weights. Params and
     copies may not share memory, but a bfloat16 weight may be its own copy.
   step: None (state.step + 1), an int, or a single int64 on the GPU, which a
-    captured graph advances itself. The first step is 1.
+    captured graph advances itself (an int is the same in every replay). The
+    first step is 1. After an update with a value on the GPU, None is refused
+    until an int is given here or set as state.step.
   """
   if not (0 <= beta_1 < 1 and 0 <= beta_2 < 1 and epsilon >= 0):
     raise ValueError("beta_1 and beta_2 must be within [0, 1) and epsilon not "
                      f"negative, got {beta_1}, {beta_2} and {epsilon}")
+  # pylint: disable=protected-access
+  if step is None and state._counted_on_gpu:
+    raise ValueError("the state's updates were counted on the GPU: give the "
+                     "step, or set state.step to the updates made so far")
   t = _native.torch()
   rate, rate_at, keep_rate = _scalar(learning_rate, t.float32, 0.0)
   scale, scale_at, keep_scale = _scalar(grad_scale, t.float32, 1.0)
@@ -361,7 +380,6 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   at = int(at)
   if step_at is None and at < 1:
     raise ValueError(f"the first step is 1, got {at}")
-  # pylint: disable=protected-access
   _calls().adamw_update(
       params, grads, copies, state._layout, state.m, state.v,
       state.m_scale, state.v_scale, state._scratch, float(rate), beta_1,
@@ -370,6 +388,8 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   del keep_rate, keep_scale, keep_step
   if step_at is None:
     state.step = at
+  else:
+    state._counted_on_gpu = True
   return params
 
 
