@@ -444,8 +444,8 @@ def dense_binding():
       raise RuntimeError(
           f"the dense operators' module is missing or does not load ({e}); "
           "build it with `python -c 'import __graft_entry__; "
-          "__graft_entry__.build()'` or `make -C jax-tpu-embedding_amd/csrc`."
-      ) from e
+          "__graft_entry__.build()'` or `make -C jax-tpu-embedding_amd/csrc "
+          "python`.") from e
     raw = getattr(torch()._C, "_cuda_getCurrentRawStream", _raw_stream)  # pylint: disable=protected-access
     _dense.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value
                  for f in _DENSE_FUNCTIONS], raw)
