@@ -335,7 +335,12 @@ def _scalar(x, dtype, missing):
   if x.numel() != 1:
     raise ValueError("a hyperparameter on the GPU must be one value, got "
                      f"shape {tuple(x.shape)}")
+  if t.autograd.forward_ad.unpack_dual(x).tangent is not None:
+    raise ValueError("a hyperparameter carries a tangent: the dense operators "
+                     "have no forward-mode derivatives")
   x = x.to(device=_native.device(), dtype=dtype)
+  if x.is_neg() or x._is_zerotensor():  # pylint: disable=protected-access
+    x = x.clone()  # its memory does not hold its value
   return missing, x.data_ptr(), x
 
 
