@@ -151,8 +151,16 @@ bool HasTangent(const Tensor& t) {
          t._fw_grad(/*level=*/0).defined();
 }
 
-// The tensor of an argument, on GPU `device` and of one of `types`. The kernels
-// know no tangents: a result without one would be taken for a constant.
+// The kernels know no tangents: a result without one would be taken for a
+// constant.
+void CheckTangent(const Tensor& t, const std::string& name) {
+  if (HasTangent(t)) {
+    Refuse(name + " carries a tangent: the dense operators have no forward-mode "
+           "derivatives");
+  }
+}
+
+// The tensor of an argument, on GPU `device` and of one of `types`.
 const Tensor& AnyTensorOf(PyObject* o, const std::string& name, int device,
                           uint32_t types) {
   if (!THPVariable_Check(o)) {
@@ -167,10 +175,7 @@ const Tensor& AnyTensorOf(PyObject* o, const std::string& name, int device,
            Text(t.scalar_type()));
   }
   if (t.layout() != at::kStrided) Refuse(name + " must be a dense tensor");
-  if (HasTangent(t)) {
-    Refuse(name + " carries a tangent: the dense operators have no forward-mode "
-           "derivatives");
-  }
+  CheckTangent(t, name);
   return t;
 }
 
@@ -663,6 +668,29 @@ void Written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// adamw_scalar(x, is_int) -> x, a tensor of one value on a GPU, as a tensor on the
+// current GPU whose memory holds it as float32 or int64 (x itself if it does).
+PyObject* AdamwScalar(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 2 || !THPVariable_Check(a[0])) {
+      Refuse("adamw_scalar takes a tensor and its kind");
+    }
+    const Tensor& x = THPVariable_Unpack(a[0]);
+    if (x.numel() != 1) {
+      Refuse("a hyperparameter on the GPU must be one value, got shape " +
+             Text(x.sizes()));
+    }
+    CheckTangent(x, "a hyperparameter");
+    const auto type = a[1] == Py_True ? at::kLong : at::kFloat;
+    const int dev = CurrentDevice();
+    if (x.scalar_type() == type && x.get_device() == dev && HoldsValues(x)) {
+      return Py_NewRef(a[0]);
+    }
+    const Tensor t = x.to(at::TensorOptions(type).device(at::kCUDA, dev));
+    return Wrap(HoldsValues(t) ? t : t.clone());
+  });
+}
+
 // adamw_update(params, grads, copies, layout, m, v, m_scale, v_scale, scratch,
 //              learning_rate, beta_1, beta_2, epsilon, weight_decay,
 //              grad_scale, step, learning_rate_ptr, step_ptr, grad_scale_ptr)
@@ -832,6 +860,7 @@ PyMethodDef kMethods[] = {
     SCEMB_METHOD("tokens_from_experts", TokensFromExperts),
     SCEMB_METHOD("tokens_from_experts_grad", TokensFromExpertsGrad),
     SCEMB_METHOD("adamw_sizes", AdamwSizes),
+    SCEMB_METHOD("adamw_scalar", AdamwScalar),
     SCEMB_METHOD("adamw_update", AdamwUpdate),
     SCEMB_METHOD("adamw_moments", AdamwMoments),
     {nullptr, nullptr, 0, nullptr}};

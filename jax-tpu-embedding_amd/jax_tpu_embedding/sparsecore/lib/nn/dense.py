@@ -324,7 +324,7 @@ def init_adamw_state(params, *, state_bits: int = 32,
   return AdamWState(sizes, decay, state_bits)
 
 
-def _scalar(x, dtype, missing):
+def _scalar(x, is_int, missing):
   """(host value, None, None) of a number, (missing, its address, a tensor to
   keep until the launch) of a single value on the GPU."""
   if x is None:
@@ -332,15 +332,7 @@ def _scalar(x, dtype, missing):
   t = _native.torch()
   if not isinstance(x, t.Tensor) or not x.is_cuda:
     return x, None, None
-  if x.numel() != 1:
-    raise ValueError("a hyperparameter on the GPU must be one value, got "
-                     f"shape {tuple(x.shape)}")
-  if t.autograd.forward_ad.unpack_dual(x).tangent is not None:
-    raise ValueError("a hyperparameter carries a tangent: the dense operators "
-                     "have no forward-mode derivatives")
-  x = x.to(device=_native.device(), dtype=dtype)
-  if x.is_neg() or x._is_zerotensor():  # pylint: disable=protected-access
-    x = x.clone()  # its memory does not hold its value
+  x = _calls().adamw_scalar(x, is_int)
   return missing, x.data_ptr(), x
 
 
@@ -378,10 +370,9 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   if step is None and state._counted_on_gpu:
     raise ValueError("the state's updates were counted on the GPU: give the "
                      "step, or set state.step to the updates made so far")
-  t = _native.torch()
-  rate, rate_at, keep_rate = _scalar(learning_rate, t.float32, 0.0)
-  scale, scale_at, keep_scale = _scalar(grad_scale, t.float32, 1.0)
-  at, step_at, keep_step = _scalar(step, t.int64, state.step + 1)
+  rate, rate_at, keep_rate = _scalar(learning_rate, False, 0.0)
+  scale, scale_at, keep_scale = _scalar(grad_scale, False, 1.0)
+  at, step_at, keep_step = _scalar(step, True, state.step + 1)
   at = int(at)
   if step_at is None and at < 1:
     raise ValueError(f"the first step is 1, got {at}")
