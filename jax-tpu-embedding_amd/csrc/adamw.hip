@@ -5,10 +5,11 @@
 // The work is HBM-bound: 28 bytes a value with float32 throughout, 14 with
 // bfloat16 gradients and moments of 8 bits, two more for a bfloat16 copy. A
 // work-group has one value vector a lane and ends: with four of them in a loop,
-// or read ahead of the computation, large tensors took 3% longer. Measured,
-// 176M values with float32 throughout 790 us, 6.2 TB/s (a device copy moves 4.9);
-// 79M with 8-bit moments, bfloat16 gradients and copies 245 us, 5.2 TB/s, where
-// the vector units are busy 0.71 of the time.
+// or read ahead of the computation, large tensors took 3% longer. Measured, step
+// after step, 176M values with float32 throughout 828 us, 6.0 TB/s (797 in turn
+// with other calls; a device copy moves 4.9); 79M with 8-bit moments, bfloat16
+// gradients and copies 220 us, 5.8 TB/s. Where the moments are read out between
+// the steps those take 245 us, the vector units busy 0.71 of the time.
 //
 // Moments of 8 bits are decoded, moved, used and encoded in registers. A block
 // of 256 values is the four values of each lane of a wavefront, so its scale
@@ -539,8 +540,8 @@ int scemb_adamw_update(const scemb_adamw_tensor_t* tensors,
                 "adamw: the state is smaller than the tensors");
   }
   // Read and written past the caches where they cannot hold it until the next
-  // step: 176M float32 values 915 us through them, 829 past them; 79M with
-  // 8-bit moments (whose codes stay) 255 and 212; but 4.9M values 22 and 24.
+  // step: 176M float32 values 901 us through them, 828 past them; 79M with
+  // 8-bit moments (whose codes stay) 250 and 220; but 4.9M values 22 and 24.
   const bool past_cache = bytes > kCacheBytes;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return copies ? UpdateAll<true>(tensors, num_tensors, *state, *options,

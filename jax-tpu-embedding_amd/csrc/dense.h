@@ -117,8 +117,10 @@ __device__ __forceinline__ void StoreSpan(T* row, const Span<kCut, V>& s,
   }
 }
 
-// Calls that move more than the last cache holds (256 MB) read past it what
-// they read once: 65,536 x 1024 bfloat16 backwards through layer norm 80 us
+// Calls of layer norm's gradient (rows in registers), of the rows to their
+// experts and back, and of AdamW that move more than the last cache holds (256
+// MB) read past it what they read once (the other kernels were not timed that
+// way): 65,536 x 1024 bfloat16 backwards through layer norm 80 us
 // through the caches, 74 past them, the sum of two rows of 1024 for each of
 // 65,536 tokens 77 and 66; but 16,384 x 1024 24 and 27, and 20,011 tokens 20 and
 // 25. Results are always written through the caches, for whoever reads them

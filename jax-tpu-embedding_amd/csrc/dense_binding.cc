@@ -155,8 +155,8 @@ bool HasTangent(const Tensor& t) {
 // constant.
 void CheckTangent(const Tensor& t, const std::string& name) {
   if (HasTangent(t)) {
-    Refuse(name + " carries a tangent: the dense operators have no forward-mode "
-           "derivatives");
+    Refuse(name + " carries a tangent: the dense operators have no "
+                  "forward-mode derivatives");
   }
 }
 
@@ -668,8 +668,9 @@ void Written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// adamw_scalar(x, is_int) -> x, a tensor of one value on a GPU, as a tensor on the
-// current GPU whose memory holds it as float32 or int64 (x itself if it does).
+// adamw_scalar(x, is_int) -> x, a tensor of one value on a GPU, as a tensor on
+// the current GPU whose memory holds it as float32 or int64 (x itself if it
+// does).
 PyObject* AdamwScalar(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
     if (n != 2 || !THPVariable_Check(a[0])) {

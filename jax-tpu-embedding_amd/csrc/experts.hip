@@ -3,10 +3,12 @@
 // back at their tokens, and the gradients.
 //
 // The sort knows both where a choice goes (positions) and where it came from
-// (sources), so every kernel works token by token: it reads a token's row
-// once however many choices it has, writes whole rows, and sums in the order
-// of the choices. Nothing is added atomically. (Row by row of the experts'
-// order, a token's row would be read once for each choice, from anywhere.)
+// (sources), so every kernel works token by token: it reads a token's row once
+// however many choices it has (the weighted sum's gradient loads it for each
+// choice, the first time from memory, then from the caches), writes whole rows,
+// and sums in the order of the choices. Nothing is added atomically. (Row by row
+// of the experts' order, a token's row would be read once for each choice, from
+// anywhere.)
 //
 // The sort is latency: 131,072 choices are 3 MB, and take 5 us to count and 7
 // to place. The rows are HBM-bound. Measured, 65,536 tokens with two of 64

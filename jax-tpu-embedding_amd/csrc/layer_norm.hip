@@ -9,14 +9,14 @@
 //   mean = first + shift, variance = mean(d^2) - shift^2,
 //   xhat = d * rstd - shift * rstd,
 // or every xhat of a row whose mean is large against its deviations would be
-// off by shift * rstd (1024 values of 10,000.3: 0.7 instead of 0). The mean that
-// is returned is float32, and the gradient takes it as it is.
+// off by shift * rstd (1024 values of 10,000.3: 0.7 instead of 0). The mean
+// that is returned is float32, and the gradient takes it as it is.
 // Backwards, h = w * dy loses its mean and its part along xhat,
 //   dx = rstd * (h - mean(h) - xhat * mean(h * xhat)),
 // which takes one pass over the row's registers for both means and one for dx.
 //
 // Both are HBM-bound: 2 values moved per element forwards, 3 backwards, and
-// what the lanes compute fits beside it (VALU busy 0.55 forwards). Measured,
+// what the lanes compute fits beside it (VALU busy 0.65 forwards). Measured,
 // bfloat16 rows with float32 weights: 65,536 x 3328 forwards 165 us, 5.3 TB/s;
 // 65,536 x 1024 backwards 75 us with the reduction, 5.4 TB/s; a device copy
 // moves 4.9 TB/s.
@@ -543,10 +543,11 @@ __global__ __launch_bounds__(256) void NormColumnsLong(NormGradArgs<T> a) {
 
 // Adds the work-groups' sums: kReduceColumns columns a work-group, the `parts`
 // rows of sums in slices that LDS joins in their order, from column `first`
-// on. It is latency alone (12
-// MB at most, from L2): all of a thread's loads are in flight at once. 16
-// columns up to 1024 (100 columns 3.6 us, with 32 a work-group 4.2), then 32
-// (4096 columns 5.8 us, with 16 8.9).
+// on. Up to 1024 columns it is latency alone (6 MB at most, from L2): all of a
+// thread's loads are in flight at once. 4096 columns have up to 25 MB of sums,
+// 16,384 (256 parts) 34 MB, longer rows in proportion. 16 columns up to 1024
+// (100 columns 3.6 us, with 32 a work-group 4.2), then 32 (4096 columns 5.8 us,
+// with 16 8.9).
 template <typename W, int kReduceColumns>
 __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
                                                    int32_t parts, int32_t dim,
@@ -600,12 +601,18 @@ __global__ __launch_bounds__(1024) void NormReduce(const float* partial,
 // Host side.
 // ---------------------------------------------------------------------------
 
-// How a row is laid out over lanes: G lanes of NV vectors each. The fewest
-// lanes that hold the row at 16 values a lane (their weights and, backwards,
-// two sums stay in registers too): lanes past a row's end do nothing (262,144 x
-// 64 bfloat16 backwards 29 us on 16 lanes, 23 on 8). G = 0 for a row that no
-// work-group holds; in passes, 10,000 rows of 16,384 float32 took 406 us
-// forwards and 620 backwards, in registers 230 and 315.
+// How a row is laid out over lanes: G lanes of NV vectors each, at most 16
+// values a lane (their weights and, backwards, two sums stay in registers too).
+// The steps are those below, each the least that holds the row: lanes past a
+// row's end do nothing (262,144 x 64 bfloat16 backwards 29 us on 16 lanes, 23 on
+// 8). They are not the fewest lanes everywhere: 33 to 64 vectors have a lane
+// each, and 16-bit rows of 1025 to 2048 and of 4097 to 8192 columns never reach
+// the second vector of {256, 2} and {1024, 2}, which costs registers alone
+// (32,768 x 2048 bfloat16 47 us forwards, 5.7 TB/s, and 88 backwards, 4.6;
+// 16,384 x 8192 101 and 174, 5.3 and 4.6; one vector a lane was not timed).
+// G = 0 for a row that no work-group holds: in passes, 4096 rows of 20,001
+// float32 take 192 us forwards and 381 backwards, 3.4 and 2.6 TB/s; in registers
+// 10,000 of 16,384 take 227 and 397, 5.8 and 5.0.
 struct Layout {
   int g;
   int nv;
@@ -631,7 +638,8 @@ Layout LayoutOf(int v, int64_t dim) {
 // Work-groups of the backward pass, and so rows of partial sums: three a CU
 // (65,536 x 1024 bfloat16: two 94 us, three 80, four 81; one of 1024 threads),
 // each group of lanes at least one row, and no more bytes of sums written and
-// read than a quarter of what the rows are.
+// read than a quarter of what the rows are (a bound on the traffic; what it
+// does to the latency of a few hundred to a few thousand rows was not timed).
 int64_t BackwardParts(Layout l, int type_bytes, int64_t rows) {
   const int groups = l.g == 0 ? 1 : BlockOf(l.g) / l.g;
   const int64_t most = l.g == 1024 || l.g == 0 ? kCus : 3 * kCus;

@@ -102,6 +102,9 @@ class RankingModel:
     scores, ids = (x @ w["router"]).topk(c.choices, dim=1)
     order = dense.sort_by_expert(ids, c.experts)
     rows = dense.tokens_to_experts(x, order)
+    # The experts' layers are products of sizes that the host gives, so this
+    # waits for the GPU, and a step as written here cannot be captured. A model
+    # with a fixed capacity for each expert needs no such wait.
     first = order.offsets.tolist()
     rows = t.cat([
         t.relu(rows[first[e]:first[e + 1]] @ w["up"][e]) @ w["down"][e]

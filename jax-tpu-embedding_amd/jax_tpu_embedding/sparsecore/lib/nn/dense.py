@@ -126,7 +126,8 @@ def layer_norm(x, weight=None, bias=None, *, epsilon: float = 1e-6,
   weight, bias: [dim], float32 or x's type, the same for both; None: one, zero.
   epsilon: added to the variance.
   return_stats: also return the float32 mean and reciprocal deviation of every
-    row ([...]), which layer_norm_grad takes.
+    row ([...]), which layer_norm_grad takes. They are constants to autograd:
+    no gradient flows through them.
 
   Statistics and products are float32; the result is rounded once. The mean's
   own rounding is taken out of the result, so a row of one value gives the bias
@@ -265,9 +266,9 @@ class AdamWState:
     value on the GPU are not in it: that value is the count.
   bits: 8 or 32.
 
-  A checkpoint keeps these tensors and the step (the value on the GPU, where that
-  counts); a state made for the same weights takes them back with copy_() and
-  `state.step = ...`.
+  A checkpoint keeps these tensors and the step (the value on the GPU, where
+  that counts); a state made for the same weights takes them back with copy_()
+  and `state.step = ...`.
   """
 
   def __init__(self, sizes, decay, bits: int):
@@ -358,10 +359,13 @@ def adamw_update(params, grads, state: AdamWState, *, learning_rate,
   copies: None, or a bfloat16 tensor of each weight's shape (or None) that gets
     the rounded weight: the working copies of float32 weights. Params and
     copies may not share memory, but a bfloat16 weight may be its own copy.
+    Gradients may not share memory with another weight or a copy; that is not
+    checked.
   step: None (state.step + 1), an int, or a single int64 on the GPU, which a
-    captured graph advances itself (an int is the same in every replay). The
-    first step is 1. After an update with a value on the GPU, None is refused
-    until an int is given here or set as state.step.
+    captured graph advances itself (what the host gives, this and every other
+    hyperparameter, is the same in all replays). The first step is 1. After an
+    update with a value on the GPU, None is refused until an int is given here
+    or set as state.step.
   """
   if not (0 <= beta_1 < 1 and 0 <= beta_2 < 1 and epsilon >= 0):
     raise ValueError("beta_1 and beta_2 must be within [0, 1) and epsilon not "
