@@ -710,6 +710,38 @@ int scemb_tokens_from_experts_grad(
     int32_t weights_type, const scemb_expert_order_t* order, void* rows_grad,
     void* weights_grad, void* stream);
 
+/* Products of rows in the order of their experts (scemb_tokens_to_experts)
+ * with each expert's weights: y[r] = rows[r] * W[e] for the rows r of expert e,
+ * [offsets[e], offsets[e + 1]); zeros for rows of none (from
+ * offsets[num_experts] on, which are not read). Sums are float32, rounded once
+ * to the type of all operands. Value (e, i, o) of W [num_experts, inner, outer]
+ * is at e * expert_stride + i * inner_stride + o * outer_stride, one of the last
+ * two being 1; y is [num_rows, outer] contiguous. With inner and outer changed
+ * about it is the gradient of the rows. Offsets do not fall; others reach no
+ * memory past the rows, but what is written is undefined. */
+int scemb_expert_matmul(const void* rows, int32_t type, int64_t rows_stride,
+                        int64_t num_rows, int64_t inner, int64_t outer,
+                        const void* weights, int64_t expert_stride,
+                        int64_t inner_stride, int64_t outer_stride,
+                        const int32_t* offsets, int32_t num_experts, void* y,
+                        void* stream);
+
+/* The weights' gradient, [num_experts, inner, outer] contiguous: the sum over
+ * the expert's rows of rows[r]^T * y_grad[r], zeros for an expert without rows;
+ * in an order that sizes and offsets decide. The workspace size is 0 where none
+ * is needed (and for what the call refuses). */
+size_t scemb_expert_matmul_weights_grad_workspace_size(int32_t type,
+                                                       int64_t num_rows,
+                                                       int64_t inner,
+                                                       int64_t outer,
+                                                       int32_t num_experts);
+int scemb_expert_matmul_weights_grad(
+    const void* rows, int64_t rows_stride, const void* y_grad,
+    int64_t y_grad_stride, int32_t type, int64_t num_rows, int64_t inner,
+    int64_t outer, const int32_t* offsets, int32_t num_experts,
+    void* weights_grad, void* workspace, size_t workspace_bytes,
+    void* stream);
+
 /* AdamW over many tensors. Tensor i's moments are the values from
  * first_i = sum over j < i of numel_j rounded up to SCEMB_ADAMW_BLOCK on.
  * With g = grad * grad_scale and t the step (from 1):

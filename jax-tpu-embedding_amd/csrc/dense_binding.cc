@@ -41,6 +41,10 @@ struct Library {
   decltype(&scemb_tokens_to_experts) tokens_to_experts;
   decltype(&scemb_tokens_from_experts) tokens_from_experts;
   decltype(&scemb_tokens_from_experts_grad) tokens_from_experts_grad;
+  decltype(&scemb_expert_matmul) expert_matmul;
+  decltype(&scemb_expert_matmul_weights_grad_workspace_size)
+      expert_matmul_weights_grad_workspace;
+  decltype(&scemb_expert_matmul_weights_grad) expert_matmul_weights_grad;
   decltype(&scemb_adamw_update) adamw_update;
   decltype(&scemb_adamw_moments) adamw_moments;
 };
@@ -545,6 +549,150 @@ PyObject* TokensFromExpertsGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------------------
+// The experts' products.
+// ---------------------------------------------------------------------------
+
+Tensor OffsetsArg(PyObject* o, int dev) {
+  const Tensor t = TensorOf(o, "order.offsets", dev, kI32);
+  if (t.dim() != 1 || t.size(0) < 2 || t.size(0) > SCEMB_MAX_EXPERTS + 1) {
+    Refuse("order.offsets must have shape [num_experts + 1], got " +
+           Text(t.sizes()));
+  }
+  return t.contiguous();
+}
+
+// The experts' weights, [experts, inner, outer], contiguous along inner or
+// outer (a copy if they are neither).
+struct ExpertWeights {
+  Tensor t;
+  int64_t experts;
+  int64_t inner;
+  int64_t outer;
+  int64_t stride[3];
+
+  ExpertWeights(PyObject* o, const Tensor& offsets, const Tensor& rows,
+                int dev)
+      : t(TensorOf(o, "weights", dev, Bit(rows.scalar_type()))) {
+    experts = offsets.size(0) - 1;
+    if (t.dim() != 3 || t.size(0) != experts || t.size(1) < 1 ||
+        t.size(2) < 1) {
+      Refuse("weights must have shape [" + std::to_string(experts) +
+             ", inner, outer], got " + Text(t.sizes()));
+    }
+    inner = t.size(1);
+    outer = t.size(2);
+    if (outer > 1 && inner > 1 && t.stride(1) != 1 && t.stride(2) != 1) {
+      t = t.contiguous();
+    }
+    // The stride of a dimension of one value says nothing.
+    stride[0] = t.stride(0);
+    stride[1] = inner == 1 ? 1 : t.stride(1);
+    stride[2] = outer == 1 ? 1 : t.stride(2);
+    if (inner == 1 && outer > 1) stride[1] = outer * stride[2];
+    if (outer == 1 && inner > 1) stride[2] = inner * stride[1];
+    if (stride[1] != 1 && stride[2] != 1) {
+      // A single row or column of values that are not neighbours.
+      t = t.contiguous();
+      stride[0] = inner * outer;
+      stride[1] = outer;
+      stride[2] = 1;
+    }
+  }
+  // Stored by output: the gradient is laid out the same.
+  bool ByOuter() const { return stride[2] != 1; }
+};
+
+Tensor MatrixArg(PyObject* o, const char* name, const Tensor& like,
+                 int64_t rows, int64_t columns, int dev) {
+  const Tensor x = TensorOf(o, name, dev, Bit(like.scalar_type()));
+  if (x.dim() != 2 || x.size(0) != rows || x.size(1) != columns) {
+    Refuse(std::string(name) + " must have shape [" + std::to_string(rows) +
+           ", " + std::to_string(columns) + "], got " + Text(x.sizes()));
+  }
+  return x;
+}
+
+Tensor ExpertRows(PyObject* o, int dev) {
+  const Tensor x = TensorOf(o, "rows", dev, kRowTypes);
+  if (x.dim() != 2 || x.size(1) < 1) {
+    Refuse("rows must have shape [choices, inner], got " + Text(x.sizes()));
+  }
+  return x;
+}
+
+void CheckInner(const ExpertWeights& w, const Tensor& rows) {
+  if (w.inner != rows.size(1)) {
+    Refuse("weights must have shape [experts, " + Text(rows.size(1)) +
+           ", outer] for these rows, got " + Text(w.t.sizes()));
+  }
+}
+
+// expert_matmul(rows, weights, offsets) -> y
+PyObject* ExpertMatmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 3) Refuse("expert_matmul takes 3 arguments");
+    const int dev = CurrentDevice();
+    const Tensor x = ExpertRows(a[0], dev);
+    const Tensor offsets = OffsetsArg(a[2], dev);
+    const ExpertWeights w(a[1], offsets, x, dev);
+    CheckInner(w, x);
+    const Rows r = RowsOf(x, w.inner);
+    const Tensor y = New({r.n, w.outer}, x.scalar_type(), x);
+    Check(lib.expert_matmul(
+        r.t.data_ptr(), Code(x.scalar_type()), r.stride, r.n, w.inner, w.outer,
+        w.t.data_ptr(), w.stride[0], w.stride[1], w.stride[2],
+        static_cast<const int32_t*>(offsets.data_ptr()),
+        static_cast<int32_t>(w.experts), y.data_ptr(), Stream(dev)));
+    return Wrap(y);
+  });
+}
+
+// expert_matmul_grad(y_grad, rows, weights, offsets, want_rows, want_weights,
+//                    workspace) -> (drows, dweights)
+PyObject* ExpertMatmulGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 7) Refuse("expert_matmul_grad takes 7 arguments");
+    const int dev = CurrentDevice();
+    const Tensor x = ExpertRows(a[1], dev);
+    const Tensor offsets = OffsetsArg(a[3], dev);
+    const ExpertWeights w(a[2], offsets, x, dev);
+    CheckInner(w, x);
+    const Tensor dy = MatrixArg(a[0], "y_grad", x, x.size(0), w.outer, dev);
+    const Rows g = RowsOf(dy, w.outer);
+    const auto* first = static_cast<const int32_t*>(offsets.data_ptr());
+    const int32_t code = Code(x.scalar_type());
+    const int32_t experts = static_cast<int32_t>(w.experts);
+    Tensor drows, dw;
+    if (a[4] == Py_True) {
+      drows = New({g.n, w.inner}, x.scalar_type(), x);
+      Check(lib.expert_matmul(g.t.data_ptr(), code, g.stride, g.n, w.outer,
+                              w.inner, w.t.data_ptr(), w.stride[0],
+                              w.stride[2], w.stride[1], first, experts,
+                              drows.data_ptr(), Stream(dev)));
+    }
+    if (a[5] == Py_True) {
+      const Rows r = RowsOf(x, w.inner);
+      // The transposed gradient is that of the operands changed about.
+      const bool turned = w.ByOuter();
+      const Rows& left = turned ? g : r;
+      const Rows& right = turned ? r : g;
+      const int64_t inner = turned ? w.outer : w.inner;
+      const int64_t outer = turned ? w.inner : w.outer;
+      dw = New({w.experts, inner, outer}, x.scalar_type(), x);
+      const size_t bytes = lib.expert_matmul_weights_grad_workspace(
+          code, r.n, inner, outer, experts);
+      const Tensor ws = bytes > 0 ? Workspace(a[6], bytes) : Tensor();
+      Check(lib.expert_matmul_weights_grad(
+          left.t.data_ptr(), left.stride, right.t.data_ptr(), right.stride,
+          code, r.n, inner, outer, first, experts, dw.data_ptr(), Data(ws),
+          bytes, Stream(dev)));
+      if (turned) dw = dw.transpose(1, 2);
+    }
+    return Tuple({drows, dw});
+  });
+}
+
+// ---------------------------------------------------------------------------
 // AdamW.
 // ---------------------------------------------------------------------------
 
@@ -860,6 +1008,8 @@ PyMethodDef kMethods[] = {
     SCEMB_METHOD("tokens_to_experts", TokensToExperts),
     SCEMB_METHOD("tokens_from_experts", TokensFromExperts),
     SCEMB_METHOD("tokens_from_experts_grad", TokensFromExpertsGrad),
+    SCEMB_METHOD("expert_matmul", ExpertMatmul),
+    SCEMB_METHOD("expert_matmul_grad", ExpertMatmulGrad),
     SCEMB_METHOD("adamw_sizes", AdamwSizes),
     SCEMB_METHOD("adamw_scalar", AdamwScalar),
     SCEMB_METHOD("adamw_update", AdamwUpdate),

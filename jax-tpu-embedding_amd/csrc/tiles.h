@@ -1,0 +1,414 @@
+// Device helpers of the matrix products (expert_matmul.hip, matmul_8bit.hip):
+// matrix instructions, panels of an operand in LDS, and the tile of a
+// work-group.
+#pragma once
+
+#include "dense.h"
+
+namespace scemb {
+
+using F32x4 = float __attribute__((ext_vector_type(4)));
+using U32x4 = uint32_t __attribute__((ext_vector_type(4)));
+
+using LdsBytes = __attribute__((address_space(3))) void*;
+
+// Memory from a pointer on that is the same for all lanes. Lanes add 32 bits,
+// which stay in registers of their own: a register that held an address and is
+// written again first waits for the load.
+struct Memory {
+  __amdgpu_buffer_rsrc_t rsrc;
+
+  explicit __device__ __forceinline__ Memory(const void* p) {
+    uint64_t at = reinterpret_cast<uint64_t>(p);
+    asm("" : "+s"(at));
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at), 0,
+                                             0xffffffff, 0x00020000);
+  }
+  // 16 bytes a lane straight to LDS; the wavefront's land one after another
+  // from `lds` on, which is the same for all its lanes.
+  __device__ __forceinline__ void ToLds(uint32_t offset, char* lds) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsBytes)lds, 16,
+                                             static_cast<int>(offset), 0, 0,
+                                             0);
+  }
+};
+
+// No memory access moves across, and all of this wavefront's loads have landed
+// but the last `kNewer`.
+template <int kNewer>
+__device__ __forceinline__ void WaitLoads() {
+  static_assert(kNewer >= 0 && kNewer < 64, "a count of six bits");
+  asm volatile("" ::: "memory");
+  // vmcnt in bits [3:0] and [15:14], the other counters at their largest.
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kNewer & 15) | (kNewer >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+
+// All wavefronts of the work-group are here; LDS that they read before is free,
+// what they waited for is in LDS.
+__device__ __forceinline__ void Barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): LDS accesses are done
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Panels: `kOuter` rows or columns of an operand by 128 bytes of the sum's
+// index ("depth"), in LDS.
+//
+// kDepth: neighbours in memory are neighbours along the depth. A row is 128
+// bytes, its 16-byte chunks permuted by the row so that the 8 lanes that read
+// one chunk of 8 rows find them in different banks.
+// kOuter: neighbours in memory are neighbours along the outer index. LDS holds
+// a row for each depth index, its chunks permuted by the depth index; reading
+// transposes (16 bits) or gathers (32 bits).
+// ---------------------------------------------------------------------------
+
+enum class Along { kDepth, kOuter };
+
+template <typename T, Along kAlong, int kOuter, int kThreads>
+struct Panel {
+  static constexpr int kBytes = kOuter * 128;
+  static constexpr int kDepth = 128 / sizeof(T);
+  static constexpr int kEach = 16 / sizeof(T);  // elements of a chunk
+  static constexpr int kPer = kBytes / 16 / kThreads;  // chunks of a thread
+  static constexpr int kRowChunks =
+      kAlong == Along::kDepth ? 8 : kOuter * sizeof(T) / 16;
+  static_assert(kPer >= 1 && kPer * 16 * kThreads == kBytes, "whole chunks");
+  static_assert(kThreads % kRowChunks == 0, "a thread's chunks share a column");
+
+  // What chunk numbers of LDS row `row` are XORed with.
+  static __device__ __forceinline__ int Key(int row) {
+    if constexpr (kAlong == Along::kDepth) return row & 7;
+    if constexpr (sizeof(T) == 4) {
+      // Lanes of four rows 4 apart read 64 bytes each.
+      return ((row >> 2) & 3) << 2;
+    }
+    // Lanes of rows 0-3, and of those 8 later, read 32 bytes each.
+    return (((row & 3) | ((row >> 3) & 1) << 2) << 1) & (kRowChunks - 1);
+  }
+
+  // The thread's chunk i: its row in LDS, and which chunk of that row in
+  // memory.
+  static __device__ __forceinline__ int Row(int i) {
+    return i * (kThreads / kRowChunks) + threadIdx.x / kRowChunks;
+  }
+  static __device__ __forceinline__ int Column(int i) {
+    return (threadIdx.x % kRowChunks) ^ Key(Row(i));
+  }
+  static __device__ __forceinline__ char* Place(char* lds, int i) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    return lds + (i * kThreads + wave * kWave) * 16;
+  }
+
+  // --- Straight to LDS: chunks are aligned, and none ends past the last
+  // element. ---
+
+  uint32_t offset[kPer];  // of chunk i from the panel's first element, bytes
+
+  // outer >= 1: the outer indices that exist. Others get some that do, and
+  // their results are not stored.
+  __device__ __forceinline__ void Start(int64_t stride, int outer) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (kAlong == Along::kDepth) {
+        offset[i] = static_cast<uint32_t>(min(Row(i), outer - 1)) *
+                        static_cast<uint32_t>(stride * sizeof(T)) +
+                    Column(i) * 16;
+      } else {
+        const int c = Column(i);
+        offset[i] = static_cast<uint32_t>(Row(i)) *
+                        static_cast<uint32_t>(stride * sizeof(T)) +
+                    (c * kEach < outer ? c : 0) * 16;
+      }
+    }
+  }
+
+  // All of the panel's depth exists.
+  __device__ __forceinline__ void Load(const char* from, char* lds) const {
+    const Memory memory(from);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) memory.ToLds(offset[i], Place(lds, i));
+  }
+
+  // --- Through registers: any alignment, any number of elements (kWhole: of
+  // whole chunks). ---
+
+  struct Chunks {
+    Vec<T, kEach> v[kPer];
+  };
+  template <bool kWhole>
+  static __device__ __forceinline__ void Fetch(const T* from, int64_t stride,
+                                               int outer, int left,
+                                               Chunks* to) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = Column(i) * kEach;
+      const int row = Row(i);
+      // Elements of the row that exist from c on.
+      int have = (kAlong == Along::kDepth ? left : outer) - c;
+      if (row >= (kAlong == Along::kDepth ? outer : left)) have = 0;
+      const T* p = from + row * stride + c;
+      if constexpr (kWhole) {
+        // Absent chunks load one that exists.
+        const auto x = LoadVec<T, kEach>(have > 0 ? p : from);
+        to->v[i] = __builtin_bit_cast(
+            Vec<T, kEach>, have > 0 ? __builtin_bit_cast(U32x4, x)
+                                    : U32x4{0, 0, 0, 0});
+      } else if (have >= kEach) {
+        to->v[i] = LoadVec<T, kEach>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          to->v[i].v[j] = j < have ? p[j] : static_cast<T>(0.f);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void Put(const Chunks& from, char* lds) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      *reinterpret_cast<U32x4*>(lds + (i * kThreads + threadIdx.x) * 16) =
+          __builtin_bit_cast(U32x4, from.v[i]);
+    }
+  }
+
+  // --- Fragments: 16 outer indices from `outer` on by 64 bytes of depth (half
+  // 0 or 1). A lane gets outer index lane % 16 and 16 bytes of depth: elements
+  // [(lane / 16) * kEach, + kEach) of the half. ---
+
+  static __device__ __forceinline__ U32x4 Fragment(const char* lds, int outer,
+                                                   int half) {
+    const int lane = threadIdx.x % kWave;
+    const int i = lane % 16, g = lane / 16;
+    if constexpr (kAlong == Along::kDepth) {
+      const int row = outer + i;
+      return *reinterpret_cast<const U32x4*>(
+          lds + row * 128 + (((half * 4 + g) ^ Key(i)) * 16));
+    } else if constexpr (sizeof(T) == 4) {
+      U32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = half * 16 + g * 4 + j;
+        const int c = (outer + i) / 4;
+        v[j] = *reinterpret_cast<const uint32_t*>(
+            lds + row * (kRowChunks * 16) + ((c ^ Key(g * 4)) * 16) +
+            (i % 4) * 4);
+      }
+      return v;
+    } else {
+      // Four lanes address four neighbours each of one depth index, 16 lanes
+      // four depth indices; lane i gets the four of outer index i.
+      using S16x4 = short __attribute__((ext_vector_type(4)));
+      using S16x4Lds = __attribute__((address_space(3))) S16x4;
+      uint2 part[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int in = g * 8 + j * 4 + i / 4;  // Key ignores multiples of 16
+        const int row = half * 32 + in;
+        const int c = outer / 8 + (i % 4) / 2;
+        part[j] = __builtin_bit_cast(
+            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (S16x4Lds*)(lds + row * (kRowChunks * 16) +
+                                   ((c ^ Key(in)) * 16) + (i % 2) * 8)));
+      }
+      return U32x4{part[0].x, part[0].y, part[1].x, part[1].y};
+    }
+  }
+};
+
+// acc[n][m] += sum over 64 bytes of depth of b[n] * a[m], for 16 of each. A
+// lane holds n = 4 * (lane / 16) + (0 to 3) of m = lane % 16.
+template <typename T>
+__device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
+                                            F32x4* acc) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bj = b[j], aj = a[j];
+      *acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+          __builtin_bit_cast(float, bj), __builtin_bit_cast(float, aj), *acc,
+          0, 0, 0);
+    }
+  } else if constexpr (__is_same(T, bf16)) {
+    using V = bf16 __attribute__((ext_vector_type(8)));
+    *acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(V, b), __builtin_bit_cast(V, a), *acc, 0, 0, 0);
+  } else {
+    using V = f16 __attribute__((ext_vector_type(8)));
+    *acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(V, b), __builtin_bit_cast(V, a), *acc, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows in segments: those of expert e are [offsets[e], offsets[e + 1]); the
+// ones behind the last belong to no expert.
+// ---------------------------------------------------------------------------
+
+// The rows of segment s, inside [0, n) whatever the offsets hold; segment
+// `experts` is the rows of none.
+struct Segment {
+  int32_t begin;
+  int32_t end;
+};
+__device__ __forceinline__ Segment SegmentOf(const int32_t* offsets,
+                                             int32_t experts, int32_t n,
+                                             int32_t s) {
+  const int32_t begin = min(max(offsets[s], 0), n);
+  const int32_t end = s < experts ? max(min(offsets[s + 1], n), begin) : n;
+  return {begin, end};
+}
+
+// The rows [row, end) of the tile'th tile, and its segment (-1: no such tile).
+// Every wavefront finds it by itself: a lane counts the tiles of neighbouring
+// segments, the lanes' counts are added up.
+struct RowTile {
+  int32_t segment;
+  int32_t row;
+  int32_t end;
+};
+template <int kRows>
+__device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
+                                               int32_t experts, int32_t n,
+                                               int32_t tile) {
+  const int per = experts / kWave + 1;  // segments of a lane, experts + 1 in all
+  const int first = LaneId() * per;
+  int32_t count = 0;
+  for (int i = 0; i < per; ++i) {
+    if (first + i <= experts) {
+      const Segment s = SegmentOf(offsets, experts, n, first + i);
+      count += (s.end - s.begin + kRows - 1) / kRows;
+    }
+  }
+  const int32_t upto = WaveInclusiveScan(count);
+  const uint64_t past = __ballot(upto > tile);
+  if (past == 0) return {-1, 0, 0};
+  const int who = __builtin_ctzll(past);
+  int32_t at = tile - __builtin_amdgcn_readlane(upto - count, who);
+  for (int i = who * per;; ++i) {
+    const Segment s = SegmentOf(offsets, experts, n, i);
+    const int32_t tiles = (s.end - s.begin + kRows - 1) / kRows;
+    if (at < tiles || i == experts) {
+      return {__builtin_amdgcn_readfirstlane(i),
+              __builtin_amdgcn_readfirstlane(s.begin + at * kRows),
+              __builtin_amdgcn_readfirstlane(s.end)};
+    }
+    at -= tiles;
+  }
+}
+
+// Tiles of a matrix in the order of the work-groups. Work-groups go to the
+// eight XCDs in turn; each XCD gets patches of up to 32 tiles, one for each of
+// its CUs, that share operands in its L2.
+struct TileGrid {
+  static constexpr int32_t kMost = 1 << 30;
+  int32_t rows;     // tiles
+  int32_t columns;
+  int32_t patch_rows;
+  int32_t patch_columns;
+
+  // More than a launch takes are cut: Groups() says so then.
+  TileGrid(int64_t r, int64_t c)
+      : rows(static_cast<int32_t>(r < kMost ? r : kMost)),
+        columns(static_cast<int32_t>(c < kMost ? c : kMost)) {
+    patch_columns = columns < 8 ? columns : 8;
+    patch_rows = 32 / patch_columns;
+    if (patch_rows > rows) patch_rows = rows;
+  }
+  int64_t Groups() const {
+    const int64_t patches =
+        CeilDiv(rows, patch_rows) * CeilDiv(columns, patch_columns);
+    return RoundUp(patches, 8) * patch_rows * patch_columns;
+  }
+  // False: no such tile.
+  __device__ __forceinline__ bool Tile(uint32_t group, int32_t* row,
+                                       int32_t* column) const {
+    const uint32_t size = patch_rows * patch_columns;
+    const uint32_t xcd = group % 8, within = group / 8 % size;
+    const uint32_t patch = group / 8 / size * 8 + xcd;
+    const uint32_t across = (columns + patch_columns - 1) / patch_columns;
+    *row = patch / across * patch_rows + within % patch_rows;
+    *column = patch % across * patch_columns + within / patch_rows;
+    return *row < rows && *column < columns;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Results.
+// ---------------------------------------------------------------------------
+
+// x[j] of lane group g (16 lanes each) and x[g] of lane group j change places.
+__device__ __forceinline__ void TransposeGroups(uint32_t x[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x[j], x[j + 2], false,
+                                                    false);
+    x[j] = r[0];
+    x[j + 2] = r[1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x[j], x[j + 1], false,
+                                                    false);
+    x[j] = r[0];
+    x[j + 1] = r[1];
+  }
+}
+
+// Elements [column, column + V) of a row, those below `columns`.
+template <typename T, int V>
+__device__ __forceinline__ void StoreUpTo(T* row, int32_t column,
+                                          int32_t columns,
+                                          const Vec<T, V>& x) {
+  if (column + V <= columns) {
+    StoreVec<T, V>(row + column, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (column + j < columns) row[column + j] = x.v[j];
+    }
+  }
+}
+
+// 64 columns of a row from the accumulators of four fragments, rounded once.
+// With 16 bits a lane gathers 16 neighbours from the other groups of lanes and
+// writes 32 bytes; with 32 bits it writes 16 bytes of each fragment.
+template <typename T>
+__device__ __forceinline__ void StoreColumns(T* row, bool exists,
+                                             int32_t column, int32_t columns,
+                                             const F32x4 acc[4]) {
+  const int g = threadIdx.x % kWave / 16;
+  if constexpr (sizeof(T) == 4) {
+    if (!exists) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      StoreUpTo(row, column + j * 16 + g * 4, columns,
+                __builtin_bit_cast(Vec<T, 4>, acc[j]));
+    }
+  } else {
+    uint32_t x[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      Vec<T, 4> v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.v[i] = static_cast<T>(acc[j][i]);
+      const uint2 u = __builtin_bit_cast(uint2, v);
+      x[0][j] = u.x;
+      x[1][j] = u.y;
+    }
+    TransposeGroups(x[0]);
+    TransposeGroups(x[1]);
+    if (!exists) return;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const U32x4 v = {x[0][2 * j], x[1][2 * j], x[0][2 * j + 1],
+                       x[1][2 * j + 1]};
+      StoreUpTo(row, column + g * 16 + j * 8, columns,
+                __builtin_bit_cast(Vec<T, 8>, v));
+    }
+  }
+}
+
+}  // namespace scemb

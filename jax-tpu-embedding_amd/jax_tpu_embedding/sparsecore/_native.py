@@ -88,6 +88,9 @@ EXPORTED_SYMBOLS = (
     "scemb_tokens_to_experts",
     "scemb_tokens_from_experts",
     "scemb_tokens_from_experts_grad",
+    "scemb_expert_matmul",
+    "scemb_expert_matmul_weights_grad_workspace_size",
+    "scemb_expert_matmul_weights_grad",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )
@@ -425,6 +428,9 @@ _DENSE_FUNCTIONS = (
     "scemb_tokens_to_experts",
     "scemb_tokens_from_experts",
     "scemb_tokens_from_experts_grad",
+    "scemb_expert_matmul",
+    "scemb_expert_matmul_weights_grad_workspace_size",
+    "scemb_expert_matmul_weights_grad",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )

@@ -108,7 +108,24 @@ def _function(name: str):
         return (drows if need[0] else None, dw if need[1] else None, None,
                 None)
 
-    _functions.update(norm=LayerNorm, to=ToExperts, back=FromExperts)
+    class Product(t.autograd.Function):
+
+      @staticmethod
+      def forward(ctx, rows, weights, offsets):
+        ctx.save_for_backward(rows, weights, offsets)
+        return _calls().expert_matmul(rows, weights, offsets)
+
+      @staticmethod
+      @once
+      def backward(ctx, y_grad):
+        rows, weights, offsets = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*_calls().expert_matmul_grad(y_grad, rows, weights, offsets,
+                                             need[0], need[1], _workspace),
+                None)
+
+    _functions.update(norm=LayerNorm, to=ToExperts, back=FromExperts,
+                      product=Product)
   return _functions[name]
 
 
@@ -240,6 +257,42 @@ def tokens_from_experts_grad(y_grad, rows, weights, order: ExpertOrder):
   """
   return _calls().tokens_from_experts_grad(y_grad, rows, weights,
                                            order.positions, order.offsets)
+
+
+def expert_matmul(rows, weights, order: ExpertOrder):
+  """Every expert's rows times its weights, [choices in all, outer]: row r of
+  expert e is rows[r] @ weights[e].
+
+  rows: [choices in all, inner] in the order of their experts, as
+    tokens_to_experts returns them; float32, bfloat16 or float16. Rows of
+    dropped choices are not read and give zeros.
+  weights: [experts, inner, outer] of rows' type. Either of the last two
+    dimensions may be the contiguous one (others are copied first), so weights
+    stored by output are given as their transpose.
+  order: sort_by_expert's; only its offsets are used, on the GPU: nothing waits
+    for the experts' numbers of rows.
+
+  Sums are float32, rounded once. float32 products are exact to float32's own
+  rounding (no shortened operands).
+  """
+  calls = _calls()
+  if calls.wants_grad(rows, weights):
+    return _function("product").apply(rows, weights, order.offsets)
+  return calls.expert_matmul(rows, weights, order.offsets)
+
+
+def expert_matmul_grad(y_grad, rows, weights, order: ExpertOrder, *,
+                       with_rows: bool = True, with_weights: bool = True):
+  """Gradients of expert_matmul: (of rows, of weights), of their types; None
+  for one that is not wanted.
+
+  Rows of dropped choices get zeros, and so do the weights of an expert without
+  rows. The weights' gradient is laid out in memory as the weights are; its sum
+  over the rows is float32, in an order that the sizes and the order decide.
+  """
+  return _calls().expert_matmul_grad(y_grad, rows, weights, order.offsets,
+                                     bool(with_rows), bool(with_weights),
+                                     _workspace)
 
 
 # ---------------------------------------------------------------------------
