@@ -8,23 +8,34 @@ namespace scemb {
 namespace {
 
 // ---------------------------------------------------------------------------
-// A tile of the result by one work-group of kWavesM x kWavesN wavefronts.
+// A tile of the result by one work-group of kWavesM x kWavesN wavefronts. LDS
+// is a ring of kSlots steps of 64 bytes of depth: while one is multiplied the
+// next two are there or on their way, and the one after those is asked for.
 // ---------------------------------------------------------------------------
+
+constexpr int kSlots = 4;
+#define SCEMB_SLOTS(bytes)                                  \
+  __shared__ __attribute__((aligned(16))) char slot0[bytes]; \
+  __shared__ __attribute__((aligned(16))) char slot1[bytes]; \
+  __shared__ __attribute__((aligned(16))) char slot2[bytes]; \
+  __shared__ __attribute__((aligned(16))) char slot3[bytes]
 
 template <typename T_, Along kA, Along kB, int kM_, int kN_, int kWavesM,
           int kWavesN, bool kDirect_>
 struct Tile {
   using T = T_;
   static constexpr int kM = kM_, kN = kN_;
-  static constexpr int kThreads = kWavesM * kWavesN * kWave;
+  static constexpr int kWaves = kWavesM * kWavesN;
+  static constexpr int kThreads = kWaves * kWave;
   static constexpr bool kDirect = kDirect_;
   static constexpr int kFragM = kM / kWavesM / 16;
   static constexpr int kFragN = kN / kWavesN / 16;
-  static_assert(kFragN == 4, "results are stored by 64 columns");
+  static_assert(kFragN % 4 == 0, "results are stored by 64 columns");
   using A = Panel<T, kA, kM, kThreads>;
   using B = Panel<T, kB, kN, kThreads>;
   static constexpr int kDepth = A::kDepth;
   static constexpr int kLds = A::kBytes + B::kBytes;
+  static constexpr int kLoads = A::kPer + B::kPer;  // of a thread and step
   static constexpr Along kAlongA = kA, kAlongB = kB;
 
   F32x4 acc[kFragM][kFragN];
@@ -38,57 +49,36 @@ struct Tile {
            (kFragN * 16);
   }
 
-  // One step of the depth from `lds`. Transposing reads are all made before
-  // `then`, which starts the loads of a later step: the compiler does not know
-  // that they do not read what those write, and would wait for them.
-  template <typename F>
-  __device__ __forceinline__ void Step(const char* lds, const F& then) {
-    constexpr bool kFirstA = kA == Along::kOuter && sizeof(T) == 2;
-    constexpr bool kFirstB = kB == Along::kOuter && sizeof(T) == 2;
-    const char* lds_b = lds + A::kBytes;
-    U32x4 a[2][kFragM], b[2][kFragN];
-    const auto read_a = [&](int half) __attribute__((always_inline)) {
+  struct Fragments {
+    U32x4 a[kFragM];
+    U32x4 b[kFragN];
+  };
+  static __device__ __forceinline__ void Read(const char* lds, Fragments* f) {
 #pragma unroll
-      for (int i = 0; i < kFragM; ++i) {
-        a[half][i] = A::Fragment(lds, WaveM() + i * 16, half);
-      }
-    };
-    const auto read_b = [&](int half) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < kFragN; ++j) {
-        b[half][j] = B::Fragment(lds_b, WaveN() + j * 16, half);
-      }
-    };
-    if constexpr (kFirstB) {
-      read_b(0);
-      read_b(1);
+    for (int j = 0; j < kFragN; ++j) {
+      f->b[j] = B::Fragment(lds, A::kBytes, WaveN() + j * 16);
     }
-    if constexpr (kFirstA) {
-      read_a(0);
-      read_a(1);
+#pragma unroll
+    for (int i = 0; i < kFragM; ++i) {
+      f->a[i] = A::Fragment(lds, 0, WaveM() + i * 16);
     }
-    then();
+  }
+  __device__ __forceinline__ void Multiply(const Fragments& f) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if constexpr (!kFirstB) read_b(half);
-      if constexpr (!kFirstA) read_a(half);
+    for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
-      for (int i = 0; i < kFragM; ++i) {
-#pragma unroll
-        for (int j = 0; j < kFragN; ++j) {
-          MultiplyAdd<T>(b[half][j], a[half][i], &acc[i][j]);
-        }
-      }
+      for (int j = 0; j < kFragN; ++j) MultiplyAdd<T>(f.b[j], f.a[i], &acc[i][j]);
     }
   }
 
   // The tile's sums over `depth`. a and b are the panels' first elements; m and
-  // n (at least 1) the outer indices that exist. lds0 and lds1 are different
-  // arrays of kLds bytes: the compiler has to see that a load into one needs no
-  // wait before the other is read.
+  // n (at least 1) the outer indices that exist. The slots are different
+  // arrays: the compiler has to see that a load into one needs no wait before
+  // another is read.
   __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
                                       const T* b, int64_t b_stride, int n,
-                                      int32_t depth, char* lds0, char* lds1) {
+                                      int32_t depth, char* slot0, char* slot1,
+                                      char* slot2, char* slot3) {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
@@ -106,6 +96,12 @@ struct Tile {
       pb.Start(b_stride, n);
       const char* at_a = reinterpret_cast<const char*>(a);
       const char* at_b = reinterpret_cast<const char*>(b);
+      const auto load = [&](char* slot) __attribute__((always_inline)) {
+        pa.Load(at_a, slot);
+        pb.Load(at_b, slot + A::kBytes);
+        at_a += a_step * sizeof(T);
+        at_b += b_step * sizeof(T);
+      };
       // What is no whole step comes first, through registers.
       int32_t left = depth % kDepth;
       if (left != 0) {
@@ -113,44 +109,75 @@ struct Tile {
         typename B::Chunks cb;
         A::template Fetch<true>(a, a_stride, m, left, &ca);
         B::template Fetch<true>(b, b_stride, n, left, &cb);
-        A::Put(ca, lds0);
-        B::Put(cb, lds0 + A::kBytes);
+        A::Put(ca, slot0);
+        B::Put(cb, slot0 + A::kBytes);
+        at_a += a_step / kDepth * left * sizeof(T);
+        at_b += b_step / kDepth * left * sizeof(T);
       } else {
         left = kDepth;
-        pa.Load(at_a, lds0);
-        pb.Load(at_b, lds0 + A::kBytes);
+        load(slot0);
       }
-      at_a += a_step / kDepth * left * sizeof(T);
-      at_b += b_step / kDepth * left * sizeof(T);
-      int32_t steps = (depth - left) / kDepth;  // that are not yet loaded
-      const auto turn = [&](char* now, char* next) __attribute__((
-                            always_inline)) {
+      // Steps that are not multiplied, and of those what is not asked for.
+      int32_t steps = 1 + (depth - left) / kDepth;
+      int32_t ahead = steps - 3;
+      if (steps > 1) load(slot1);
+      if (steps > 2) load(slot2);
+      if (ahead >= 0) {
+        WaitLoads<2 * kLoads>();
+      } else {
         WaitLoads<0>();
-        Barrier();
-        Step(now, [&]() __attribute__((always_inline)) {
-          pa.Load(at_a, next);
-          pb.Load(at_b, next + A::kBytes);
-          at_a += a_step * sizeof(T);
-          at_b += b_step * sizeof(T);
-        });
-      };
-      for (; steps >= 2; steps -= 2) {
-        turn(lds0, lds1);
-        turn(lds1, lds0);
       }
-      if (steps == 1) turn(lds0, lds1);
-      WaitLoads<0>();
       Barrier();
-      Step(steps == 1 ? lds1 : lds0, [] {});
+      // With two wavefronts a SIMD one reads while the other multiplies: the
+      // second half of them are a barrier behind.
+      constexpr bool kTurns = kWaves == 8;
+      const bool second =
+          __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) >= kWaves / 2;
+      if (kTurns && second) Barrier();
+      const auto turn = [&](const char* now, char* free) __attribute__((
+                            always_inline)) {
+        if (ahead > 0) load(free);
+        Fragments f;
+        Read(now, &f);
+        // The next step is there.
+        if (ahead > 0) {
+          WaitLoads<2 * kLoads>();
+        } else {
+          WaitLoads<0>();
+        }
+        --ahead;
+        if constexpr (kTurns) {
+          Barrier();
+          __builtin_amdgcn_s_setprio(1);
+          Multiply(f);
+          __builtin_amdgcn_s_setprio(0);
+          Barrier();
+        } else {
+          __builtin_amdgcn_sched_barrier(0);
+          Multiply(f);
+          __builtin_amdgcn_sched_barrier(0);
+          Barrier();
+        }
+      };
+      for (; steps >= 4; steps -= 4) {
+        turn(slot0, slot3);
+        turn(slot1, slot0);
+        turn(slot2, slot1);
+        turn(slot3, slot2);
+      }
+      if (steps >= 1) turn(slot0, slot3);
+      if (steps >= 2) turn(slot1, slot0);
+      if (steps >= 3) turn(slot2, slot1);
+      if (kTurns && !second) Barrier();
     } else {
       typename A::Chunks ca;
       typename B::Chunks cb;
       A::template Fetch<false>(a, a_stride, m, depth, &ca);
       B::template Fetch<false>(b, b_stride, n, depth, &cb);
       for (int32_t at = 0; at < depth; at += kDepth) {
-        char* lds = (at / kDepth & 1) ? lds1 : lds0;
-        A::Put(ca, lds);
-        B::Put(cb, lds + A::kBytes);
+        char* slot = (at / kDepth & 1) ? slot1 : slot0;
+        A::Put(ca, slot);
+        B::Put(cb, slot + A::kBytes);
         __syncthreads();
         a += a_step;
         b += b_step;
@@ -158,7 +185,9 @@ struct Tile {
           A::template Fetch<false>(a, a_stride, m, depth - at - kDepth, &ca);
           B::template Fetch<false>(b, b_stride, n, depth - at - kDepth, &cb);
         }
-        Step(lds, [] {});
+        Fragments f;
+        Read(slot, &f);
+        Multiply(f);
       }
     }
   }
@@ -170,7 +199,11 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
       const int row = WaveM() + i * 16 + threadIdx.x % 16;
-      StoreColumns(c + row * stride, row < m, WaveN(), n, acc[i]);
+#pragma unroll
+      for (int j = 0; j < kFragN; j += 4) {
+        StoreColumns(c + row * stride, row < m, WaveN() + j * 16, n,
+                     &acc[i][j]);
+      }
     }
   }
 };
@@ -183,13 +216,12 @@ struct Weights {
 
 // y[r] = x[r] * W[expert of r] for rows in segments; zeros for rows of none.
 template <typename C>
-__global__ __launch_bounds__(C::kThreads) void RowsKernel(
+__global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
     const typename C::T* x, int64_t x_stride, int32_t rows, int32_t depth,
     Weights w, int32_t columns, const int32_t* offsets, int32_t experts,
     typename C::T* y, TileGrid grid) {
   using T = typename C::T;
-  __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
-  __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
+  SCEMB_SLOTS(C::kLds);
   int32_t tile, column;
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
   const RowTile t = FindRowTile<C::kM>(offsets, experts, rows, tile);
@@ -201,20 +233,19 @@ __global__ __launch_bounds__(C::kThreads) void RowsKernel(
   const T* b = static_cast<const T*>(w.data) + t.segment * w.expert +
                (C::kAlongB == Along::kDepth ? column * w.stride : column);
   c.Run(x + t.row * x_stride, x_stride, m, b, w.stride, n,
-        t.segment < experts ? depth : 0, lds0, lds1);
+        t.segment < experts ? depth : 0, slot0, slot1, slot2, slot3);
   c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n);
 }
 
 // dw[e] = the sum over the segment's rows of x[r]^T dy[r], or part `split` of
 // `splits` of the rows in float32.
 template <typename C, typename Out>
-__global__ __launch_bounds__(C::kThreads) void WeightsKernel(
+__global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
     const typename C::T* x, int64_t x_stride, int32_t inner,
     const typename C::T* dy, int64_t dy_stride, int32_t outer, int32_t rows,
     const int32_t* offsets, int32_t experts, Out* dw, int32_t splits,
     TileGrid grid) {
-  __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
-  __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
+  SCEMB_SLOTS(C::kLds);
   int32_t tile, column;
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
   const int32_t tiles = (inner + C::kM - 1) / C::kM;
@@ -232,8 +263,8 @@ __global__ __launch_bounds__(C::kThreads) void WeightsKernel(
   const int n = min(outer - column, C::kN);
   C c;
   c.Run(x + s.begin * x_stride + row, x_stride, m,
-        dy + s.begin * dy_stride + column, dy_stride, n, s.end - s.begin, lds0,
-        lds1);
+        dy + s.begin * dy_stride + column, dy_stride, n, s.end - s.begin,
+        slot0, slot1, slot2, slot3);
   c.Store(dw + (static_cast<int64_t>(part) * inner + row) * outer + column,
           outer, m, n);
 }
@@ -359,11 +390,11 @@ WeightsPlan PlanWeights(int bytes, int64_t rows, int64_t inner, int64_t outer,
   };
   p.large = bytes == 2 && tiles(256) >= kCus;
   const int64_t have = tiles(p.large ? 256 : 128);
-  const int64_t steps = rows / experts / (128 / bytes);
+  const int64_t steps = rows / experts / (64 / bytes);
   const int64_t most = static_cast<int64_t>(
       (64 << 20) / (4.0 * experts * inner * outer));
   const int64_t splits =
-      std::min({CeilDiv(2 * kCus, have), steps / 4, most, int64_t{1024}});
+      std::min({CeilDiv(2 * kCus, have), steps / 8, most, int64_t{1024}});
   p.splits = static_cast<int32_t>(std::max<int64_t>(splits, 1));
   return p;
 }

@@ -19,8 +19,13 @@ struct Memory {
   __amdgpu_buffer_rsrc_t rsrc;
 
   explicit __device__ __forceinline__ Memory(const void* p) {
-    uint64_t at = reinterpret_cast<uint64_t>(p);
-    asm("" : "+s"(at));
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint64_t at =
+        static_cast<uint64_t>(static_cast<uint32_t>(
+            __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))))
+            << 32 |
+        static_cast<uint32_t>(
+            __builtin_amdgcn_readfirstlane(static_cast<int>(v)));
     rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at), 0,
                                              0xffffffff, 0x00020000);
   }
@@ -54,12 +59,12 @@ __device__ __forceinline__ void Barrier() {
 }
 
 // ---------------------------------------------------------------------------
-// Panels: `kOuter` rows or columns of an operand by 128 bytes of the sum's
-// index ("depth"), in LDS.
+// Panels: `kOuter` rows or columns of an operand by 64 bytes of the sum's index
+// ("depth"), in LDS.
 //
-// kDepth: neighbours in memory are neighbours along the depth. A row is 128
-// bytes, its 16-byte chunks permuted by the row so that the 8 lanes that read
-// one chunk of 8 rows find them in different banks.
+// kDepth: neighbours in memory are neighbours along the depth. A row is 64
+// bytes, its four 16-byte chunks permuted so that 8 lanes that read one chunk
+// of 8 rows find them in different banks.
 // kOuter: neighbours in memory are neighbours along the outer index. LDS holds
 // a row for each depth index, its chunks permuted by the depth index; reading
 // transposes (16 bits) or gathers (32 bits).
@@ -69,18 +74,18 @@ enum class Along { kDepth, kOuter };
 
 template <typename T, Along kAlong, int kOuter, int kThreads>
 struct Panel {
-  static constexpr int kBytes = kOuter * 128;
-  static constexpr int kDepth = 128 / sizeof(T);
+  static constexpr int kBytes = kOuter * 64;
+  static constexpr int kDepth = 64 / sizeof(T);
   static constexpr int kEach = 16 / sizeof(T);  // elements of a chunk
   static constexpr int kPer = kBytes / 16 / kThreads;  // chunks of a thread
   static constexpr int kRowChunks =
-      kAlong == Along::kDepth ? 8 : kOuter * sizeof(T) / 16;
+      kAlong == Along::kDepth ? 4 : kOuter * sizeof(T) / 16;
   static_assert(kPer >= 1 && kPer * 16 * kThreads == kBytes, "whole chunks");
   static_assert(kThreads % kRowChunks == 0, "a thread's chunks share a column");
 
   // What chunk numbers of LDS row `row` are XORed with.
   static __device__ __forceinline__ int Key(int row) {
-    if constexpr (kAlong == Along::kDepth) return row & 7;
+    if constexpr (kAlong == Along::kDepth) return (row >> 1) & 3;
     if constexpr (sizeof(T) == 4) {
       // Lanes of four rows 4 apart read 64 bytes each.
       return ((row >> 2) & 3) << 2;
@@ -174,27 +179,27 @@ struct Panel {
     }
   }
 
-  // --- Fragments: 16 outer indices from `outer` on by 64 bytes of depth (half
-  // 0 or 1). A lane gets outer index lane % 16 and 16 bytes of depth: elements
-  // [(lane / 16) * kEach, + kEach) of the half. ---
+  // --- Fragments: 16 outer indices from `outer` on. A lane gets outer index
+  // lane % 16 and 16 bytes of depth, from element (lane / 16) * kEach on. The
+  // panel begins `first` bytes into `lds`. (An address is the array and one sum:
+  // the compiler follows no long chain to the array, and would wait for loads
+  // into other ones.) ---
 
-  static __device__ __forceinline__ U32x4 Fragment(const char* lds, int outer,
-                                                   int half) {
+  static __device__ __forceinline__ U32x4 Fragment(const char* lds, int first,
+                                                   int outer) {
     const int lane = threadIdx.x % kWave;
     const int i = lane % 16, g = lane / 16;
     if constexpr (kAlong == Along::kDepth) {
-      const int row = outer + i;
-      return *reinterpret_cast<const U32x4*>(
-          lds + row * 128 + (((half * 4 + g) ^ Key(i)) * 16));
+      const int at = first + (outer + i) * 64 + ((g ^ Key(i)) * 16);
+      return *reinterpret_cast<const U32x4*>(lds + at);
     } else if constexpr (sizeof(T) == 4) {
       U32x4 v;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int row = half * 16 + g * 4 + j;
-        const int c = (outer + i) / 4;
-        v[j] = *reinterpret_cast<const uint32_t*>(
-            lds + row * (kRowChunks * 16) + ((c ^ Key(g * 4)) * 16) +
-            (i % 4) * 4);
+        const int row = g * 4 + j;
+        const int c = ((outer + i) / 4) ^ Key(row);
+        const int at = first + row * (kRowChunks * 16) + c * 16 + (i % 4) * 4;
+        v[j] = *reinterpret_cast<const uint32_t*>(lds + at);
       }
       return v;
     } else {
@@ -205,13 +210,12 @@ struct Panel {
       uint2 part[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int in = g * 8 + j * 4 + i / 4;  // Key ignores multiples of 16
-        const int row = half * 32 + in;
-        const int c = outer / 8 + (i % 4) / 2;
+        const int row = g * 8 + j * 4 + i / 4;
+        const int c = (outer / 8 + (i % 4) / 2) ^ Key(row);
+        const int at = first + row * (kRowChunks * 16) + c * 16 + (i % 2) * 8;
         part[j] = __builtin_bit_cast(
-            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                       (S16x4Lds*)(lds + row * (kRowChunks * 16) +
-                                   ((c ^ Key(in)) * 16) + (i % 2) * 8)));
+            uint2,
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((S16x4Lds*)(lds + at)));
       }
       return U32x4{part[0].x, part[0].y, part[1].x, part[1].y};
     }
@@ -378,7 +382,7 @@ __device__ __forceinline__ void StoreUpTo(T* row, int32_t column,
 template <typename T>
 __device__ __forceinline__ void StoreColumns(T* row, bool exists,
                                              int32_t column, int32_t columns,
-                                             const F32x4 acc[4]) {
+                                             const F32x4* acc) {
   const int g = threadIdx.x % kWave / 16;
   if constexpr (sizeof(T) == 4) {
     if (!exists) return;
