@@ -742,6 +742,30 @@ int scemb_expert_matmul_weights_grad(
     void* weights_grad, void* workspace, size_t workspace_bytes,
     void* stream);
 
+/* The norm of all values of many tensors, norm = sqrt(sum of x^2), and
+ * factor = min(1, max_norm / norm) (may be NULL; a norm that is no number makes
+ * it none), single float32 values on the device: what scales the gradients down
+ * to max_norm, as scemb_adamw_options_t.grad_scale_ptr or by
+ * scemb_scale_gradients. Squares are summed in 64 bits, in an order that the
+ * sizes decide. A tensor of no values may be NULL. */
+typedef struct scemb_gradient {
+  void* data;
+  int64_t numel;
+  int32_t type;
+  int32_t reserved;
+} scemb_gradient_t;
+size_t scemb_gradient_norm_workspace_size(const scemb_gradient_t* gradients,
+                                          int32_t num_gradients);
+int scemb_gradient_norm(const scemb_gradient_t* gradients,
+                        int32_t num_gradients, double max_norm, float* norm,
+                        float* factor, void* workspace, size_t workspace_bytes,
+                        void* stream);
+/* Multiplies every value by *factor (on the device), in float32, rounded once;
+ * with a factor of one nothing is read or written. */
+int scemb_scale_gradients(const scemb_gradient_t* gradients,
+                          int32_t num_gradients, const float* factor,
+                          void* stream);
+
 /* AdamW over many tensors. Tensor i's moments are the values from
  * first_i = sum over j < i of numel_j rounded up to SCEMB_ADAMW_BLOCK on.
  * With g = grad * grad_scale and t the step (from 1):

@@ -45,6 +45,9 @@ struct Library {
   decltype(&scemb_expert_matmul_weights_grad_workspace_size)
       expert_matmul_weights_grad_workspace;
   decltype(&scemb_expert_matmul_weights_grad) expert_matmul_weights_grad;
+  decltype(&scemb_gradient_norm_workspace_size) gradient_norm_workspace;
+  decltype(&scemb_gradient_norm) gradient_norm;
+  decltype(&scemb_scale_gradients) scale_gradients;
   decltype(&scemb_adamw_update) adamw_update;
   decltype(&scemb_adamw_moments) adamw_moments;
 };
@@ -789,26 +792,33 @@ scemb_adamw_state_t StateOf(PyObject* m, PyObject* v, PyObject* m_scale,
   return s;
 }
 
-// Two weights or copies that share memory would be written by two work-groups
-// at once.
-void CheckApart(const std::vector<scemb_adamw_tensor_t>& tensors) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  spans.reserve(2 * tensors.size());
-  const auto add = [&](const void* p, int64_t bytes) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    spans.emplace_back(at, at + static_cast<uintptr_t>(bytes));
-  };
-  for (const auto& t : tensors) {
-    if (t.numel == 0) continue;
-    add(t.param, t.numel * (t.param_type == SCEMB_F32 ? 4 : 2));
-    if (t.copy != nullptr) add(t.copy, t.numel * 2);
-  }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i) {
-    if (spans[i].first < spans[i - 1].second) {
-      Refuse("two params or copies share memory");
+// Bytes [first, second) of memory.
+using Spans = std::vector<std::pair<uintptr_t, uintptr_t>>;
+
+void AddSpan(Spans* spans, const void* p, int64_t bytes) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  spans->emplace_back(at, at + static_cast<uintptr_t>(bytes));
+}
+
+// Two tensors that share memory would be written by two work-groups at once.
+void CheckApart(Spans* spans, const char* what) {
+  std::sort(spans->begin(), spans->end());
+  for (size_t i = 1; i < spans->size(); ++i) {
+    if ((*spans)[i].first < (*spans)[i - 1].second) {
+      Refuse(std::string("two ") + what + " share memory");
     }
   }
+}
+
+void CheckApart(const std::vector<scemb_adamw_tensor_t>& tensors) {
+  Spans spans;
+  spans.reserve(2 * tensors.size());
+  for (const auto& t : tensors) {
+    if (t.numel == 0) continue;
+    AddSpan(&spans, t.param, t.numel * (t.param_type == SCEMB_F32 ? 4 : 2));
+    if (t.copy != nullptr) AddSpan(&spans, t.copy, t.numel * 2);
+  }
+  CheckApart(&spans, "params or copies");
 }
 
 // Autograd is told of a write: a backward pass that needs the old values raises.
@@ -955,6 +965,106 @@ PyObject* AdamwMoments(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------------------
+// The gradients' norm.
+// ---------------------------------------------------------------------------
+
+// Gradients as the library takes them; those that are None are left out. A
+// tensor without gaps is taken as it lies in memory, whatever its strides. With
+// `write` it has to be such a tensor, else a copy is.
+struct Gradients {
+  std::vector<scemb_gradient_t> list;
+  std::vector<Tensor> keep;
+
+  Gradients(const Sequence& grads, int dev, bool write) {
+    list.reserve(grads.n);
+    for (Py_ssize_t i = 0; i < grads.n; ++i) {
+      if (grads[i] == Py_None) continue;
+      const bool fits = Fits(grads[i], dev, kRowTypes);
+      if (!fits) {
+        const Tensor& t = AnyTensorOf(grads[i], At("grads", i), dev, kRowTypes);
+        const bool whole = t.is_non_overlapping_and_dense();
+        if (write && !(whole && HoldsValues(t))) {
+          Refuse(At("grads", i) + " must have no gaps in memory and hold its "
+                                  "values");
+        }
+        // A negated view has the same squares.
+        keep.push_back(t._is_zerotensor() ? t.clone()
+                       : whole            ? t
+                                          : t.contiguous());
+      }
+      const Tensor& t = fits ? THPVariable_Unpack(grads[i]) : keep.back();
+      list.push_back({t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(),
+                      Code(t.scalar_type()), 0});
+    }
+  }
+  int32_t size() const { return static_cast<int32_t>(list.size()); }
+};
+
+struct Norm {
+  Tensor norm;
+  Tensor factor;
+};
+
+// max_norm: None for no factor.
+Norm NormOf(const Gradients& g, PyObject* max_norm, PyObject* workspace,
+            int dev) {
+  double limit = 0.0;
+  if (max_norm != Py_None) {
+    limit = Float(max_norm);
+    if (!(limit >= 0)) Refuse("max_norm must not be negative, got " + Text(limit));
+  }
+  const auto options =
+      at::TensorOptions(at::kFloat).device(at::kCUDA, dev);
+  Norm out;
+  out.norm = at::empty({}, options);
+  if (max_norm != Py_None) out.factor = at::empty({}, options);
+  const size_t bytes = lib.gradient_norm_workspace(g.list.data(), g.size());
+  if (bytes == 0) Check(SCEMB_ERR_INVALID_ARGUMENT);
+  const Tensor ws = Workspace(workspace, bytes);
+  Check(lib.gradient_norm(g.list.data(), g.size(), limit, FloatData(out.norm),
+                          FloatData(out.factor), Data(ws), bytes,
+                          Stream(dev)));
+  return out;
+}
+
+// gradient_norm(grads, max_norm, workspace) -> (norm, factor)
+PyObject* GradientNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 3) Refuse("gradient_norm takes 3 arguments");
+    const int dev = CurrentDevice();
+    const Sequence grads(a[0], "grads must be a sequence of tensors");
+    const Norm out = NormOf(Gradients(grads, dev, false), a[1], a[2], dev);
+    return Tuple({out.norm, out.factor});
+  });
+}
+
+// clip_gradients(grads, max_norm, workspace) -> norm
+PyObject* ClipGradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 3) Refuse("clip_gradients takes 3 arguments");
+    const int dev = CurrentDevice();
+    const Sequence grads(a[0], "grads must be a sequence of tensors");
+    const Gradients g(grads, dev, true);
+    Spans spans;
+    spans.reserve(g.list.size());
+    for (const auto& t : g.list) {
+      if (t.numel > 0) {
+        AddSpan(&spans, t.data, t.numel * (t.type == SCEMB_F32 ? 4 : 2));
+      }
+    }
+    CheckApart(&spans, "grads");
+    if (a[1] == Py_None) Refuse("max_norm must be a number");
+    const Norm out = NormOf(g, a[1], a[2], dev);
+    Check(lib.scale_gradients(g.list.data(), g.size(), FloatData(out.factor),
+                              Stream(dev)));
+    for (Py_ssize_t i = 0; i < grads.n; ++i) {
+      if (grads[i] != Py_None) Written(THPVariable_Unpack(grads[i]));
+    }
+    return Wrap(out.norm);
+  });
+}
+
+// ---------------------------------------------------------------------------
 // The module.
 // ---------------------------------------------------------------------------
 
@@ -1010,6 +1120,8 @@ PyMethodDef kMethods[] = {
     SCEMB_METHOD("tokens_from_experts_grad", TokensFromExpertsGrad),
     SCEMB_METHOD("expert_matmul", ExpertMatmul),
     SCEMB_METHOD("expert_matmul_grad", ExpertMatmulGrad),
+    SCEMB_METHOD("gradient_norm", GradientNorm),
+    SCEMB_METHOD("clip_gradients", ClipGradients),
     SCEMB_METHOD("adamw_sizes", AdamwSizes),
     SCEMB_METHOD("adamw_scalar", AdamwScalar),
     SCEMB_METHOD("adamw_update", AdamwUpdate),

@@ -91,6 +91,9 @@ EXPORTED_SYMBOLS = (
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",
+    "scemb_gradient_norm_workspace_size",
+    "scemb_gradient_norm",
+    "scemb_scale_gradients",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )
@@ -431,6 +434,9 @@ _DENSE_FUNCTIONS = (
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",
+    "scemb_gradient_norm_workspace_size",
+    "scemb_gradient_norm",
+    "scemb_scale_gradients",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )

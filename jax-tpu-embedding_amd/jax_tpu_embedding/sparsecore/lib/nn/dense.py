@@ -453,3 +453,40 @@ def adamw_moments(state: AdamWState):
     return state.m, state.v
   return _calls().adamw_moments(state.m, state.v, state.m_scale,
                                 state.v_scale)
+
+
+# ---------------------------------------------------------------------------
+# The gradients' norm.
+# ---------------------------------------------------------------------------
+
+
+def gradient_norm(grads, *, max_norm: float | None = None):
+  """The norm of all values of all gradients, sqrt(sum of g^2), a single
+  float32 on the GPU; with max_norm (norm, factor), the factor being
+  min(1, max_norm / norm), which adamw_update takes as grad_scale: gradients
+  clipped to a global norm without a pass that writes them.
+
+  grads: a sequence of float32, bfloat16 or float16 tensors of any shapes and
+    strides, or None (left out). What is given twice counts twice.
+  max_norm: not negative.
+
+  Squares are summed in 64 bits, in an order that the sizes decide. With an
+  infinity among the values the norm is infinite and the factor 0, with a NaN
+  both are NaN.
+  """
+  norm, factor = _calls().gradient_norm(grads, max_norm, _workspace)
+  return norm if max_norm is None else (norm, factor)
+
+
+def clip_gradients(grads, max_norm: float):
+  """Scales all gradients, in place, by min(1, max_norm / their norm); returns
+  the norm that they had, a single float32 on the GPU.
+
+  grads: as for gradient_norm, but tensors have to be without gaps in memory
+    (any order of dimensions) and share none.
+
+  Products are float32, rounded once. Gradients whose norm is within max_norm
+  are not written. With an infinity among the values the factor is 0 (and the
+  infinities become NaN), with a NaN all values become NaN.
+  """
+  return _calls().clip_gradients(grads, max_norm, _workspace)
