@@ -28,9 +28,8 @@ struct Tile {
   static constexpr int kWaves = kWavesM * kWavesN;
   static constexpr int kThreads = kWaves * kWave;
   static constexpr bool kDirect = kDirect_;
-  static constexpr int kFragM = kM / kWavesM / 16;
-  static constexpr int kFragN = kN / kWavesN / 16;
-  static_assert(kFragN % 4 == 0, "results are stored by 64 columns");
+  static constexpr int kFragM = kM / kWavesM / 32;
+  static constexpr int kFragN = kN / kWavesN / 32;
   using A = Panel<T, kA, kM, kThreads>;
   using B = Panel<T, kB, kN, kThreads>;
   static constexpr int kDepth = A::kDepth;
@@ -38,36 +37,44 @@ struct Tile {
   static constexpr int kLoads = A::kPer + B::kPer;  // of a thread and step
   static constexpr Along kAlongA = kA, kAlongB = kB;
 
-  F32x4 acc[kFragM][kFragN];
+  F32x16 acc[kFragM][kFragN];
 
   static __device__ __forceinline__ int WaveM() {
     return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / kWavesN *
-           (kFragM * 16);
+           (kFragM * 32);
   }
   static __device__ __forceinline__ int WaveN() {
     return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWavesN *
-           (kFragN * 16);
+           (kFragN * 32);
   }
 
   struct Fragments {
-    U32x4 a[kFragM];
-    U32x4 b[kFragN];
+    U32x4 a[2][kFragM];
+    U32x4 b[2][kFragN];
   };
   static __device__ __forceinline__ void Read(const char* lds, Fragments* f) {
 #pragma unroll
-    for (int j = 0; j < kFragN; ++j) {
-      f->b[j] = B::Fragment(lds, A::kBytes, WaveN() + j * 16);
-    }
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int i = 0; i < kFragM; ++i) {
-      f->a[i] = A::Fragment(lds, 0, WaveM() + i * 16);
+      for (int j = 0; j < kFragN; ++j) {
+        f->b[half][j] = B::Fragment(lds, A::kBytes, WaveN() + j * 32, half);
+      }
+#pragma unroll
+      for (int i = 0; i < kFragM; ++i) {
+        f->a[half][i] = A::Fragment(lds, 0, WaveM() + i * 32, half);
+      }
     }
   }
   __device__ __forceinline__ void Multiply(const Fragments& f) {
 #pragma unroll
-    for (int i = 0; i < kFragM; ++i) {
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int j = 0; j < kFragN; ++j) MultiplyAdd<T>(f.b[j], f.a[i], &acc[i][j]);
+      for (int i = 0; i < kFragM; ++i) {
+#pragma unroll
+        for (int j = 0; j < kFragN; ++j) {
+          MultiplyAdd<T>(f.b[half][j], f.a[half][i], &acc[i][j]);
+        }
+      }
     }
   }
 
@@ -82,7 +89,7 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
-      for (int j = 0; j < kFragN; ++j) acc[i][j] = F32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < kFragN; ++j) acc[i][j] = F32x16{};
     }
     if (depth <= 0) return;
     const int64_t a_step =
@@ -198,11 +205,11 @@ struct Tile {
                                         int n) const {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
-      const int row = WaveM() + i * 16 + threadIdx.x % 16;
+      const int row = WaveM() + i * 32 + threadIdx.x % 32;
 #pragma unroll
-      for (int j = 0; j < kFragN; j += 4) {
-        StoreColumns(c + row * stride, row < m, WaveN() + j * 16, n,
-                     &acc[i][j]);
+      for (int j = 0; j < kFragN; ++j) {
+        StoreColumns(c + row * stride, row < m, WaveN() + j * 32, n,
+                     acc[i][j]);
       }
     }
   }
@@ -311,6 +318,8 @@ __global__ __launch_bounds__(kJoinBlock) void JoinParts(const float* parts,
 // ---------------------------------------------------------------------------
 
 template <typename T, Along kA, Along kB, bool kDirect>
+using Small = Tile<T, kA, kB, 32, 128, 1, 4, kDirect>;
+template <typename T, Along kA, Along kB, bool kDirect>
 using Middle = Tile<T, kA, kB, 128, 128, 2, 2, kDirect>;
 template <typename T, Along kA, Along kB>
 using Large = Tile<T, kA, kB, 256, 256, 2, 4, true>;
@@ -365,7 +374,12 @@ struct RowsCall {
                         w.expert * kBytes % 16 == 0 &&
                         depth * kBytes % 16 == 0 &&
                         (kB == Along::kDepth || columns * kBytes % 16 == 0);
-    if (!direct) return Launch<Middle<T, Along::kDepth, kB, false>>();
+    const bool small = rows <= 32ll * experts;
+    if (!direct) {
+      return small ? Launch<Small<T, Along::kDepth, kB, false>>()
+                   : Launch<Middle<T, Along::kDepth, kB, false>>();
+    }
+    if (small) return Launch<Small<T, Along::kDepth, kB, true>>();
     if constexpr (kBytes == 2) {
       if (rows >= 256ll * experts) {
         return Launch<Large<T, Along::kDepth, kB>>();

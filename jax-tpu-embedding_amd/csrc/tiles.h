@@ -7,7 +7,7 @@
 
 namespace scemb {
 
-using F32x4 = float __attribute__((ext_vector_type(4)));
+using F32x16 = float __attribute__((ext_vector_type(16)));
 using U32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
 using LdsBytes = __attribute__((address_space(3))) void*;
@@ -63,8 +63,8 @@ __device__ __forceinline__ void Barrier() {
 // ("depth"), in LDS.
 //
 // kDepth: neighbours in memory are neighbours along the depth. A row is 64
-// bytes, its four 16-byte chunks permuted so that 8 lanes that read one chunk
-// of 8 rows find them in different banks.
+// bytes, its four 16-byte chunks permuted so that 16 lanes that read one chunk
+// of 16 rows find them in different banks (of 64).
 // kOuter: neighbours in memory are neighbours along the outer index. LDS holds
 // a row for each depth index, its chunks permuted by the depth index; reading
 // transposes (16 bits) or gathers (32 bits).
@@ -77,34 +77,42 @@ struct Panel {
   static constexpr int kBytes = kOuter * 64;
   static constexpr int kDepth = 64 / sizeof(T);
   static constexpr int kEach = 16 / sizeof(T);  // elements of a chunk
-  static constexpr int kPer = kBytes / 16 / kThreads;  // chunks of a thread
+  // Threads that load a panel; where it has fewer chunks than threads, several
+  // wavefronts load the same ones to the same places, and every wavefront has
+  // the same number of loads to wait for.
+  static constexpr int kLoaders =
+      kBytes / 16 < kThreads ? kBytes / 16 : kThreads;
+  static constexpr int kPer = kBytes / 16 / kLoaders;  // chunks of a thread
   static constexpr int kRowChunks =
       kAlong == Along::kDepth ? 4 : kOuter * sizeof(T) / 16;
-  static_assert(kPer >= 1 && kPer * 16 * kThreads == kBytes, "whole chunks");
-  static_assert(kThreads % kRowChunks == 0, "a thread's chunks share a column");
+  static_assert(kPer * 16 * kLoaders == kBytes && kLoaders % kWave == 0 &&
+                    kThreads % kLoaders == 0,
+                "whole chunks");
+  static_assert(kLoaders % kRowChunks == 0, "a thread's chunks share a column");
 
   // What chunk numbers of LDS row `row` are XORed with.
   static __device__ __forceinline__ int Key(int row) {
-    if constexpr (kAlong == Along::kDepth) return (row >> 1) & 3;
+    if constexpr (kAlong == Along::kDepth) return (row >> 2) & 3;
     if constexpr (sizeof(T) == 4) {
-      // Lanes of four rows 4 apart read 64 bytes each.
-      return ((row >> 2) & 3) << 2;
+      // Lanes of two rows 4 apart read 128 bytes each.
+      return ((row >> 2) & 1) * 8 & (kRowChunks - 1);
     }
-    // Lanes of rows 0-3, and of those 8 later, read 32 bytes each.
-    return (((row & 3) | ((row >> 3) & 1) << 2) << 1) & (kRowChunks - 1);
+    // Lanes of rows 0-3, and of those 8 later, read 64 bytes each.
+    return (((row & 3) | ((row >> 3) & 1) << 2) << 2) & (kRowChunks - 1);
   }
 
   // The thread's chunk i: its row in LDS, and which chunk of that row in
   // memory.
   static __device__ __forceinline__ int Row(int i) {
-    return i * (kThreads / kRowChunks) + threadIdx.x / kRowChunks;
+    return i * (kLoaders / kRowChunks) + threadIdx.x % kLoaders / kRowChunks;
   }
   static __device__ __forceinline__ int Column(int i) {
     return (threadIdx.x % kRowChunks) ^ Key(Row(i));
   }
   static __device__ __forceinline__ char* Place(char* lds, int i) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    return lds + (i * kThreads + wave * kWave) * 16;
+    const int wave =
+        __builtin_amdgcn_readfirstlane(threadIdx.x % kLoaders / kWave);
+    return lds + (i * kLoaders + wave * kWave) * 16;
   }
 
   // --- Straight to LDS: chunks are aligned, and none ends past the last
@@ -174,29 +182,30 @@ struct Panel {
   static __device__ __forceinline__ void Put(const Chunks& from, char* lds) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      *reinterpret_cast<U32x4*>(lds + (i * kThreads + threadIdx.x) * 16) =
+      *reinterpret_cast<U32x4*>(
+          lds + (i * kLoaders + threadIdx.x % kLoaders) * 16) =
           __builtin_bit_cast(U32x4, from.v[i]);
     }
   }
 
-  // --- Fragments: 16 outer indices from `outer` on. A lane gets outer index
-  // lane % 16 and 16 bytes of depth, from element (lane / 16) * kEach on. The
-  // panel begins `first` bytes into `lds`. (An address is the array and one sum:
-  // the compiler follows no long chain to the array, and would wait for loads
-  // into other ones.) ---
+  // --- Fragments: 32 outer indices from `outer` on by half a step. A lane gets
+  // outer index lane % 32 and 16 bytes of depth, from element
+  // (2 * half + lane / 32) * kEach on. The panel begins `first` bytes into
+  // `lds`. (An address is the array and one sum: the compiler follows no long
+  // chain to the array, and would wait for loads into other ones.) ---
 
   static __device__ __forceinline__ U32x4 Fragment(const char* lds, int first,
-                                                   int outer) {
+                                                   int outer, int half) {
     const int lane = threadIdx.x % kWave;
-    const int i = lane % 16, g = lane / 16;
+    const int i = lane % 32, chunk = half * 2 + lane / 32;
     if constexpr (kAlong == Along::kDepth) {
-      const int at = first + (outer + i) * 64 + ((g ^ Key(i)) * 16);
+      const int at = first + (outer + i) * 64 + ((chunk ^ Key(i)) * 16);
       return *reinterpret_cast<const U32x4*>(lds + at);
     } else if constexpr (sizeof(T) == 4) {
       U32x4 v;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int row = g * 4 + j;
+        const int row = chunk * 4 + j;
         const int c = ((outer + i) / 4) ^ Key(row);
         const int at = first + row * (kRowChunks * 16) + c * 16 + (i % 4) * 4;
         v[j] = *reinterpret_cast<const uint32_t*>(lds + at);
@@ -204,15 +213,16 @@ struct Panel {
       return v;
     } else {
       // Four lanes address four neighbours each of one depth index, 16 lanes
-      // four depth indices; lane i gets the four of outer index i.
+      // four depth indices; lane j of the 16 gets the four of outer index j.
       using S16x4 = short __attribute__((ext_vector_type(4)));
       using S16x4Lds = __attribute__((address_space(3))) S16x4;
+      const int in = lane % 16, from = outer + lane / 16 % 2 * 16;
       uint2 part[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int row = g * 8 + j * 4 + i / 4;
-        const int c = (outer / 8 + (i % 4) / 2) ^ Key(row);
-        const int at = first + row * (kRowChunks * 16) + c * 16 + (i % 2) * 8;
+        const int row = chunk * 8 + j * 4 + in / 4;
+        const int c = (from / 8 + in % 4 / 2) ^ Key(row);
+        const int at = first + row * (kRowChunks * 16) + c * 16 + in % 2 * 8;
         part[j] = __builtin_bit_cast(
             uint2,
             __builtin_amdgcn_ds_read_tr16_b64_v4i16((S16x4Lds*)(lds + at)));
@@ -222,26 +232,26 @@ struct Panel {
   }
 };
 
-// acc[n][m] += sum over 64 bytes of depth of b[n] * a[m], for 16 of each. A
-// lane holds n = 4 * (lane / 16) + (0 to 3) of m = lane % 16.
+// acc[n][m] += the sum over half a step of b[n] * a[m], for 32 of each. A lane
+// holds m = lane % 32 and n = 8 * (i / 4) + 4 * (lane / 32) + i % 4 in element i.
 template <typename T>
 __device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
-                                            F32x4* acc) {
+                                            F32x16* acc) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t bj = b[j], aj = a[j];
-      *acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+      *acc = __builtin_amdgcn_mfma_f32_32x32x2f32(
           __builtin_bit_cast(float, bj), __builtin_bit_cast(float, aj), *acc,
           0, 0, 0);
     }
   } else if constexpr (__is_same(T, bf16)) {
     using V = bf16 __attribute__((ext_vector_type(8)));
-    *acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+    *acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
         __builtin_bit_cast(V, b), __builtin_bit_cast(V, a), *acc, 0, 0, 0);
   } else {
     using V = f16 __attribute__((ext_vector_type(8)));
-    *acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+    *acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
         __builtin_bit_cast(V, b), __builtin_bit_cast(V, a), *acc, 0, 0, 0);
   }
 }
@@ -343,24 +353,6 @@ struct TileGrid {
 // Results.
 // ---------------------------------------------------------------------------
 
-// x[j] of lane group g (16 lanes each) and x[g] of lane group j change places.
-__device__ __forceinline__ void TransposeGroups(uint32_t x[4]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const auto r = __builtin_amdgcn_permlane32_swap(x[j], x[j + 2], false,
-                                                    false);
-    x[j] = r[0];
-    x[j + 2] = r[1];
-  }
-#pragma unroll
-  for (int j = 0; j < 4; j += 2) {
-    const auto r = __builtin_amdgcn_permlane16_swap(x[j], x[j + 1], false,
-                                                    false);
-    x[j] = r[0];
-    x[j + 1] = r[1];
-  }
-}
-
 // Elements [column, column + V) of a row, those below `columns`.
 template <typename T, int V>
 __device__ __forceinline__ void StoreUpTo(T* row, int32_t column,
@@ -376,40 +368,49 @@ __device__ __forceinline__ void StoreUpTo(T* row, int32_t column,
   }
 }
 
-// 64 columns of a row from the accumulators of four fragments, rounded once.
-// With 16 bits a lane gathers 16 neighbours from the other groups of lanes and
-// writes 32 bytes; with 32 bits it writes 16 bytes of each fragment.
+// 32 columns of a row from a fragment's accumulators, rounded once. With 16
+// bits the two lanes of a row exchange halves, so that each writes 16 bytes at
+// a time.
 template <typename T>
 __device__ __forceinline__ void StoreColumns(T* row, bool exists,
                                              int32_t column, int32_t columns,
-                                             const F32x4* acc) {
-  const int g = threadIdx.x % kWave / 16;
+                                             const F32x16& acc) {
+  const int h = threadIdx.x % kWave / 32;
   if constexpr (sizeof(T) == 4) {
     if (!exists) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      StoreUpTo(row, column + j * 16 + g * 4, columns,
-                __builtin_bit_cast(Vec<T, 4>, acc[j]));
+    for (int q = 0; q < 4; ++q) {
+      Vec<T, 4> v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.v[i] = acc[q * 4 + i];
+      StoreUpTo(row, column + q * 8 + h * 4, columns, v);
     }
   } else {
     uint32_t x[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int q = 0; q < 4; ++q) {
       Vec<T, 4> v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v.v[i] = static_cast<T>(acc[j][i]);
+      for (int i = 0; i < 4; ++i) v.v[i] = static_cast<T>(acc[q * 4 + i]);
       const uint2 u = __builtin_bit_cast(uint2, v);
-      x[0][j] = u.x;
-      x[1][j] = u.y;
+      x[0][q] = u.x;
+      x[1][q] = u.y;
     }
-    TransposeGroups(x[0]);
-    TransposeGroups(x[1]);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x[w][q], x[w][q + 1],
+                                                        false, false);
+        x[w][q] = r[0];
+        x[w][q + 1] = r[1];
+      }
+    }
     if (!exists) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const U32x4 v = {x[0][2 * j], x[1][2 * j], x[0][2 * j + 1],
-                       x[1][2 * j + 1]};
-      StoreUpTo(row, column + g * 16 + j * 8, columns,
+    for (int q = 0; q < 4; q += 2) {
+      const U32x4 v = {x[0][q], x[1][q], x[0][q + 1], x[1][q + 1]};
+      StoreUpTo(row, column + q * 8 + h * 8, columns,
                 __builtin_bit_cast(Vec<T, 8>, v));
     }
   }
