@@ -8,17 +8,9 @@ namespace scemb {
 namespace {
 
 // ---------------------------------------------------------------------------
-// A tile of the result by one work-group of kWavesM x kWavesN wavefronts. LDS
-// is a ring of kSlots steps of 64 bytes of depth: while one is multiplied the
-// next two are there or on their way, and the one after those is asked for.
+// A tile of the result by one work-group of kWavesM x kWavesN wavefronts. Of
+// two steps of the depth in LDS one is multiplied while the other is loaded.
 // ---------------------------------------------------------------------------
-
-constexpr int kSlots = 4;
-#define SCEMB_SLOTS(bytes)                                  \
-  __shared__ __attribute__((aligned(16))) char slot0[bytes]; \
-  __shared__ __attribute__((aligned(16))) char slot1[bytes]; \
-  __shared__ __attribute__((aligned(16))) char slot2[bytes]; \
-  __shared__ __attribute__((aligned(16))) char slot3[bytes]
 
 template <typename T_, Along kA, Along kB, int kM_, int kN_, int kWavesM,
           int kWavesN, bool kDirect_>
@@ -34,7 +26,6 @@ struct Tile {
   using B = Panel<T, kB, kN, kThreads>;
   static constexpr int kDepth = A::kDepth;
   static constexpr int kLds = A::kBytes + B::kBytes;
-  static constexpr int kLoads = A::kPer + B::kPer;  // of a thread and step
   static constexpr Along kAlongA = kA, kAlongB = kB;
 
   F32x16 acc[kFragM][kFragN];
@@ -48,44 +39,46 @@ struct Tile {
            (kFragN * 32);
   }
 
+  // What half a step is multiplied from.
   struct Fragments {
     U32x4 a[2][kFragM];
     U32x4 b[2][kFragN];
   };
-  static __device__ __forceinline__ void Read(const char* lds, Fragments* f) {
+  static __device__ __forceinline__ void Read(const char* lds, int half,
+                                              Fragments* f) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int j = 0; j < kFragN; ++j) {
-        f->b[half][j] = B::Fragment(lds, A::kBytes, WaveN() + j * 32, half);
+        f->b[q][j] =
+            B::Fragment(lds, A::kBytes, WaveN() + j * 32, half * 2 + q);
       }
 #pragma unroll
       for (int i = 0; i < kFragM; ++i) {
-        f->a[half][i] = A::Fragment(lds, 0, WaveM() + i * 32, half);
+        f->a[q][i] = A::Fragment(lds, 0, WaveM() + i * 32, half * 2 + q);
       }
     }
   }
   __device__ __forceinline__ void Multiply(const Fragments& f) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
         for (int j = 0; j < kFragN; ++j) {
-          MultiplyAdd<T>(f.b[half][j], f.a[half][i], &acc[i][j]);
+          MultiplyAdd<T>(f.b[q][j], f.a[q][i], &acc[i][j]);
         }
       }
     }
   }
 
   // The tile's sums over `depth`. a and b are the panels' first elements; m and
-  // n (at least 1) the outer indices that exist. The slots are different
+  // n (at least 1) the outer indices that exist. lds0 and lds1 are different
   // arrays: the compiler has to see that a load into one needs no wait before
-  // another is read.
+  // the other is read.
   __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
                                       const T* b, int64_t b_stride, int n,
-                                      int32_t depth, char* slot0, char* slot1,
-                                      char* slot2, char* slot3) {
+                                      int32_t depth, char* lds0, char* lds1) {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
@@ -103,9 +96,9 @@ struct Tile {
       pb.Start(b_stride, n);
       const char* at_a = reinterpret_cast<const char*>(a);
       const char* at_b = reinterpret_cast<const char*>(b);
-      const auto load = [&](char* slot) __attribute__((always_inline)) {
-        pa.Load(at_a, slot);
-        pb.Load(at_b, slot + A::kBytes);
+      const auto load = [&](char* lds) __attribute__((always_inline)) {
+        pa.Load(at_a, lds);
+        pb.Load(at_b, lds + A::kBytes);
         at_a += a_step * sizeof(T);
         at_b += b_step * sizeof(T);
       };
@@ -116,24 +109,16 @@ struct Tile {
         typename B::Chunks cb;
         A::template Fetch<true>(a, a_stride, m, left, &ca);
         B::template Fetch<true>(b, b_stride, n, left, &cb);
-        A::Put(ca, slot0);
-        B::Put(cb, slot0 + A::kBytes);
+        A::Put(ca, lds0);
+        B::Put(cb, lds0 + A::kBytes);
         at_a += a_step / kDepth * left * sizeof(T);
         at_b += b_step / kDepth * left * sizeof(T);
       } else {
         left = kDepth;
-        load(slot0);
+        load(lds0);
       }
-      // Steps that are not multiplied, and of those what is not asked for.
-      int32_t steps = 1 + (depth - left) / kDepth;
-      int32_t ahead = steps - 3;
-      if (steps > 1) load(slot1);
-      if (steps > 2) load(slot2);
-      if (ahead >= 0) {
-        WaitLoads<2 * kLoads>();
-      } else {
-        WaitLoads<0>();
-      }
+      int32_t ahead = (depth - left) / kDepth;  // steps behind the current one
+      WaitLoads<0>();
       Barrier();
       // With two wavefronts a SIMD one reads while the other multiplies: the
       // second half of them are a barrier behind.
@@ -141,19 +126,13 @@ struct Tile {
       const bool second =
           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) >= kWaves / 2;
       if (kTurns && second) Barrier();
-      const auto turn = [&](const char* now, char* free) __attribute__((
+      const auto half = [&](const char* now, int h) __attribute__((
                             always_inline)) {
-        if (ahead > 0) load(free);
         Fragments f;
-        Read(now, &f);
-        // The next step is there.
-        if (ahead > 0) {
-          WaitLoads<2 * kLoads>();
-        } else {
-          WaitLoads<0>();
-        }
-        --ahead;
+        Read(now, h, &f);
         if constexpr (kTurns) {
+          // Whoever reads the next step first has its loads waited for by all.
+          if (h == 1) WaitLoads<0>();
           Barrier();
           __builtin_amdgcn_s_setprio(1);
           Multiply(f);
@@ -163,18 +142,24 @@ struct Tile {
           __builtin_amdgcn_sched_barrier(0);
           Multiply(f);
           __builtin_amdgcn_sched_barrier(0);
-          Barrier();
+          if (h == 1) {
+            WaitLoads<0>();
+            Barrier();
+          }
         }
       };
-      for (; steps >= 4; steps -= 4) {
-        turn(slot0, slot3);
-        turn(slot1, slot0);
-        turn(slot2, slot1);
-        turn(slot3, slot2);
+      const auto turn = [&](const char* now, char* next) __attribute__((
+                            always_inline)) {
+        if (ahead > 0) load(next);
+        half(now, 0);
+        half(now, 1);
+        --ahead;
+      };
+      while (ahead >= 1) {
+        turn(lds0, lds1);
+        turn(lds1, lds0);
       }
-      if (steps >= 1) turn(slot0, slot3);
-      if (steps >= 2) turn(slot1, slot0);
-      if (steps >= 3) turn(slot2, slot1);
+      if (ahead == 0) turn(lds0, lds1);
       if (kTurns && !second) Barrier();
     } else {
       typename A::Chunks ca;
@@ -182,9 +167,9 @@ struct Tile {
       A::template Fetch<false>(a, a_stride, m, depth, &ca);
       B::template Fetch<false>(b, b_stride, n, depth, &cb);
       for (int32_t at = 0; at < depth; at += kDepth) {
-        char* slot = (at / kDepth & 1) ? slot1 : slot0;
-        A::Put(ca, slot);
-        B::Put(cb, slot + A::kBytes);
+        char* lds = (at / kDepth & 1) ? lds1 : lds0;
+        A::Put(ca, lds);
+        B::Put(cb, lds + A::kBytes);
         __syncthreads();
         a += a_step;
         b += b_step;
@@ -192,9 +177,12 @@ struct Tile {
           A::template Fetch<false>(a, a_stride, m, depth - at - kDepth, &ca);
           B::template Fetch<false>(b, b_stride, n, depth - at - kDepth, &cb);
         }
-        Fragments f;
-        Read(slot, &f);
-        Multiply(f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          Fragments f;
+          Read(lds, h, &f);
+          Multiply(f);
+        }
       }
     }
   }
@@ -228,7 +216,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
     Weights w, int32_t columns, const int32_t* offsets, int32_t experts,
     typename C::T* y, TileGrid grid) {
   using T = typename C::T;
-  SCEMB_SLOTS(C::kLds);
+  __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
+  __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
   int32_t tile, column;
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
   const RowTile t = FindRowTile<C::kM>(offsets, experts, rows, tile);
@@ -240,7 +229,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
   const T* b = static_cast<const T*>(w.data) + t.segment * w.expert +
                (C::kAlongB == Along::kDepth ? column * w.stride : column);
   c.Run(x + t.row * x_stride, x_stride, m, b, w.stride, n,
-        t.segment < experts ? depth : 0, slot0, slot1, slot2, slot3);
+        t.segment < experts ? depth : 0, lds0, lds1);
   c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n);
 }
 
@@ -252,7 +241,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
     const typename C::T* dy, int64_t dy_stride, int32_t outer, int32_t rows,
     const int32_t* offsets, int32_t experts, Out* dw, int32_t splits,
     TileGrid grid) {
-  SCEMB_SLOTS(C::kLds);
+  __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
+  __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
   int32_t tile, column;
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
   const int32_t tiles = (inner + C::kM - 1) / C::kM;
@@ -271,7 +261,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   C c;
   c.Run(x + s.begin * x_stride + row, x_stride, m,
         dy + s.begin * dy_stride + column, dy_stride, n, s.end - s.begin,
-        slot0, slot1, slot2, slot3);
+        lds0, lds1);
   c.Store(dw + (static_cast<int64_t>(part) * inner + row) * outer + column,
           outer, m, n);
 }
@@ -404,11 +394,11 @@ WeightsPlan PlanWeights(int bytes, int64_t rows, int64_t inner, int64_t outer,
   };
   p.large = bytes == 2 && tiles(256) >= kCus;
   const int64_t have = tiles(p.large ? 256 : 128);
-  const int64_t steps = rows / experts / (64 / bytes);
+  const int64_t steps = rows / experts / (128 / bytes);
   const int64_t most = static_cast<int64_t>(
       (64 << 20) / (4.0 * experts * inner * outer));
   const int64_t splits =
-      std::min({CeilDiv(2 * kCus, have), steps / 8, most, int64_t{1024}});
+      std::min({CeilDiv(2 * kCus, have), steps / 4, most, int64_t{1024}});
   p.splits = static_cast<int32_t>(std::max<int64_t>(splits, 1));
   return p;
 }

@@ -59,12 +59,13 @@ __device__ __forceinline__ void Barrier() {
 }
 
 // ---------------------------------------------------------------------------
-// Panels: `kOuter` rows or columns of an operand by 64 bytes of the sum's index
+// Panels: `kOuter` rows or columns of an operand by 128 bytes of the sum's index
 // ("depth"), in LDS.
 //
-// kDepth: neighbours in memory are neighbours along the depth. A row is 64
-// bytes, its four 16-byte chunks permuted so that 16 lanes that read one chunk
-// of 16 rows find them in different banks (of 64).
+// kDepth: neighbours in memory are neighbours along the depth. A row is 128
+// bytes, a line of the caches (of 64 bytes, every line came from L2 twice), its
+// eight 16-byte chunks permuted so that 16 lanes that read one chunk of 16 rows
+// find them in different banks (of 64).
 // kOuter: neighbours in memory are neighbours along the outer index. LDS holds
 // a row for each depth index, its chunks permuted by the depth index; reading
 // transposes (16 bits) or gathers (32 bits).
@@ -74,8 +75,8 @@ enum class Along { kDepth, kOuter };
 
 template <typename T, Along kAlong, int kOuter, int kThreads>
 struct Panel {
-  static constexpr int kBytes = kOuter * 64;
-  static constexpr int kDepth = 64 / sizeof(T);
+  static constexpr int kBytes = kOuter * 128;
+  static constexpr int kDepth = 128 / sizeof(T);
   static constexpr int kEach = 16 / sizeof(T);  // elements of a chunk
   // Threads that load a panel; where it has fewer chunks than threads, several
   // wavefronts load the same ones to the same places, and every wavefront has
@@ -84,7 +85,7 @@ struct Panel {
       kBytes / 16 < kThreads ? kBytes / 16 : kThreads;
   static constexpr int kPer = kBytes / 16 / kLoaders;  // chunks of a thread
   static constexpr int kRowChunks =
-      kAlong == Along::kDepth ? 4 : kOuter * sizeof(T) / 16;
+      kAlong == Along::kDepth ? 8 : kOuter * sizeof(T) / 16;
   static_assert(kPer * 16 * kLoaders == kBytes && kLoaders % kWave == 0 &&
                     kThreads % kLoaders == 0,
                 "whole chunks");
@@ -92,7 +93,7 @@ struct Panel {
 
   // What chunk numbers of LDS row `row` are XORed with.
   static __device__ __forceinline__ int Key(int row) {
-    if constexpr (kAlong == Along::kDepth) return (row >> 2) & 3;
+    if constexpr (kAlong == Along::kDepth) return (row >> 1) & 7;
     if constexpr (sizeof(T) == 4) {
       // Lanes of two rows 4 apart read 128 bytes each.
       return ((row >> 2) & 1) * 8 & (kRowChunks - 1);
@@ -188,18 +189,18 @@ struct Panel {
     }
   }
 
-  // --- Fragments: 32 outer indices from `outer` on by half a step. A lane gets
-  // outer index lane % 32 and 16 bytes of depth, from element
-  // (2 * half + lane / 32) * kEach on. The panel begins `first` bytes into
+  // --- Fragments: 32 outer indices from `outer` on by a quarter of the depth.
+  // A lane gets outer index lane % 32 and 16 bytes of depth, from element
+  // (2 * quarter + lane / 32) * kEach on. The panel begins `first` bytes into
   // `lds`. (An address is the array and one sum: the compiler follows no long
   // chain to the array, and would wait for loads into other ones.) ---
 
   static __device__ __forceinline__ U32x4 Fragment(const char* lds, int first,
-                                                   int outer, int half) {
+                                                   int outer, int quarter) {
     const int lane = threadIdx.x % kWave;
-    const int i = lane % 32, chunk = half * 2 + lane / 32;
+    const int i = lane % 32, chunk = quarter * 2 + lane / 32;
     if constexpr (kAlong == Along::kDepth) {
-      const int at = first + (outer + i) * 64 + ((chunk ^ Key(i)) * 16);
+      const int at = first + (outer + i) * 128 + ((chunk ^ Key(i)) * 16);
       return *reinterpret_cast<const U32x4*>(lds + at);
     } else if constexpr (sizeof(T) == 4) {
       U32x4 v;
@@ -232,7 +233,7 @@ struct Panel {
   }
 };
 
-// acc[n][m] += the sum over half a step of b[n] * a[m], for 32 of each. A lane
+// acc[n][m] += the sum over a quarter of b[n] * a[m], for 32 of each. A lane
 // holds m = lane % 32 and n = 8 * (i / 4) + 4 * (lane / 32) + i % 4 in element i.
 template <typename T>
 __device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
