@@ -742,6 +742,33 @@ int scemb_expert_matmul_weights_grad(
     void* weights_grad, void* workspace, size_t workspace_bytes,
     void* stream);
 
+/* Weights in 8 bits (e4m3: a sign, 4 bits of exponent, 3 of mantissa, 448 the
+ * largest), where SCEMB_BLOCK_8BIT x SCEMB_BLOCK_8BIT values (inner x outer)
+ * share a scale 2^e, e >= -126 being the least with no magnitude of the block
+ * above 448 * 2^e: a code is value / 2^e, rounded to nearest even. codes is
+ * [num_experts, outer, inner rounded up to SCEMB_BLOCK_8BIT] (zeros behind
+ * inner), exponents [num_experts, ceil(outer / SCEMB_BLOCK_8BIT), ceil(inner /
+ * SCEMB_BLOCK_8BIT)] holds e + 127. A block with a value that is not finite is
+ * NaN throughout. Strides as for scemb_expert_matmul. */
+#define SCEMB_BLOCK_8BIT 128
+#define SCEMB_MAX_INNER_8BIT (1 << 22)
+int scemb_quantize_weights(const void* weights, int32_t type,
+                           int64_t expert_stride, int64_t inner_stride,
+                           int64_t outer_stride, int64_t inner, int64_t outer,
+                           int32_t num_experts, uint8_t* codes,
+                           int32_t* exponents, void* stream);
+
+/* scemb_expert_matmul with such weights: rows are brought to 8 bits the same way,
+ * SCEMB_BLOCK_8BIT neighbours of a row sharing a scale, in the workspace; sums
+ * are float32, rounded once to rows' type. offsets NULL: one expert that has
+ * all rows. */
+size_t scemb_matmul_8bit_workspace_size(int64_t num_rows, int64_t inner);
+int scemb_matmul_8bit(const void* rows, int32_t type, int64_t rows_stride,
+                      int64_t num_rows, int64_t inner, int64_t outer,
+                      const uint8_t* codes, const int32_t* exponents,
+                      const int32_t* offsets, int32_t num_experts, void* y,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* The norm of all values of many tensors, norm = sqrt(sum of x^2), and
  * factor = min(1, max_norm / norm) (may be NULL; a norm that is no number makes
  * it none), single float32 values on the device: what scales the gradients down

@@ -45,6 +45,9 @@ struct Library {
   decltype(&scemb_expert_matmul_weights_grad_workspace_size)
       expert_matmul_weights_grad_workspace;
   decltype(&scemb_expert_matmul_weights_grad) expert_matmul_weights_grad;
+  decltype(&scemb_quantize_weights) quantize_weights;
+  decltype(&scemb_matmul_8bit_workspace_size) matmul_8bit_workspace;
+  decltype(&scemb_matmul_8bit) matmul_8bit;
   decltype(&scemb_gradient_norm_workspace_size) gradient_norm_workspace;
   decltype(&scemb_gradient_norm) gradient_norm;
   decltype(&scemb_scale_gradients) scale_gradients;
@@ -564,14 +567,33 @@ Tensor OffsetsArg(PyObject* o, int dev) {
   return t.contiguous();
 }
 
-// The experts' weights, [experts, inner, outer], contiguous along inner or
-// outer (a copy if they are neither).
+// The strides of weights [experts, inner, outer] that are contiguous along inner
+// or outer; others are copied first.
+struct WeightStrides {
+  int64_t expert;
+  int64_t inner;
+  int64_t outer;
+
+  explicit WeightStrides(Tensor* t) {
+    const int64_t i = t->size(1), o = t->size(2);
+    if ((i > 1 && o > 1 && t->stride(1) != 1 && t->stride(2) != 1) ||
+        (i == 1 && t->stride(2) != 1) || (o == 1 && t->stride(1) != 1)) {
+      *t = t->contiguous();
+    }
+    expert = t->stride(0);
+    // The stride of a dimension of one value says nothing.
+    outer = o == 1 ? (i == 1 ? 1 : i) : t->stride(2);
+    inner = i == 1 ? (o == 1 ? 1 : o) : t->stride(1);
+  }
+};
+
+// The experts' weights, [experts, inner, outer].
 struct ExpertWeights {
   Tensor t;
   int64_t experts;
   int64_t inner;
   int64_t outer;
-  int64_t stride[3];
+  std::optional<WeightStrides> stride;
 
   ExpertWeights(PyObject* o, const Tensor& offsets, const Tensor& rows,
                 int dev)
@@ -584,25 +606,10 @@ struct ExpertWeights {
     }
     inner = t.size(1);
     outer = t.size(2);
-    if (outer > 1 && inner > 1 && t.stride(1) != 1 && t.stride(2) != 1) {
-      t = t.contiguous();
-    }
-    // The stride of a dimension of one value says nothing.
-    stride[0] = t.stride(0);
-    stride[1] = inner == 1 ? 1 : t.stride(1);
-    stride[2] = outer == 1 ? 1 : t.stride(2);
-    if (inner == 1 && outer > 1) stride[1] = outer * stride[2];
-    if (outer == 1 && inner > 1) stride[2] = inner * stride[1];
-    if (stride[1] != 1 && stride[2] != 1) {
-      // A single row or column of values that are not neighbours.
-      t = t.contiguous();
-      stride[0] = inner * outer;
-      stride[1] = outer;
-      stride[2] = 1;
-    }
+    stride.emplace(&t);
   }
   // Stored by output: the gradient is laid out the same.
-  bool ByOuter() const { return stride[2] != 1; }
+  bool ByOuter() const { return stride->outer != 1; }
 };
 
 Tensor MatrixArg(PyObject* o, const char* name, const Tensor& like,
@@ -643,7 +650,7 @@ PyObject* ExpertMatmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor y = New({r.n, w.outer}, x.scalar_type(), x);
     Check(lib.expert_matmul(
         r.t.data_ptr(), Code(x.scalar_type()), r.stride, r.n, w.inner, w.outer,
-        w.t.data_ptr(), w.stride[0], w.stride[1], w.stride[2],
+        w.t.data_ptr(), w.stride->expert, w.stride->inner, w.stride->outer,
         static_cast<const int32_t*>(offsets.data_ptr()),
         static_cast<int32_t>(w.experts), y.data_ptr(), Stream(dev)));
     return Wrap(y);
@@ -669,8 +676,8 @@ PyObject* ExpertMatmulGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[4] == Py_True) {
       drows = New({g.n, w.inner}, x.scalar_type(), x);
       Check(lib.expert_matmul(g.t.data_ptr(), code, g.stride, g.n, w.outer,
-                              w.inner, w.t.data_ptr(), w.stride[0],
-                              w.stride[2], w.stride[1], first, experts,
+                              w.inner, w.t.data_ptr(), w.stride->expert,
+                              w.stride->outer, w.stride->inner, first, experts,
                               drows.data_ptr(), Stream(dev)));
     }
     if (a[5] == Py_True) {
@@ -692,6 +699,100 @@ PyObject* ExpertMatmulGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (turned) dw = dw.transpose(1, 2);
     }
     return Tuple({drows, dw});
+  });
+}
+
+// quantize_weights(weights) -> (codes, exponents)
+PyObject* QuantizeWeights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 1) Refuse("quantize_weights takes 1 argument");
+    const int dev = CurrentDevice();
+    Tensor w = TensorOf(a[0], "weights", dev, kRowTypes);
+    if ((w.dim() != 2 && w.dim() != 3) || w.numel() == 0 ||
+        (w.dim() == 3 && w.size(0) > SCEMB_MAX_EXPERTS)) {
+      Refuse("weights must have shape [inner, outer] or [experts, inner, "
+             "outer], none 0 and at most " +
+             std::to_string(SCEMB_MAX_EXPERTS) + " experts, got " +
+             Text(w.sizes()));
+    }
+    const bool single = w.dim() == 2;
+    if (single) w = w.unsqueeze(0);
+    const int64_t experts = w.size(0), inner = w.size(1), outer = w.size(2);
+    const WeightStrides stride(&w);
+    const auto blocks = [](int64_t v) {
+      return (v + SCEMB_BLOCK_8BIT - 1) / SCEMB_BLOCK_8BIT;
+    };
+    Tensor codes = New({experts, outer, blocks(inner) * SCEMB_BLOCK_8BIT},
+                       at::kFloat8_e4m3fn, w);
+    Tensor exponents =
+        New({experts, blocks(outer), blocks(inner)}, at::kInt, w);
+    Check(lib.quantize_weights(
+        w.data_ptr(), Code(w.scalar_type()), stride.expert, stride.inner,
+        stride.outer, inner, outer, static_cast<int32_t>(experts),
+        static_cast<uint8_t*>(codes.data_ptr()),
+        static_cast<int32_t*>(exponents.data_ptr()), Stream(dev)));
+    if (single) {
+      codes = codes.squeeze(0);
+      exponents = exponents.squeeze(0);
+    }
+    return Tuple({codes, exponents});
+  });
+}
+
+// matmul_8bit(rows, codes, exponents, inner, offsets or None, workspace) -> y
+PyObject* Matmul8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject* {
+    if (n != 6) Refuse("matmul_8bit takes 6 arguments");
+    const int dev = CurrentDevice();
+    const Tensor x = ExpertRows(a[0], dev);
+    const int64_t inner = Int(a[3]);
+    if (x.size(1) != inner) {
+      Refuse("rows must have shape [rows, " + std::to_string(inner) +
+             "] for these weights, got " + Text(x.sizes()));
+    }
+    const bool grouped = a[4] != Py_None;
+    Tensor codes =
+        TensorOf(a[1], "weights.codes", dev, Bit(at::kFloat8_e4m3fn));
+    Tensor exponents = TensorOf(a[2], "weights.exponents", dev, kI32);
+    const Tensor offsets = grouped ? OffsetsArg(a[4], dev) : Tensor();
+    const int64_t experts = grouped ? offsets.size(0) - 1 : 1;
+    const int64_t blocks = (inner + SCEMB_BLOCK_8BIT - 1) / SCEMB_BLOCK_8BIT;
+    const int64_t d = grouped ? 3 : 2;
+    const bool fits =
+        codes.dim() == d && exponents.dim() == d &&
+        (!grouped || (codes.size(0) == experts &&
+                      exponents.size(0) == experts)) &&
+        codes.size(-1) == blocks * SCEMB_BLOCK_8BIT && codes.size(-2) > 0 &&
+        exponents.size(-1) == blocks &&
+        exponents.size(-2) ==
+            (codes.size(-2) + SCEMB_BLOCK_8BIT - 1) / SCEMB_BLOCK_8BIT;
+    if (!fits) {
+      Refuse(std::string(grouped ? "weights must be of as many experts as the "
+                                   "order's, "
+                                 : "weights of several experts need an order, "
+                                   "and others have none, ") +
+             "got codes of shape " + Text(codes.sizes()) +
+             " and exponents of shape " + Text(exponents.sizes()));
+    }
+    codes = codes.contiguous();
+    exponents = exponents.contiguous();
+    if (reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 != 0) {
+      codes = codes.clone();
+    }
+    const int64_t outer = codes.size(-2);
+    const Rows r = RowsOf(x, inner);
+    const Tensor y = New({r.n, outer}, x.scalar_type(), x);
+    const size_t bytes = lib.matmul_8bit_workspace(r.n, inner);
+    if (bytes == 0) Check(SCEMB_ERR_INVALID_ARGUMENT);
+    const Tensor ws = Workspace(a[5], bytes);
+    Check(lib.matmul_8bit(
+        r.t.data_ptr(), Code(x.scalar_type()), r.stride, r.n, inner, outer,
+        static_cast<const uint8_t*>(codes.data_ptr()),
+        static_cast<const int32_t*>(exponents.data_ptr()),
+        static_cast<const int32_t*>(Data(offsets)),
+        static_cast<int32_t>(experts), y.data_ptr(), Data(ws), bytes,
+        Stream(dev)));
+    return Wrap(y);
   });
 }
 
@@ -1120,6 +1221,8 @@ PyMethodDef kMethods[] = {
     SCEMB_METHOD("tokens_from_experts_grad", TokensFromExpertsGrad),
     SCEMB_METHOD("expert_matmul", ExpertMatmul),
     SCEMB_METHOD("expert_matmul_grad", ExpertMatmulGrad),
+    SCEMB_METHOD("quantize_weights", QuantizeWeights),
+    SCEMB_METHOD("matmul_8bit", Matmul8bit),
     SCEMB_METHOD("gradient_norm", GradientNorm),
     SCEMB_METHOD("clip_gradients", ClipGradients),
     SCEMB_METHOD("adamw_sizes", AdamwSizes),

@@ -8,200 +8,8 @@ namespace scemb {
 namespace {
 
 // ---------------------------------------------------------------------------
-// A tile of the result by one work-group of kWavesM x kWavesN wavefronts. Of
-// two steps of the depth in LDS one is multiplied while the other is loaded.
+// The kernels.
 // ---------------------------------------------------------------------------
-
-template <typename T_, Along kA, Along kB, int kM_, int kN_, int kWavesM,
-          int kWavesN, bool kDirect_>
-struct Tile {
-  using T = T_;
-  static constexpr int kM = kM_, kN = kN_;
-  static constexpr int kWaves = kWavesM * kWavesN;
-  static constexpr int kThreads = kWaves * kWave;
-  static constexpr bool kDirect = kDirect_;
-  static constexpr int kFragM = kM / kWavesM / 32;
-  static constexpr int kFragN = kN / kWavesN / 32;
-  using A = Panel<T, kA, kM, kThreads>;
-  using B = Panel<T, kB, kN, kThreads>;
-  static constexpr int kDepth = A::kDepth;
-  static constexpr int kLds = A::kBytes + B::kBytes;
-  static constexpr Along kAlongA = kA, kAlongB = kB;
-
-  F32x16 acc[kFragM][kFragN];
-
-  static __device__ __forceinline__ int WaveM() {
-    return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / kWavesN *
-           (kFragM * 32);
-  }
-  static __device__ __forceinline__ int WaveN() {
-    return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWavesN *
-           (kFragN * 32);
-  }
-
-  // What half a step is multiplied from.
-  struct Fragments {
-    U32x4 a[2][kFragM];
-    U32x4 b[2][kFragN];
-  };
-  static __device__ __forceinline__ void Read(const char* lds, int half,
-                                              Fragments* f) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int j = 0; j < kFragN; ++j) {
-        f->b[q][j] =
-            B::Fragment(lds, A::kBytes, WaveN() + j * 32, half * 2 + q);
-      }
-#pragma unroll
-      for (int i = 0; i < kFragM; ++i) {
-        f->a[q][i] = A::Fragment(lds, 0, WaveM() + i * 32, half * 2 + q);
-      }
-    }
-  }
-  __device__ __forceinline__ void Multiply(const Fragments& f) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int i = 0; i < kFragM; ++i) {
-#pragma unroll
-        for (int j = 0; j < kFragN; ++j) {
-          MultiplyAdd<T>(f.b[q][j], f.a[q][i], &acc[i][j]);
-        }
-      }
-    }
-  }
-
-  // The tile's sums over `depth`. a and b are the panels' first elements; m and
-  // n (at least 1) the outer indices that exist. lds0 and lds1 are different
-  // arrays: the compiler has to see that a load into one needs no wait before
-  // the other is read.
-  __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
-                                      const T* b, int64_t b_stride, int n,
-                                      int32_t depth, char* lds0, char* lds1) {
-#pragma unroll
-    for (int i = 0; i < kFragM; ++i) {
-#pragma unroll
-      for (int j = 0; j < kFragN; ++j) acc[i][j] = F32x16{};
-    }
-    if (depth <= 0) return;
-    const int64_t a_step =
-        kA == Along::kDepth ? kDepth : kDepth * a_stride;
-    const int64_t b_step =
-        kB == Along::kDepth ? kDepth : kDepth * b_stride;
-    if constexpr (kDirect) {
-      A pa;
-      B pb;
-      pa.Start(a_stride, m);
-      pb.Start(b_stride, n);
-      const char* at_a = reinterpret_cast<const char*>(a);
-      const char* at_b = reinterpret_cast<const char*>(b);
-      const auto load = [&](char* lds) __attribute__((always_inline)) {
-        pa.Load(at_a, lds);
-        pb.Load(at_b, lds + A::kBytes);
-        at_a += a_step * sizeof(T);
-        at_b += b_step * sizeof(T);
-      };
-      // What is no whole step comes first, through registers.
-      int32_t left = depth % kDepth;
-      if (left != 0) {
-        typename A::Chunks ca;
-        typename B::Chunks cb;
-        A::template Fetch<true>(a, a_stride, m, left, &ca);
-        B::template Fetch<true>(b, b_stride, n, left, &cb);
-        A::Put(ca, lds0);
-        B::Put(cb, lds0 + A::kBytes);
-        at_a += a_step / kDepth * left * sizeof(T);
-        at_b += b_step / kDepth * left * sizeof(T);
-      } else {
-        left = kDepth;
-        load(lds0);
-      }
-      int32_t ahead = (depth - left) / kDepth;  // steps behind the current one
-      WaitLoads<0>();
-      Barrier();
-      // With two wavefronts a SIMD one reads while the other multiplies: the
-      // second half of them are a barrier behind.
-      constexpr bool kTurns = kWaves == 8;
-      const bool second =
-          __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) >= kWaves / 2;
-      if (kTurns && second) Barrier();
-      const auto half = [&](const char* now, int h) __attribute__((
-                            always_inline)) {
-        Fragments f;
-        Read(now, h, &f);
-        if constexpr (kTurns) {
-          // Whoever reads the next step first has its loads waited for by all.
-          if (h == 1) WaitLoads<0>();
-          Barrier();
-          __builtin_amdgcn_s_setprio(1);
-          Multiply(f);
-          __builtin_amdgcn_s_setprio(0);
-          Barrier();
-        } else {
-          __builtin_amdgcn_sched_barrier(0);
-          Multiply(f);
-          __builtin_amdgcn_sched_barrier(0);
-          if (h == 1) {
-            WaitLoads<0>();
-            Barrier();
-          }
-        }
-      };
-      const auto turn = [&](const char* now, char* next) __attribute__((
-                            always_inline)) {
-        if (ahead > 0) load(next);
-        half(now, 0);
-        half(now, 1);
-        --ahead;
-      };
-      while (ahead >= 1) {
-        turn(lds0, lds1);
-        turn(lds1, lds0);
-      }
-      if (ahead == 0) turn(lds0, lds1);
-      if (kTurns && !second) Barrier();
-    } else {
-      typename A::Chunks ca;
-      typename B::Chunks cb;
-      A::template Fetch<false>(a, a_stride, m, depth, &ca);
-      B::template Fetch<false>(b, b_stride, n, depth, &cb);
-      for (int32_t at = 0; at < depth; at += kDepth) {
-        char* lds = (at / kDepth & 1) ? lds1 : lds0;
-        A::Put(ca, lds);
-        B::Put(cb, lds + A::kBytes);
-        __syncthreads();
-        a += a_step;
-        b += b_step;
-        if (at + kDepth < depth) {
-          A::template Fetch<false>(a, a_stride, m, depth - at - kDepth, &ca);
-          B::template Fetch<false>(b, b_stride, n, depth - at - kDepth, &cb);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          Fragments f;
-          Read(lds, h, &f);
-          Multiply(f);
-        }
-      }
-    }
-  }
-
-  // Stores what exists of the tile: c is its first element.
-  template <typename Out>
-  __device__ __forceinline__ void Store(Out* c, int64_t stride, int m,
-                                        int n) const {
-#pragma unroll
-    for (int i = 0; i < kFragM; ++i) {
-      const int row = WaveM() + i * 32 + threadIdx.x % 32;
-#pragma unroll
-      for (int j = 0; j < kFragN; ++j) {
-        StoreColumns(c + row * stride, row < m, WaveN() + j * 32, n,
-                     acc[i][j]);
-      }
-    }
-  }
-};
 
 struct Weights {
   const void* data;
@@ -229,8 +37,9 @@ __global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
   const T* b = static_cast<const T*>(w.data) + t.segment * w.expert +
                (C::kAlongB == Along::kDepth ? column * w.stride : column);
   c.Run(x + t.row * x_stride, x_stride, m, b, w.stride, n,
-        t.segment < experts ? depth : 0, lds0, lds1);
-  c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n);
+        t.segment < experts ? depth : 0, lds0, lds1, NoScales{});
+  c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n,
+          lds0);
 }
 
 // dw[e] = the sum over the segment's rows of x[r]^T dy[r], or part `split` of
@@ -261,9 +70,9 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   C c;
   c.Run(x + s.begin * x_stride + row, x_stride, m,
         dy + s.begin * dy_stride + column, dy_stride, n, s.end - s.begin,
-        lds0, lds1);
+        lds0, lds1, NoScales{});
   c.Store(dw + (static_cast<int64_t>(part) * inner + row) * outer + column,
-          outer, m, n);
+          outer, m, n, lds0);
 }
 
 // out[e][i] = the sum over the splits of part[e][split][i], in their order.
@@ -306,13 +115,6 @@ __global__ __launch_bounds__(kJoinBlock) void JoinParts(const float* parts,
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-
-template <typename T, Along kA, Along kB, bool kDirect>
-using Small = Tile<T, kA, kB, 32, 128, 1, 4, kDirect>;
-template <typename T, Along kA, Along kB, bool kDirect>
-using Middle = Tile<T, kA, kB, 128, 128, 2, 2, kDirect>;
-template <typename T, Along kA, Along kB>
-using Large = Tile<T, kA, kB, 256, 256, 2, 4, true>;
 
 constexpr int kCus = 256;
 
@@ -366,16 +168,16 @@ struct RowsCall {
                         (kB == Along::kDepth || columns * kBytes % 16 == 0);
     const bool small = rows <= 32ll * experts;
     if (!direct) {
-      return small ? Launch<Small<T, Along::kDepth, kB, false>>()
-                   : Launch<Middle<T, Along::kDepth, kB, false>>();
+      return small ? Launch<SmallTile<T, Along::kDepth, kB, false>>()
+                   : Launch<MiddleTile<T, Along::kDepth, kB, false>>();
     }
-    if (small) return Launch<Small<T, Along::kDepth, kB, true>>();
+    if (small) return Launch<SmallTile<T, Along::kDepth, kB, true>>();
     if constexpr (kBytes == 2) {
       if (rows >= 256ll * experts) {
-        return Launch<Large<T, Along::kDepth, kB>>();
+        return Launch<LargeTile<T, Along::kDepth, kB>>();
       }
     }
-    return Launch<Middle<T, Along::kDepth, kB, true>>();
+    return Launch<MiddleTile<T, Along::kDepth, kB, true>>();
   }
 };
 
@@ -440,11 +242,11 @@ struct WeightsCall {
     const bool direct =
         Loadable(x, x_stride, kBytes) && Loadable(dy, dy_stride, kBytes) &&
         inner * kBytes % 16 == 0 && outer * kBytes % 16 == 0;
-    if (!direct) return Launch<Middle<T, kOuter, kOuter, false>>(out);
+    if (!direct) return Launch<MiddleTile<T, kOuter, kOuter, false>>(out);
     if constexpr (kBytes == 2) {
-      if (plan.large) return Launch<Large<T, kOuter, kOuter>>(out);
+      if (plan.large) return Launch<LargeTile<T, kOuter, kOuter>>(out);
     }
-    return Launch<Middle<T, kOuter, kOuter, true>>(out);
+    return Launch<MiddleTile<T, kOuter, kOuter, true>>(out);
   }
 
   int Run() const {

@@ -257,6 +257,56 @@ __device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
   }
 }
 
+// 8-bit operands (e4m3), whose values of a block share a power of two.
+struct E4m3 {
+  uint8_t bits;
+};
+// The same that are multiplied as bfloat16, which holds them and their scale
+// exactly.
+struct E4m3Wide {
+  uint8_t bits;
+};
+
+// The sum over half a step (32 of each lane's bytes) of operands in 8 bits.
+// scale: exponents, with a bias of 127. The instruction adds eight products at a
+// time, each cut off 13 bits below the largest one's power of two, and adds that
+// to the float32 sum. For 64 products of normal values that is 2.7e-6 of the
+// magnitudes' sum (of any codes 2.9e-5, 3.2e-4 at most): the codes themselves are
+// off by up to 2^-4, half a step of a 16-bit result is 2^-9 or 2^-11 of it. It is
+// far above float32's, whose results take E4m3Wide.
+__device__ __forceinline__ void MultiplyAdd8(const U32x4& b0, const U32x4& b1,
+                                             int32_t b_scale, const U32x4& a0,
+                                             const U32x4& a1, int32_t a_scale,
+                                             F32x16* acc) {
+  using V = int __attribute__((ext_vector_type(8)));
+  struct Both {
+    U32x4 v[2];
+  };
+  const V b = __builtin_bit_cast(V, (Both{{b0, b1}}));
+  const V a = __builtin_bit_cast(V, (Both{{a0, a1}}));
+  *acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+      b, a, *acc, /*e4m3*/ 0, /*e4m3*/ 0, 0, b_scale, 0, a_scale);
+}
+
+// 16 codes as bfloat16.
+struct Wide {
+  U32x4 v[2];
+};
+__device__ __forceinline__ Wide Widen(const U32x4& codes, int32_t scale) {
+  const float s =
+      __builtin_bit_cast(float, static_cast<uint32_t>(scale) << 23);
+  Wide w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c = codes[i];
+    w.v[i / 2][i % 2 * 2] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, false));
+    w.v[i / 2][i % 2 * 2 + 1] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, true));
+  }
+  return w;
+}
+
 // ---------------------------------------------------------------------------
 // Rows in segments: those of expert e are [offsets[e], offsets[e + 1]); the
 // ones behind the last belong to no expert.
@@ -288,6 +338,11 @@ template <int kRows>
 __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
                                                int32_t experts, int32_t n,
                                                int32_t tile) {
+  // Without offsets all rows are the one expert's.
+  if (offsets == nullptr) {
+    if (tile >= (n + kRows - 1) / kRows) return {-1, 0, 0};
+    return {0, tile * kRows, n};
+  }
   const int per = experts / kWave + 1;  // segments of a lane, experts + 1 in all
   const int first = LaneId() * per;
   int32_t count = 0;
@@ -369,52 +424,310 @@ __device__ __forceinline__ void StoreUpTo(T* row, int32_t column,
   }
 }
 
-// 32 columns of a row from a fragment's accumulators, rounded once. With 16
-// bits the two lanes of a row exchange halves, so that each writes 16 bytes at
-// a time.
-template <typename T>
-__device__ __forceinline__ void StoreColumns(T* row, bool exists,
-                                             int32_t column, int32_t columns,
-                                             const F32x16& acc) {
-  const int h = threadIdx.x % kWave / 32;
-  if constexpr (sizeof(T) == 4) {
-    if (!exists) return;
+// 32 rows of kFragments * 32 columns from their accumulators, rounded once. A
+// lane's values are spread over its row: they go through `lds` (the wavefront's
+// own) and leave as whole rows, neighbouring lanes writing
+// neighbouring 16 bytes. c is the first row's first element of the tile's
+// matrix of `columns` columns, of which `n` are left, and `m` rows.
+template <typename T, int kFragments>
+struct RowsOut {
+  static constexpr int kRowBytes = kFragments * 32 * sizeof(T);
+  static constexpr int kBytes = 32 * kRowBytes;
+  static constexpr int kChunks = kRowBytes / 16;
+  static_assert(kChunks == 4 || kChunks == 8 || kChunks == 16, "row of a lane");
+
+  // 16 lanes that access one chunk of 16 rows find them in different banks.
+  static __device__ __forceinline__ int Key(int row) {
+    return row / (16 / kChunks) % kChunks;
+  }
+  static __device__ __forceinline__ void Store(const F32x16* acc, char* lds,
+                                               T* c, int64_t columns, int m,
+                                               int n) {
+    constexpr int V = 16 / sizeof(T);
+    const int lane = threadIdx.x % kWave;
+    const int row = lane % 32, h = lane / 32;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      Vec<T, 4> v;
+    for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v.v[i] = acc[q * 4 + i];
-      StoreUpTo(row, column + q * 8 + h * 4, columns, v);
-    }
-  } else {
-    uint32_t x[2][4];
+      for (int q = 0; q < 4; ++q) {
+        Vec<T, 4> v;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      Vec<T, 4> v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v.v[i] = static_cast<T>(acc[q * 4 + i]);
-      const uint2 u = __builtin_bit_cast(uint2, v);
-      x[0][q] = u.x;
-      x[1][q] = u.y;
-    }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-#pragma unroll
-      for (int q = 0; q < 4; q += 2) {
-        const auto r = __builtin_amdgcn_permlane32_swap(x[w][q], x[w][q + 1],
-                                                        false, false);
-        x[w][q] = r[0];
-        x[w][q + 1] = r[1];
+        for (int i = 0; i < 4; ++i) v.v[i] = static_cast<T>(acc[f][q * 4 + i]);
+        const int at = f * 32 + q * 8 + h * 4;  // its column
+        char* p = lds + row * kRowBytes + ((at / V) ^ Key(row)) * 16 +
+                  at % V * sizeof(T);
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<U32x4*>(p) = __builtin_bit_cast(U32x4, v);
+        } else {
+          *reinterpret_cast<uint2*>(p) = __builtin_bit_cast(uint2, v);
+        }
       }
     }
-    if (!exists) return;
+    constexpr int kAtOnce = kWave / kChunks;  // rows
 #pragma unroll
-    for (int q = 0; q < 4; q += 2) {
-      const U32x4 v = {x[0][q], x[1][q], x[0][q + 1], x[1][q + 1]};
-      StoreUpTo(row, column + q * 8 + h * 8, columns,
-                __builtin_bit_cast(Vec<T, 8>, v));
+    for (int i = 0; i < 32 / kAtOnce; ++i) {
+      const int r = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+      const U32x4 x = *reinterpret_cast<const U32x4*>(
+          lds + r * kRowBytes + (chunk ^ Key(r)) * 16);
+      if (r < m) {
+        StoreUpTo(c + r * columns, chunk * V, n,
+                  __builtin_bit_cast(Vec<T, V>, x));
+      }
     }
   }
-}
+};
+
+// ---------------------------------------------------------------------------
+// A tile of the result by one work-group of kWavesM x kWavesN wavefronts. Of
+// two steps of the depth in LDS one is multiplied while the other is loaded.
+// ---------------------------------------------------------------------------
+
+template <typename T_, Along kA, Along kB, int kM_, int kN_, int kWavesM,
+          int kWavesN, bool kDirect_>
+struct Tile {
+  using T = T_;
+  static constexpr int kM = kM_, kN = kN_;
+  static constexpr int kWaves = kWavesM * kWavesN;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr bool kDirect = kDirect_;
+  static constexpr int kFragM = kM / kWavesM / 32;
+  static constexpr int kFragN = kN / kWavesN / 32;
+  using A = Panel<T, kA, kM, kThreads>;
+  using B = Panel<T, kB, kN, kThreads>;
+  static constexpr int kDepth = A::kDepth;
+  static constexpr int kLds = A::kBytes + B::kBytes;
+  static constexpr Along kAlongA = kA, kAlongB = kB;
+
+  F32x16 acc[kFragM][kFragN];
+
+  static __device__ __forceinline__ int WaveM() {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / kWavesN *
+           (kFragM * 32);
+  }
+  static __device__ __forceinline__ int WaveN() {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWavesN *
+           (kFragN * 32);
+  }
+
+  // What half a step is multiplied from.
+  struct Fragments {
+    U32x4 a[2][kFragM];
+    U32x4 b[2][kFragN];
+  };
+  static __device__ __forceinline__ void Read(const char* lds, int half,
+                                              Fragments* f) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+      for (int j = 0; j < kFragN; ++j) {
+        f->b[q][j] =
+            B::Fragment(lds, A::kBytes, WaveN() + j * 32, half * 2 + q);
+      }
+#pragma unroll
+      for (int i = 0; i < kFragM; ++i) {
+        f->a[q][i] = A::Fragment(lds, 0, WaveM() + i * 32, half * 2 + q);
+      }
+    }
+  }
+  template <typename Scales>
+  __device__ __forceinline__ void Multiply(const Fragments& f,
+                                           const Scales& scales) {
+    if constexpr (__is_same(T, E4m3Wide)) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        Wide b[kFragN];
+#pragma unroll
+        for (int j = 0; j < kFragN; ++j) b[j] = Widen(f.b[q][j], scales.b);
+#pragma unroll
+        for (int i = 0; i < kFragM; ++i) {
+          const Wide a = Widen(f.a[q][i], scales.a[i]);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+#pragma unroll
+            for (int j = 0; j < kFragN; ++j) {
+              MultiplyAdd<bf16>(b[j].v[part], a.v[part], &acc[i][j]);
+            }
+          }
+        }
+      }
+    } else if constexpr (sizeof(T) == 1) {
+#pragma unroll
+      for (int i = 0; i < kFragM; ++i) {
+#pragma unroll
+        for (int j = 0; j < kFragN; ++j) {
+          MultiplyAdd8(f.b[0][j], f.b[1][j], scales.b, f.a[0][i], f.a[1][i],
+                       scales.a[i], &acc[i][j]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int i = 0; i < kFragM; ++i) {
+#pragma unroll
+          for (int j = 0; j < kFragN; ++j) {
+            MultiplyAdd<T>(f.b[q][j], f.a[q][i], &acc[i][j]);
+          }
+        }
+      }
+    }
+  }
+
+  // The tile's sums over `depth`. a and b are the panels' first elements; m and
+  // n (at least 1) the outer indices that exist. lds0 and lds1 are different
+  // arrays: the compiler has to see that a load into one needs no wait before
+  // the other is read. scales: those of 8-bit operands, which are loaded a step
+  // ahead as the operands are.
+  template <typename Scales>
+  __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
+                                      const T* b, int64_t b_stride, int n,
+                                      int32_t depth, char* lds0, char* lds1,
+                                      Scales scales) {
+#pragma unroll
+    for (int i = 0; i < kFragM; ++i) {
+#pragma unroll
+      for (int j = 0; j < kFragN; ++j) acc[i][j] = F32x16{};
+    }
+    if (depth <= 0) return;
+    const int64_t a_step =
+        kA == Along::kDepth ? kDepth : kDepth * a_stride;
+    const int64_t b_step =
+        kB == Along::kDepth ? kDepth : kDepth * b_stride;
+    if constexpr (kDirect) {
+      A pa;
+      B pb;
+      pa.Start(a_stride, m);
+      pb.Start(b_stride, n);
+      const char* at_a = reinterpret_cast<const char*>(a);
+      const char* at_b = reinterpret_cast<const char*>(b);
+      const auto load = [&](char* lds) __attribute__((always_inline)) {
+        pa.Load(at_a, lds);
+        pb.Load(at_b, lds + A::kBytes);
+        at_a += a_step * sizeof(T);
+        at_b += b_step * sizeof(T);
+      };
+      // What is no whole step comes first, through registers (8 bits have no
+      // such steps).
+      int32_t left = sizeof(T) == 1 ? 0 : depth % kDepth;
+      if (left != 0) {
+        typename A::Chunks ca;
+        typename B::Chunks cb;
+        A::template Fetch<true>(a, a_stride, m, left, &ca);
+        B::template Fetch<true>(b, b_stride, n, left, &cb);
+        A::Put(ca, lds0);
+        B::Put(cb, lds0 + A::kBytes);
+        at_a += a_step / kDepth * left * sizeof(T);
+        at_b += b_step / kDepth * left * sizeof(T);
+      } else {
+        left = kDepth;
+        load(lds0);
+        scales.Load();
+      }
+      int32_t ahead = (depth - left) / kDepth;  // steps behind the current one
+      WaitLoads<0>();
+      Barrier();
+      // With two wavefronts a SIMD one reads while the other multiplies: the
+      // second half of them are a barrier behind.
+      constexpr bool kTurns = kWaves == 8;
+      const bool second =
+          __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) >= kWaves / 2;
+      if (kTurns && second) Barrier();
+      const auto half = [&](const char* now, int h) __attribute__((
+                            always_inline)) {
+        Fragments f;
+        Read(now, h, &f);
+        if constexpr (kTurns) {
+          // Whoever reads the next step first has its loads waited for by all.
+          if (h == 1) WaitLoads<0>();
+          Barrier();
+          __builtin_amdgcn_s_setprio(1);
+          Multiply(f, scales);
+          __builtin_amdgcn_s_setprio(0);
+          Barrier();
+        } else {
+          __builtin_amdgcn_sched_barrier(0);
+          Multiply(f, scales);
+          __builtin_amdgcn_sched_barrier(0);
+          if (h == 1) {
+            WaitLoads<0>();
+            Barrier();
+          }
+        }
+      };
+      const auto turn = [&](const char* now, char* next) __attribute__((
+                            always_inline)) {
+        scales.Take();
+        if (ahead > 0) {
+          load(next);
+          scales.Load();
+        }
+        half(now, 0);
+        half(now, 1);
+        --ahead;
+      };
+      while (ahead >= 1) {
+        turn(lds0, lds1);
+        turn(lds1, lds0);
+      }
+      if (ahead == 0) turn(lds0, lds1);
+      if (kTurns && !second) Barrier();
+    } else {
+      typename A::Chunks ca;
+      typename B::Chunks cb;
+      A::template Fetch<false>(a, a_stride, m, depth, &ca);
+      B::template Fetch<false>(b, b_stride, n, depth, &cb);
+      for (int32_t at = 0; at < depth; at += kDepth) {
+        char* lds = (at / kDepth & 1) ? lds1 : lds0;
+        A::Put(ca, lds);
+        B::Put(cb, lds + A::kBytes);
+        __syncthreads();
+        a += a_step;
+        b += b_step;
+        if (at + kDepth < depth) {
+          A::template Fetch<false>(a, a_stride, m, depth - at - kDepth, &ca);
+          B::template Fetch<false>(b, b_stride, n, depth - at - kDepth, &cb);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          Fragments f;
+          Read(lds, h, &f);
+          Multiply(f, scales);
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  // Stores what exists of the tile: c is its first element, m and n the rows
+  // and columns from there on.
+  template <typename Out>
+  __device__ __forceinline__ void Store(Out* c, int64_t stride, int m, int n,
+                                        char* lds) const {
+    using R = RowsOut<Out, kFragN>;
+    static_assert(R::kBytes * kWaves <= kLds, "every wavefront its own");
+    lds += __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * R::kBytes;
+#pragma unroll
+    for (int i = 0; i < kFragM; ++i) {
+      const int row = WaveM() + i * 32;
+      R::Store(acc[i], lds, c + row * stride + WaveN(), stride, m - row,
+               n - WaveN());
+    }
+  }
+};
+
+// No scales: operands of 16 or 32 bits.
+struct NoScales {
+  __device__ __forceinline__ void Load() {}
+  __device__ __forceinline__ void Take() {}
+};
+
+// The work-group sizes of a product, and its kinds of tiles: for few rows of an
+// expert, for most calls, and for many.
+template <typename T, Along kA, Along kB, bool kDirect>
+using SmallTile = Tile<T, kA, kB, 32, 128, 1, 4, kDirect>;
+template <typename T, Along kA, Along kB, bool kDirect>
+using MiddleTile = Tile<T, kA, kB, 128, 128, 2, 2, kDirect>;
+template <typename T, Along kA, Along kB>
+using LargeTile = Tile<T, kA, kB, 256, 256, 2, 4, true>;
 
 }  // namespace scemb

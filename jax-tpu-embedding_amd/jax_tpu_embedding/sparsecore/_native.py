@@ -91,6 +91,9 @@ EXPORTED_SYMBOLS = (
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",
+    "scemb_quantize_weights",
+    "scemb_matmul_8bit_workspace_size",
+    "scemb_matmul_8bit",
     "scemb_gradient_norm_workspace_size",
     "scemb_gradient_norm",
     "scemb_scale_gradients",
@@ -434,6 +437,9 @@ _DENSE_FUNCTIONS = (
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",
+    "scemb_quantize_weights",
+    "scemb_matmul_8bit_workspace_size",
+    "scemb_matmul_8bit",
     "scemb_gradient_norm_workspace_size",
     "scemb_gradient_norm",
     "scemb_scale_gradients",

@@ -33,6 +33,9 @@ from jax_tpu_embedding.sparsecore import _native
 # (SCEMB_ADAMW_BLOCK and SCEMB_MAX_EXPERTS).
 ADAMW_BLOCK = 256
 MAX_EXPERTS = 1024
+# Values that share a scale in 8-bit products, along each dimension
+# (SCEMB_BLOCK_8BIT).
+BLOCK_8BIT = 128
 
 _binding = None
 
@@ -293,6 +296,62 @@ def expert_matmul_grad(y_grad, rows, weights, order: ExpertOrder, *,
   return _calls().expert_matmul_grad(y_grad, rows, weights, order.offsets,
                                      bool(with_rows), bool(with_weights),
                                      _workspace)
+
+
+class Weights8(NamedTuple):
+  """Weights in 8 bits, as quantize_weights makes them: what a server keeps.
+
+  codes: float8_e4m3fn, [(experts,) outer, inner rounded up to BLOCK_8BIT]: the
+    inner dimension one after another, zeros behind it.
+  exponents: int32, [(experts,) blocks of outer, blocks of inner]: a value is
+    its code times 2^(exponent - 127).
+  inner: the inner dimension.
+  """
+
+  codes: object
+  exponents: object
+  inner: int
+
+
+def quantize_weights(weights) -> Weights8:
+  """Weights for matmul_8bit, once.
+
+  weights: [inner, outer] or [experts, inner, outer], float32, bfloat16 or
+    float16, any strides; inner at most 2^22.
+
+  BLOCK_8BIT x BLOCK_8BIT values share a scale, the least power of two (2^-126
+  at least) with no magnitude of the block above 448 times it; values are
+  rounded to the nearest code, which is 2^-4 of the value off at most (2^-10 of
+  the scale where that is more). A block that holds an infinity or a NaN is NaN
+  throughout.
+  """
+  inner = weights.shape[-2] if getattr(weights, "ndim", 0) >= 2 else 0
+  return Weights8(*_calls().quantize_weights(weights), inner)
+
+
+def matmul_8bit(rows, weights: Weights8, order: ExpertOrder | None = None):
+  """rows @ weights in 8-bit floating point, of rows' type, for serving: there
+  are no gradients, and rows that autograd would follow are refused.
+
+  rows: [rows, inner], float32, bfloat16 or float16. They are brought to 8 bits
+    in the call, as the weights are, but with a scale for each BLOCK_8BIT
+    neighbours of a row.
+  weights: quantize_weights's; of several experts with an order, else of none.
+  order: sort_by_expert's, for rows in the order of their experts as
+    tokens_to_experts returns them; rows of dropped choices are not read and
+    give zeros.
+
+  Products of codes are summed in float32 and rounded once. A row that holds an
+  infinity or a NaN gives a row of NaN.
+  """
+  calls = _calls()
+  if calls.wants_grad(rows):
+    raise ValueError("matmul_8bit has no gradients: call it under "
+                     "torch.no_grad(), or detach the rows")
+  return calls.matmul_8bit(rows, weights.codes, weights.exponents,
+                           weights.inner,
+                           None if order is None else order.offsets,
+                           _workspace)
 
 
 # ---------------------------------------------------------------------------
