@@ -279,11 +279,10 @@ __device__ __forceinline__ void MultiplyAdd8(const U32x4& b0, const U32x4& b1,
                                              const U32x4& a1, int32_t a_scale,
                                              F32x16* acc) {
   using V = int __attribute__((ext_vector_type(8)));
-  struct Both {
-    U32x4 v[2];
-  };
-  const V b = __builtin_bit_cast(V, (Both{{b0, b1}}));
-  const V a = __builtin_bit_cast(V, (Both{{a0, a1}}));
+  const V b = __builtin_bit_cast(
+      V, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+  const V a = __builtin_bit_cast(
+      V, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
   *acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
       b, a, *acc, /*e4m3*/ 0, /*e4m3*/ 0, 0, b_scale, 0, a_scale);
 }
@@ -573,6 +572,16 @@ struct Tile {
     }
   }
 
+  // The products so far are made here: without side effects, the compiler moves
+  // them behind barriers and the reads that follow.
+  __device__ __forceinline__ void Stay() {
+#pragma unroll
+    for (int i = 0; i < kFragM; ++i) {
+#pragma unroll
+      for (int j = 0; j < kFragN; ++j) asm volatile("" : "+v"(acc[i][j]));
+    }
+  }
+
   // The tile's sums over `depth`. a and b are the panels' first elements; m and
   // n (at least 1) the outer indices that exist. lds0 and lds1 are different
   // arrays: the compiler has to see that a load into one needs no wait before
@@ -642,11 +651,13 @@ struct Tile {
           Barrier();
           __builtin_amdgcn_s_setprio(1);
           Multiply(f, scales);
+          Stay();
           __builtin_amdgcn_s_setprio(0);
           Barrier();
         } else {
           __builtin_amdgcn_sched_barrier(0);
           Multiply(f, scales);
+          Stay();
           __builtin_amdgcn_sched_barrier(0);
           if (h == 1) {
             WaitLoads<0>();
