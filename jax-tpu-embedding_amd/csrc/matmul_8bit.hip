@@ -204,7 +204,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void Product8(
   __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
   int32_t tile, column;
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
-  const RowTile t = FindRowTile<C::kM>(offsets, experts, rows, tile);
+  const RowTile t = FindRowTile(offsets, experts, rows, tile, C::kM);
   if (t.segment < 0) return;
   column *= C::kN;
   const int m = min(t.end - t.row, C::kM);
@@ -229,7 +229,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void Product8(
                static_cast<int64_t>(t.row) * padded;
   const E* b = reinterpret_cast<const E*>(w) +
                (static_cast<int64_t>(t.segment) * columns + column) * padded;
-  c.Run(a, padded, m, b, padded, n, t.segment < experts ? padded : 0, lds0,
+  c.Run(a, padded, m, padded, b, padded, n, padded,
+        t.segment < experts ? padded : 0, lds0,
         lds1, scales);
   c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n,
           lds0);

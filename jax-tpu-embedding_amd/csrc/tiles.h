@@ -73,6 +73,18 @@ __device__ __forceinline__ void Barrier() {
 
 enum class Along { kDepth, kOuter };
 
+// x without its first `bytes` bytes (an even number up to 16), zeros behind.
+__device__ __forceinline__ U32x4 ShiftDown(U32x4 x, int bytes) {
+  if (bytes & 16) x = U32x4{0, 0, 0, 0};
+  if (bytes & 8) x = U32x4{x[2], x[3], 0, 0};
+  if (bytes & 4) x = U32x4{x[1], x[2], x[3], 0};
+  if (bytes & 2) {
+    x = U32x4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16,
+              x[2] >> 16 | x[3] << 16, x[3] >> 16};
+  }
+  return x;
+}
+
 template <typename T, Along kAlong, int kOuter, int kThreads>
 struct Panel {
   static constexpr int kBytes = kOuter * 128;
@@ -146,37 +158,47 @@ struct Panel {
     for (int i = 0; i < kPer; ++i) memory.ToLds(offset[i], Place(lds, i));
   }
 
-  // --- Through registers: any alignment, any number of elements (kWhole: of
-  // whole chunks). ---
+  // --- Through registers: any alignment, any number of elements (kWhole: whole
+  // chunks). ---
 
   struct Chunks {
-    Vec<T, kEach> v[kPer];
+    U32x4 v[kPer];
+    int drop[kPer];  // bytes at the start that are not the chunk's
   };
+  // `total`: elements of a whole row in memory (where kAlong is kDepth, of the
+  // whole depth). Chunks that reach past a row's end are loaded up to there, and
+  // shifted when they are put into LDS: no element by itself, no branch and no
+  // wait, so that a thread's loads are all under way while a step is multiplied.
   template <bool kWhole>
   static __device__ __forceinline__ void Fetch(const T* from, int64_t stride,
                                                int outer, int left,
-                                               Chunks* to) {
+                                               int32_t total, Chunks* to) {
+    const int along = kAlong == Along::kDepth ? left : outer;
+    const int rows = kAlong == Along::kDepth ? outer : left;
+    if (kWhole || total >= kEach) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = Column(i) * kEach;
-      const int row = Row(i);
-      // Elements of the row that exist from c on.
-      int have = (kAlong == Along::kDepth ? left : outer) - c;
-      if (row >= (kAlong == Along::kDepth ? outer : left)) have = 0;
-      const T* p = from + row * stride + c;
-      if constexpr (kWhole) {
-        // Absent chunks load one that exists.
-        const auto x = LoadVec<T, kEach>(have > 0 ? p : from);
-        to->v[i] = __builtin_bit_cast(
-            Vec<T, kEach>, have > 0 ? __builtin_bit_cast(U32x4, x)
-                                    : U32x4{0, 0, 0, 0});
-      } else if (have >= kEach) {
-        to->v[i] = LoadVec<T, kEach>(p);
-      } else {
+      for (int i = 0; i < kPer; ++i) {
+        const int c = Column(i) * kEach, row = Row(i);
+        const int have = row < rows ? min(max(along - c, 0), kEach) : 0;
+        // With nothing there: the first row's first elements, or, in a panel
+        // that begins close to the row's end, its last.
+        const T* p = have > 0 ? from + row * stride + (c + have - kEach)
+                              : from + min(0, along - kEach);
+        to->v[i] = __builtin_bit_cast(U32x4, LoadVec<T, kEach>(p));
+        to->drop[i] = (kEach - have) * static_cast<int>(sizeof(T));
+      }
+    } else if constexpr (!kWhole) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = Column(i) * kEach, row = Row(i);
+        const int have = row < rows ? along - c : 0;
+        Vec<T, kEach> x;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-          to->v[i].v[j] = j < have ? p[j] : static_cast<T>(0.f);
+          x.v[j] = j < have ? from[row * stride + c + j] : static_cast<T>(0.f);
         }
+        to->v[i] = __builtin_bit_cast(U32x4, x);
+        to->drop[i] = 0;
       }
     }
   }
@@ -185,7 +207,7 @@ struct Panel {
     for (int i = 0; i < kPer; ++i) {
       *reinterpret_cast<U32x4*>(
           lds + (i * kLoaders + threadIdx.x % kLoaders) * 16) =
-          __builtin_bit_cast(U32x4, from.v[i]);
+          ShiftDown(from.v[i], from.drop[i]);
     }
   }
 
@@ -333,14 +355,16 @@ struct RowTile {
   int32_t row;
   int32_t end;
 };
-template <int kRows>
+__device__ __forceinline__ int32_t TilesOf(const Segment& s, int32_t rows) {
+  return (s.end - s.begin + rows - 1) / rows;
+}
 __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
                                                int32_t experts, int32_t n,
-                                               int32_t tile) {
+                                               int32_t tile, int32_t tile_rows) {
   // Without offsets all rows are the one expert's.
   if (offsets == nullptr) {
-    if (tile >= (n + kRows - 1) / kRows) return {-1, 0, 0};
-    return {0, tile * kRows, n};
+    if (tile >= (n + tile_rows - 1) / tile_rows) return {-1, 0, 0};
+    return {0, tile * tile_rows, n};
   }
   const int per = experts / kWave + 1;  // segments of a lane, experts + 1 in all
   const int first = LaneId() * per;
@@ -348,7 +372,7 @@ __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
   for (int i = 0; i < per; ++i) {
     if (first + i <= experts) {
       const Segment s = SegmentOf(offsets, experts, n, first + i);
-      count += (s.end - s.begin + kRows - 1) / kRows;
+      count += TilesOf(s, tile_rows);
     }
   }
   const int32_t upto = WaveInclusiveScan(count);
@@ -358,14 +382,66 @@ __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
   int32_t at = tile - __builtin_amdgcn_readlane(upto - count, who);
   for (int i = who * per;; ++i) {
     const Segment s = SegmentOf(offsets, experts, n, i);
-    const int32_t tiles = (s.end - s.begin + kRows - 1) / kRows;
+    const int32_t tiles = TilesOf(s, tile_rows);
     if (at < tiles || i == experts) {
       return {__builtin_amdgcn_readfirstlane(i),
-              __builtin_amdgcn_readfirstlane(s.begin + at * kRows),
+              __builtin_amdgcn_readfirstlane(s.begin + at * tile_rows),
               __builtin_amdgcn_readfirstlane(s.end)};
     }
     at -= tiles;
   }
+}
+
+// The number of tiles before segment `segment`; every wavefront by itself.
+__device__ __forceinline__ int32_t TilesBefore(const int32_t* offsets,
+                                               int32_t experts, int32_t n,
+                                               int32_t segment,
+                                               int32_t tile_rows) {
+  int32_t count = 0;
+  for (int s = LaneId(); s < segment; s += kWave) {
+    count += TilesOf(SegmentOf(offsets, experts, n, s), tile_rows);
+  }
+  return __builtin_amdgcn_readlane(WaveInclusiveScan(count), kWave - 1);
+}
+
+// The expert with the `rank`th most rows (equal ones in their order); every
+// wavefront by itself.
+constexpr int kMostRanked = 4 * kWave;
+__device__ __forceinline__ int32_t ExpertOfRank(const int32_t* offsets,
+                                                int32_t experts, int32_t n,
+                                                int32_t rank) {
+  constexpr int kPer = kMostRanked / kWave;
+  int32_t rows[kPer], before[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = i * kWave + LaneId();
+    before[i] = 0;
+    rows[i] = -1;
+    if (e < experts) {
+      const Segment s = SegmentOf(offsets, experts, n, e);
+      rows[i] = s.end - s.begin;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int some = min(experts - k * kWave, kWave);
+    for (int j = 0; j < some; ++j) {
+      const int32_t other = __builtin_amdgcn_readlane(rows[k], j);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        before[i] += other > rows[i] ||
+                     (other == rows[i] && k * kWave + j < i * kWave + LaneId());
+      }
+    }
+  }
+  int32_t found = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint64_t here =
+        __ballot(before[i] == rank && i * kWave + LaneId() < experts);
+    if (here != 0) found = i * kWave + __builtin_ctzll(here);
+  }
+  return __builtin_amdgcn_readfirstlane(found);
 }
 
 // Tiles of a matrix in the order of the work-groups. Work-groups go to the
@@ -583,14 +659,16 @@ struct Tile {
   }
 
   // The tile's sums over `depth`. a and b are the panels' first elements; m and
-  // n (at least 1) the outer indices that exist. lds0 and lds1 are different
+  // n (at least 1) the outer indices that exist; the totals the elements of a row
+  // of the operands in memory. lds0 and lds1 are different
   // arrays: the compiler has to see that a load into one needs no wait before
   // the other is read. scales: those of 8-bit operands, which are loaded a step
   // ahead as the operands are.
   template <typename Scales>
   __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
-                                      const T* b, int64_t b_stride, int n,
-                                      int32_t depth, char* lds0, char* lds1,
+                                      int32_t a_total, const T* b,
+                                      int64_t b_stride, int n,
+                                      int32_t b_total, int32_t depth, char* lds0, char* lds1,
                                       Scales scales) {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
@@ -621,8 +699,8 @@ struct Tile {
       if (left != 0) {
         typename A::Chunks ca;
         typename B::Chunks cb;
-        A::template Fetch<true>(a, a_stride, m, left, &ca);
-        B::template Fetch<true>(b, b_stride, n, left, &cb);
+        A::template Fetch<true>(a, a_stride, m, left, 0, &ca);
+        B::template Fetch<true>(b, b_stride, n, left, 0, &cb);
         A::Put(ca, lds0);
         B::Put(cb, lds0 + A::kBytes);
         at_a += a_step / kDepth * left * sizeof(T);
@@ -685,8 +763,8 @@ struct Tile {
     } else {
       typename A::Chunks ca;
       typename B::Chunks cb;
-      A::template Fetch<false>(a, a_stride, m, depth, &ca);
-      B::template Fetch<false>(b, b_stride, n, depth, &cb);
+      A::template Fetch<false>(a, a_stride, m, depth, a_total, &ca);
+      B::template Fetch<false>(b, b_stride, n, depth, b_total, &cb);
       for (int32_t at = 0; at < depth; at += kDepth) {
         char* lds = (at / kDepth & 1) ? lds1 : lds0;
         A::Put(ca, lds);
@@ -695,8 +773,9 @@ struct Tile {
         a += a_step;
         b += b_step;
         if (at + kDepth < depth) {
-          A::template Fetch<false>(a, a_stride, m, depth - at - kDepth, &ca);
-          B::template Fetch<false>(b, b_stride, n, depth - at - kDepth, &cb);
+          const int32_t rest = depth - at - kDepth;
+          A::template Fetch<false>(a, a_stride, m, rest, a_total, &ca);
+          B::template Fetch<false>(b, b_stride, n, rest, b_total, &cb);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
