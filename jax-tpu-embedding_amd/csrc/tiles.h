@@ -445,8 +445,8 @@ __device__ __forceinline__ int32_t ExpertOfRank(const int32_t* offsets,
 }
 
 // Tiles of a matrix in the order of the work-groups. Work-groups go to the
-// eight XCDs in turn; each XCD gets patches of up to 32 tiles, one for each of
-// its CUs, that share operands in its L2.
+// eight XCDs in turn; each XCD gets patches of up to `most` tiles that share
+// operands in its L2, 32 being one for each of its CUs.
 struct TileGrid {
   static constexpr int32_t kMost = 1 << 30;
   int32_t rows;     // tiles
@@ -455,11 +455,13 @@ struct TileGrid {
   int32_t patch_columns;
 
   // More than a launch takes are cut: Groups() says so then.
-  TileGrid(int64_t r, int64_t c)
+  TileGrid(int64_t r, int64_t c, int64_t most = 32)
       : rows(static_cast<int32_t>(r < kMost ? r : kMost)),
         columns(static_cast<int32_t>(c < kMost ? c : kMost)) {
-    patch_columns = columns < 8 ? columns : 8;
-    patch_rows = 32 / patch_columns;
+    const int32_t size = static_cast<int32_t>(most < 1 ? 1 : most);
+    const int32_t wide = size >= 32 ? 8 : size >= 8 ? 4 : size >= 2 ? 2 : 1;
+    patch_columns = columns < wide ? columns : wide;
+    patch_rows = size / patch_columns;
     if (patch_rows > rows) patch_rows = rows;
   }
   int64_t Groups() const {
