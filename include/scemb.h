@@ -773,7 +773,7 @@ int scemb_matmul_8bit(const void* rows, int32_t type, int64_t rows_stride,
  * factor = min(1, max_norm / norm) (may be NULL; a norm that is no number makes
  * it none), single float32 values on the device: what scales the gradients down
  * to max_norm, as scemb_adamw_options_t.grad_scale_ptr or by
- * scemb_scale_gradients. Squares are summed in 64 bits, in an order that the
+ * scemb_clip_gradients. Squares are summed in 64 bits, in an order that the
  * sizes decide. A tensor of no values may be NULL. */
 typedef struct scemb_gradient {
   void* data;
@@ -787,11 +787,13 @@ int scemb_gradient_norm(const scemb_gradient_t* gradients,
                         int32_t num_gradients, double max_norm, float* norm,
                         float* factor, void* workspace, size_t workspace_bytes,
                         void* stream);
-/* Multiplies every value by *factor (on the device), in float32, rounded once;
- * with a factor of one nothing is read or written. */
-int scemb_scale_gradients(const scemb_gradient_t* gradients,
-                          int32_t num_gradients, const float* factor,
-                          void* stream);
+/* The same norm, and every value multiplied by the factor in place, in float32,
+ * rounded once; where the factor is one nothing is written. The workspace is that
+ * of the norm. */
+int scemb_clip_gradients(const scemb_gradient_t* gradients,
+                         int32_t num_gradients, double max_norm, float* norm,
+                         void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* AdamW over many tensors. Tensor i's moments are the values from
  * first_i = sum over j < i of numel_j rounded up to SCEMB_ADAMW_BLOCK on.

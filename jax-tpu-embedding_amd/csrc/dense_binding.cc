@@ -50,7 +50,7 @@ struct Library {
   decltype(&scemb_matmul_8bit) matmul_8bit;
   decltype(&scemb_gradient_norm_workspace_size) gradient_norm_workspace;
   decltype(&scemb_gradient_norm) gradient_norm;
-  decltype(&scemb_scale_gradients) scale_gradients;
+  decltype(&scemb_clip_gradients) clip_gradients;
   decltype(&scemb_adamw_update) adamw_update;
   decltype(&scemb_adamw_moments) adamw_moments;
 };
@@ -1101,31 +1101,22 @@ struct Gradients {
   int32_t size() const { return static_cast<int32_t>(list.size()); }
 };
 
-struct Norm {
-  Tensor norm;
-  Tensor factor;
-};
-
-// max_norm: None for no factor.
-Norm NormOf(const Gradients& g, PyObject* max_norm, PyObject* workspace,
-            int dev) {
-  double limit = 0.0;
-  if (max_norm != Py_None) {
-    limit = Float(max_norm);
-    if (!(limit >= 0)) Refuse("max_norm must not be negative, got " + Text(limit));
+double LimitOf(PyObject* max_norm) {
+  const double limit = Float(max_norm);
+  if (!(limit >= 0)) {
+    Refuse("max_norm must not be negative, got " + Text(limit));
   }
-  const auto options =
-      at::TensorOptions(at::kFloat).device(at::kCUDA, dev);
-  Norm out;
-  out.norm = at::empty({}, options);
-  if (max_norm != Py_None) out.factor = at::empty({}, options);
-  const size_t bytes = lib.gradient_norm_workspace(g.list.data(), g.size());
-  if (bytes == 0) Check(SCEMB_ERR_INVALID_ARGUMENT);
-  const Tensor ws = Workspace(workspace, bytes);
-  Check(lib.gradient_norm(g.list.data(), g.size(), limit, FloatData(out.norm),
-                          FloatData(out.factor), Data(ws), bytes,
-                          Stream(dev)));
-  return out;
+  return limit;
+}
+
+Tensor NormWorkspace(const Gradients& g, PyObject* get, size_t* bytes) {
+  *bytes = lib.gradient_norm_workspace(g.list.data(), g.size());
+  if (*bytes == 0) Check(SCEMB_ERR_INVALID_ARGUMENT);
+  return Workspace(get, *bytes);
+}
+
+Tensor Single(int dev) {
+  return at::empty({}, at::TensorOptions(at::kFloat).device(at::kCUDA, dev));
 }
 
 // gradient_norm(grads, max_norm, workspace) -> (norm, factor)
@@ -1134,8 +1125,16 @@ PyObject* GradientNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 3) Refuse("gradient_norm takes 3 arguments");
     const int dev = CurrentDevice();
     const Sequence grads(a[0], "grads must be a sequence of tensors");
-    const Norm out = NormOf(Gradients(grads, dev, false), a[1], a[2], dev);
-    return Tuple({out.norm, out.factor});
+    const Gradients g(grads, dev, false);
+    const bool limited = a[1] != Py_None;
+    const double limit = limited ? LimitOf(a[1]) : 0.0;
+    const Tensor norm = Single(dev);
+    const Tensor factor = limited ? Single(dev) : Tensor();
+    size_t bytes = 0;
+    const Tensor ws = NormWorkspace(g, a[2], &bytes);
+    Check(lib.gradient_norm(g.list.data(), g.size(), limit, FloatData(norm),
+                            FloatData(factor), Data(ws), bytes, Stream(dev)));
+    return Tuple({norm, factor});
   });
 }
 
@@ -1155,13 +1154,16 @@ PyObject* ClipGradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     CheckApart(&spans, "grads");
     if (a[1] == Py_None) Refuse("max_norm must be a number");
-    const Norm out = NormOf(g, a[1], a[2], dev);
-    Check(lib.scale_gradients(g.list.data(), g.size(), FloatData(out.factor),
-                              Stream(dev)));
+    const double limit = LimitOf(a[1]);
+    const Tensor norm = Single(dev);
+    size_t bytes = 0;
+    const Tensor ws = NormWorkspace(g, a[2], &bytes);
+    Check(lib.clip_gradients(g.list.data(), g.size(), limit, FloatData(norm),
+                             Data(ws), bytes, Stream(dev)));
     for (Py_ssize_t i = 0; i < grads.n; ++i) {
       if (grads[i] != Py_None) Written(THPVariable_Unpack(grads[i]));
     }
-    return Wrap(out.norm);
+    return Wrap(norm);
   });
 }
 

@@ -66,7 +66,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
     s = {t.row, min(t.end, t.row + piece)};
   } else {
     // The longest sums first: one that begins last is all that runs then (64
-    // experts, the largest with a quarter of all rows: 1345 us in their order on the XCDs, 1081).
+    // experts, the largest with a quarter of all rows: 1345 us in their order,
+    // 1081 this way).
     if (experts <= kMostRanked) {
       part = ExpertOfRank(offsets, experts, rows, part);
     }
@@ -126,8 +127,6 @@ __global__ __launch_bounds__(kJoinBlock) void JoinPieces(
 // Host side.
 // ---------------------------------------------------------------------------
 
-constexpr int kCus = 256;
-
 // Whether rows of `stride` values can be loaded 16 bytes a lane at offsets of
 // 32 bits within a panel of 256.
 bool Loadable(const void* p, int64_t stride, int bytes) {
@@ -183,7 +182,7 @@ struct RowsCall {
     }
     if (small) return Launch<SmallTile<T, Along::kDepth, kB, true>>();
     if constexpr (kBytes == 2) {
-      if (rows >= 256ll * experts) {
+      if (rows >= 256ll * experts && WorthLarge(rows, columns)) {
         return Launch<LargeTile<T, Along::kDepth, kB>>();
       }
     }

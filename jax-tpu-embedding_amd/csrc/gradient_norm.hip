@@ -20,18 +20,23 @@ constexpr int64_t kMostParts = 8192;  // stretches of a call, about
 constexpr int kFinishThreads = 1024;
 
 // Tensors of a launch: what the kernel's arguments hold.
-constexpr int kMaxTensors = 168;
+constexpr int kMaxTensors = 320;
 struct Tensors {
-  void* data[kMaxTensors];
-  uint64_t size[kMaxTensors];   // number of values * 4 + type
-  uint32_t first[kMaxTensors];  // first work-group
+  uint64_t data[kMaxTensors];  // address, and the type from bit 48 on
+  uint32_t size[kMaxTensors];  // number of values
   int32_t n;
-  int32_t rounds;  // of a work-group
+  int32_t log_step;  // values of a work-group
 };
-static_assert(sizeof(Tensors) <= 3584, "kernel arguments");
-static_assert(SCEMB_F32 < 4 && SCEMB_BF16 < 4 && SCEMB_F16 < 4, "two bits");
+static_assert(sizeof(Tensors) <= 3904, "kernel arguments are 4096 bytes");
 
-// The work-group's stretch.
+__device__ __forceinline__ int32_t TypeAt(uint64_t data) {
+  return static_cast<int32_t>(data >> 48);
+}
+__device__ __forceinline__ char* AddressAt(uint64_t data) {
+  return reinterpret_cast<char*>(data & ((1ull << 48) - 1));
+}
+
+// The work-group's stretch. A lane counts the stretches of neighbouring tensors.
 struct Stretch {
   char* data;
   int32_t n;
@@ -39,18 +44,27 @@ struct Stretch {
 };
 __device__ __forceinline__ Stretch StretchOf(const Tensors& t,
                                              uint32_t group) {
-  int i = -1;
+  constexpr int kPer = kMaxTensors / kWave;
+  const uint64_t step = 1ull << t.log_step;
+  const auto stretches = [&](int i) -> uint32_t {
+    return i < t.n ? static_cast<uint32_t>((t.size[i] + step - 1) >> t.log_step)
+                   : 0;
+  };
+  const int first = LaneId() * kPer;
+  uint32_t mine = 0;
 #pragma unroll
-  for (int k = 0; k < (kMaxTensors + kWave - 1) / kWave; ++k) {
-    const int at = threadIdx.x % kWave + k * kWave;
-    i += __popcll(__ballot(at < t.n && t.first[at] <= group));
-  }
+  for (int i = 0; i < kPer; ++i) mine += stretches(first + i);
+  const uint32_t upto = WaveInclusiveScan(mine);
+  const int who = __builtin_ctzll(__ballot(upto > group));
+  uint32_t at = group - __builtin_amdgcn_readlane(upto - mine, who);
+  int i = who * kPer;
+  for (uint32_t n = stretches(i); at >= n; n = stretches(++i)) at -= n;
   i = __builtin_amdgcn_readfirstlane(i);
-  const int64_t step = t.rounds * kRound;
-  const int64_t begin = (group - t.first[i]) * step;
-  const int32_t type = static_cast<int32_t>(t.size[i] & 3);
-  const int64_t left = static_cast<int64_t>(t.size[i] >> 2) - begin;
-  return {static_cast<char*>(t.data[i]) + begin * (type == SCEMB_F32 ? 4 : 2),
+  const uint64_t begin = static_cast<uint64_t>(
+      __builtin_amdgcn_readfirstlane(at)) << t.log_step;
+  const uint64_t left = t.size[i] - begin;
+  const int32_t type = TypeAt(t.data[i]);
+  return {AddressAt(t.data[i]) + begin * (type == SCEMB_F32 ? 4 : 2),
           static_cast<int32_t>(left < step ? left : step), type};
 }
 
@@ -89,7 +103,7 @@ __device__ __forceinline__ double SumSquares(const T* p, int32_t n) {
   return sum[0] + sum[1];
 }
 
-// The sum over a work-group's lanes, in thread 0.
+// The sum over a work-group's lanes, in every one of them.
 template <int kAll>
 __device__ __forceinline__ double GroupSum(double x) {
   __shared__ double waves[kAll / kWave];
@@ -97,9 +111,8 @@ __device__ __forceinline__ double GroupSum(double x) {
   for (int d = kWave / 2; d > 0; d /= 2) x += __shfl_down(x, d, kWave);
   if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = x;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kAll / kWave; ++w) x += waves[w];
-  }
+  x = waves[0];
+  for (int w = 1; w < kAll / kWave; ++w) x += waves[w];
   return x;
 }
 
@@ -119,19 +132,98 @@ __global__ __launch_bounds__(kThreads) void SquareSums(Tensors t,
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
+// A norm that is no number makes the factor none.
+__device__ __forceinline__ float FactorOf(double norm, double max_norm) {
+  return norm <= max_norm ? 1.f : static_cast<float>(max_norm / norm);
+}
+
+// The work-groups' sums added up by one.
+template <int kAll>
+__device__ __forceinline__ double SumOf(const double* parts, int32_t n) {
+  double sum = 0.0;
+#pragma unroll 4
+  for (int32_t i = threadIdx.x; i < n; i += kAll) sum += parts[i];
+  return GroupSum<kAll>(sum);
+}
+
 __global__ __launch_bounds__(kFinishThreads) void FinishNorm(
     const double* parts, int32_t n, double max_norm, float* norm,
     float* factor) {
-  double sum = 0.0;
-  for (int32_t i = threadIdx.x; i < n; i += kFinishThreads) sum += parts[i];
-  sum = GroupSum<kFinishThreads>(sum);
+  const double root = sqrt(SumOf<kFinishThreads>(parts, n));
   if (threadIdx.x == 0) {
-    const double root = sqrt(sum);
     *norm = static_cast<float>(root);
-    // A norm that is no number makes the factor none.
-    if (factor != nullptr) {
-      *factor = root <= max_norm ? 1.f : static_cast<float>(max_norm / root);
+    if (factor != nullptr) *factor = FactorOf(root, max_norm);
+  }
+}
+
+// All of a few values by one work-group in one launch, 8 values of a lane at a
+// time: two launches are 4 us each, however little they do.
+constexpr int64_t kFew = 32768;
+constexpr int kEach = 8;
+template <typename T>
+__device__ __forceinline__ double SquaresOf(const T* p, int32_t n) {
+  double sum = 0.0;
+  if (n >= kEach) {
+    constexpr int V = kVec<T>;
+#pragma unroll
+    for (int j = 0; j < kEach; j += V) {
+      const auto x = LoadVec<T, V>(p + j);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double v = static_cast<double>(static_cast<float>(x.v[i]));
+        sum = fma(v, v, sum);
+      }
     }
+  } else {
+    for (int32_t j = 0; j < n; ++j) {
+      const double v = static_cast<double>(static_cast<float>(p[j]));
+      sum = fma(v, v, sum);
+    }
+  }
+  return sum;
+}
+__global__ __launch_bounds__(kFinishThreads) void NormOfFew(
+    Tensors t, double max_norm, float* norm, float* factor) {
+  __shared__ int32_t first[kMaxTensors + 1];
+  __shared__ int32_t scratch[kFinishThreads / kWave + 1];
+  const int32_t i = threadIdx.x;
+  const int32_t mine =
+      i < t.n ? static_cast<int32_t>((t.size[i] + kEach - 1) / kEach) : 0;
+  int32_t all;
+  const int32_t before =
+      BlockExclusiveScan<int32_t, kFinishThreads>(mine, scratch, &all);
+  if (i < t.n) first[i] = before;
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll 4
+  for (int32_t v = threadIdx.x; v < all; v += kFinishThreads) {
+    // The last tensor that begins at or before v (those of no values are not
+    // given).
+    int32_t lo = 0, hi = t.n;
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) / 2;
+      if (first[mid] <= v) {
+        lo = mid;
+      } else {
+        hi = mid;
+      }
+    }
+    const int32_t at = (v - first[lo]) * kEach;
+    const int32_t left = static_cast<int32_t>(t.size[lo]) - at;
+    const uint64_t data = t.data[lo];
+    const char* p = AddressAt(data);
+    if (TypeAt(data) == SCEMB_F32) {
+      sum += SquaresOf(reinterpret_cast<const float*>(p) + at, left);
+    } else if (TypeAt(data) == SCEMB_BF16) {
+      sum += SquaresOf(reinterpret_cast<const bf16*>(p) + at, left);
+    } else {
+      sum += SquaresOf(reinterpret_cast<const f16*>(p) + at, left);
+    }
+  }
+  const double root = sqrt(GroupSum<kFinishThreads>(sum));
+  if (threadIdx.x == 0) {
+    *norm = static_cast<float>(root);
+    if (factor != nullptr) *factor = FactorOf(root, max_norm);
   }
 }
 
@@ -169,10 +261,23 @@ __device__ __forceinline__ void ScaleAll(T* p, int32_t n, float factor) {
   }
 }
 
+// Scales by *factor; with parts every work-group finds the factor itself (a
+// launch less), and the first stores the norm.
+constexpr int64_t kOwnSums = 2048;  // parts up to which that is done
 template <bool kStream>
-__global__ __launch_bounds__(kThreads) void ScaleTensors(Tensors t,
-                                                         const float* factor) {
-  const float f = *factor;
+__global__ __launch_bounds__(kThreads) void ScaleTensors(
+    Tensors t, const double* parts, int32_t n, double max_norm, float* norm,
+    const float* factor) {
+  float f;
+  if (parts != nullptr) {
+    const double root = sqrt(SumOf<kThreads>(parts, n));
+    f = FactorOf(root, max_norm);
+    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
+      *norm = static_cast<float>(root);
+    }
+  } else {
+    f = *factor;
+  }
   if (f == 1.f) return;
   const Stretch s = StretchOf(t, blockIdx.x);
   if (s.type == SCEMB_F32) {
@@ -207,22 +312,30 @@ int CheckGradients(const scemb_gradient_t* gradients, int32_t n) {
   return 0;
 }
 
+constexpr int kLogRound = 12;
+static_assert(kRound == 1 << kLogRound, "values of a work-group at a time");
+constexpr int kMostLog = 30;
+
 struct Plan {
   int64_t values = 0;
   int64_t bytes = 0;
-  int32_t rounds = 1;  // of a work-group
-  int64_t parts = 0;   // work-groups
+  int32_t log_step = kLogRound;
+  int64_t parts = 0;  // work-groups
 };
+// A tensor of more than 32 bits of values goes in pieces of whole stretches.
+constexpr int64_t kMostValues = 1ll << 31;
+
 Plan PlanOf(const scemb_gradient_t* gradients, int32_t n) {
   Plan p;
   for (int32_t i = 0; i < n; ++i) {
     p.values += gradients[i].numel;
     p.bytes += gradients[i].numel * TypeBytes(gradients[i].type);
   }
-  p.rounds = static_cast<int32_t>(std::min<int64_t>(
-      std::max<int64_t>(CeilDiv(p.values, kRound * kMostParts), 1), 1 << 16));
+  while (p.log_step < kMostLog && p.values >> p.log_step > kMostParts) {
+    ++p.log_step;
+  }
   for (int32_t i = 0; i < n; ++i) {
-    p.parts += CeilDiv(gradients[i].numel, kRound * p.rounds);
+    p.parts += CeilDiv(gradients[i].numel, 1ll << p.log_step);
   }
   return p;
 }
@@ -234,26 +347,83 @@ int ForTensors(const scemb_gradient_t* gradients, int32_t n, const Plan& plan,
                const F& launch) {
   Tensors t;
   t.n = 0;
-  t.rounds = plan.rounds;
+  t.log_step = plan.log_step;
   int64_t groups = 0, done = 0;
   for (int32_t i = 0; i < n; ++i) {
-    const int64_t mine = CeilDiv(gradients[i].numel, kRound * plan.rounds);
-    if (mine == 0) continue;
-    if (t.n == kMaxTensors || groups + mine > MostGroups(kThreads)) {
-      const int rc = launch(t, groups, done);
-      if (rc != 0) return rc;
-      done += groups;
-      groups = 0;
-      t.n = 0;
+    const scemb_gradient_t& g = gradients[i];
+    for (int64_t at = 0; at < g.numel; at += kMostValues) {
+      const int64_t values = std::min(g.numel - at, kMostValues);
+      const int64_t mine = CeilDiv(values, 1ll << plan.log_step);
+      if (t.n == kMaxTensors || groups + mine > MostGroups(kThreads)) {
+        const int rc = launch(t, groups, done);
+        if (rc != 0) return rc;
+        done += groups;
+        groups = 0;
+        t.n = 0;
+      }
+      t.data[t.n] = reinterpret_cast<uint64_t>(
+                        static_cast<char*>(g.data) + at * TypeBytes(g.type)) |
+                    static_cast<uint64_t>(g.type) << 48;
+      t.size[t.n] = static_cast<uint32_t>(values);
+      ++t.n;
+      groups += mine;
     }
-    t.data[t.n] = gradients[i].data;
-    t.size[t.n] = static_cast<uint64_t>(gradients[i].numel) << 2 |
-                  static_cast<uint64_t>(gradients[i].type);
-    t.first[t.n] = static_cast<uint32_t>(groups);
-    ++t.n;
-    groups += mine;
   }
   return t.n == 0 ? 0 : launch(t, groups, done);
+}
+
+int Sum(const scemb_gradient_t* gradients, int32_t n, const Plan& plan,
+        double* parts, hipStream_t stream) {
+  const bool past_cache = plan.bytes > kCacheBytes;
+  return ForTensors(
+      gradients, n, plan, [&](const Tensors& t, int64_t groups, int64_t done) {
+        const dim3 grid(static_cast<uint32_t>(groups));
+        if (past_cache) {
+          hipLaunchKernelGGL(SquareSums<true>, grid, dim3(kThreads), 0, stream,
+                             t, parts + done);
+        } else {
+          hipLaunchKernelGGL(SquareSums<false>, grid, dim3(kThreads), 0,
+                             stream, t, parts + done);
+        }
+        SCEMB_LAUNCH_CHECK();
+        return 0;
+      });
+}
+
+int Finish(const Plan& plan, const double* parts, double max_norm, float* norm,
+           float* factor, hipStream_t stream) {
+  hipLaunchKernelGGL(FinishNorm, dim3(1), dim3(kFinishThreads), 0, stream,
+                     parts, static_cast<int32_t>(plan.parts), max_norm, norm,
+                     factor);
+  SCEMB_LAUNCH_CHECK();
+  return 0;
+}
+
+// Nonzero: an error, said.
+int CheckNorm(const scemb_gradient_t* gradients, int32_t n, double max_norm,
+              const float* norm) {
+  const int bad = CheckGradients(gradients, n);
+  if (bad != 0) return bad;
+  if (norm == nullptr || !(max_norm >= 0)) {
+    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
+                "gradient norm: the norm's place is missing, or max_norm is "
+                "negative or no number");
+  }
+  return 0;
+}
+
+// The sums' places and a factor's in the workspace.
+struct Space {
+  double* parts;
+  float* factor;
+  Space(Arena* arena, const Plan& plan)
+      : parts(arena->Take<double>(plan.parts)), factor(arena->Take<float>(1)) {}
+};
+int CheckSpace(const Arena& arena, const Plan& plan) {
+  if (arena.measuring() || arena.overflow() || plan.parts > 0x7fffffff) {
+    return Fail(SCEMB_ERR_WORKSPACE, "gradient norm: workspace too small");
+  }
+  return 0;
 }
 
 }  // namespace
@@ -266,7 +436,7 @@ size_t scemb_gradient_norm_workspace_size(const scemb_gradient_t* gradients,
   using namespace scemb;
   if (CheckGradients(gradients, num_gradients) != 0) return 0;
   Arena arena(nullptr, 0);
-  arena.Take<double>(PlanOf(gradients, num_gradients).parts);
+  Space(&arena, PlanOf(gradients, num_gradients));
   return arena.used();
 }
 
@@ -275,65 +445,65 @@ int scemb_gradient_norm(const scemb_gradient_t* gradients,
                         float* factor, void* workspace, size_t workspace_bytes,
                         void* stream) {
   using namespace scemb;
-  const int bad = CheckGradients(gradients, num_gradients);
+  const int bad = CheckNorm(gradients, num_gradients, max_norm, norm);
   if (bad != 0) return bad;
-  if (norm == nullptr || !(max_norm >= 0)) {
-    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
-                "gradient norm: the norm's place is missing, or max_norm is "
-                "negative or no number");
-  }
   const Plan plan = PlanOf(gradients, num_gradients);
   Arena arena(workspace, workspace_bytes);
-  double* parts = arena.Take<double>(plan.parts);
-  if (workspace == nullptr || arena.overflow() || plan.parts > 0x7fffffff) {
-    return Fail(SCEMB_ERR_WORKSPACE, "gradient norm: workspace too small");
-  }
+  const Space space(&arena, plan);
+  const int small = CheckSpace(arena, plan);
+  if (small != 0) return small;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool past_cache = plan.bytes > kCacheBytes;
-  const int rc = ForTensors(
-      gradients, num_gradients, plan,
-      [&](const Tensors& t, int64_t groups, int64_t done) {
-        const dim3 grid(static_cast<uint32_t>(groups));
-        if (past_cache) {
-          hipLaunchKernelGGL(SquareSums<true>, grid, dim3(kThreads), 0, s, t,
-                             parts + done);
-        } else {
-          hipLaunchKernelGGL(SquareSums<false>, grid, dim3(kThreads), 0, s, t,
-                             parts + done);
-        }
-        SCEMB_LAUNCH_CHECK();
-        return 0;
-      });
+  int32_t some = 0;  // tensors with values
+  for (int32_t i = 0; i < num_gradients; ++i) some += gradients[i].numel > 0;
+  if (plan.values <= kFew && some > 0 && some <= kMaxTensors) {
+    return ForTensors(gradients, num_gradients, plan,
+                      [&](const Tensors& t, int64_t, int64_t) {
+                        hipLaunchKernelGGL(NormOfFew, dim3(1),
+                                           dim3(kFinishThreads), 0, s, t,
+                                           max_norm, norm, factor);
+                        SCEMB_LAUNCH_CHECK();
+                        return 0;
+                      });
+  }
+  const int rc = Sum(gradients, num_gradients, plan, space.parts, s);
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(FinishNorm, dim3(1), dim3(kFinishThreads), 0, s, parts,
-                     static_cast<int32_t>(plan.parts), max_norm, norm, factor);
-  SCEMB_LAUNCH_CHECK();
-  return 0;
+  return Finish(plan, space.parts, max_norm, norm, factor, s);
 }
 
-int scemb_scale_gradients(const scemb_gradient_t* gradients,
-                          int32_t num_gradients, const float* factor,
-                          void* stream) {
+int scemb_clip_gradients(const scemb_gradient_t* gradients,
+                         int32_t num_gradients, double max_norm, float* norm,
+                         void* workspace, size_t workspace_bytes,
+                         void* stream) {
   using namespace scemb;
-  const int bad = CheckGradients(gradients, num_gradients);
+  const int bad = CheckNorm(gradients, num_gradients, max_norm, norm);
   if (bad != 0) return bad;
-  if (factor == nullptr) {
-    return Fail(SCEMB_ERR_INVALID_ARGUMENT,
-                "scale gradients: the factor is missing");
-  }
   const Plan plan = PlanOf(gradients, num_gradients);
+  Arena arena(workspace, workspace_bytes);
+  const Space space(&arena, plan);
+  const int small = CheckSpace(arena, plan);
+  if (small != 0) return small;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  int rc = Sum(gradients, num_gradients, plan, space.parts, s);
+  if (rc != 0) return rc;
+  const bool own_sums = plan.parts > 0 && plan.parts <= kOwnSums;
+  if (!own_sums) {
+    rc = Finish(plan, space.parts, max_norm, norm, space.factor, s);
+    if (rc != 0) return rc;
+  }
   const bool past_cache = plan.bytes > kCacheBytes;
   return ForTensors(
       gradients, num_gradients, plan,
-      [&](const Tensors& t, int64_t groups, int64_t) {
+      [&](const Tensors& t, int64_t groups, int64_t done) {
         const dim3 grid(static_cast<uint32_t>(groups));
+        const double* parts = own_sums ? space.parts : nullptr;
+        const int32_t n = static_cast<int32_t>(plan.parts);
+        float* to = done == 0 ? norm : nullptr;
         if (past_cache) {
           hipLaunchKernelGGL(ScaleTensors<true>, grid, dim3(kThreads), 0, s, t,
-                             factor);
+                             parts, n, max_norm, to, space.factor);
         } else {
           hipLaunchKernelGGL(ScaleTensors<false>, grid, dim3(kThreads), 0, s,
-                             t, factor);
+                             t, parts, n, max_norm, to, space.factor);
         }
         SCEMB_LAUNCH_CHECK();
         return 0;

@@ -294,7 +294,7 @@ struct Call8 {
     if (rows <= 32ll * experts) {
       return Launch<SmallTile<E, kDepth, kDepth, true>>();
     }
-    if (rows >= 256ll * experts) {
+    if (rows >= 256ll * experts && WorthLarge(rows, columns)) {
       return Launch<LargeTile<E, kDepth, kDepth>>();
     }
     return Launch<MiddleTile<E, kDepth, kDepth, true>>();

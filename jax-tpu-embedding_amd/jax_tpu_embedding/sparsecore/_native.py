@@ -96,7 +96,7 @@ EXPORTED_SYMBOLS = (
     "scemb_matmul_8bit",
     "scemb_gradient_norm_workspace_size",
     "scemb_gradient_norm",
-    "scemb_scale_gradients",
+    "scemb_clip_gradients",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )
@@ -442,7 +442,7 @@ _DENSE_FUNCTIONS = (
     "scemb_matmul_8bit",
     "scemb_gradient_norm_workspace_size",
     "scemb_gradient_norm",
-    "scemb_scale_gradients",
+    "scemb_clip_gradients",
     "scemb_adamw_update",
     "scemb_adamw_moments",
 )
