@@ -4,7 +4,8 @@ Tables and dense weights side by side: the lookup's activations of all
 features go through layer norm to a router, every sample through its best
 experts and back, and a last layer norm to a logit. The tables are updated by
 embedding.tpu_sparse_dense_matmul_grad (Adagrad), everything else by
-dense.adamw_update with moments of 8 or 32 bits.
+dense.adamw_update with moments of 8 or 32 bits; all gradients may be clipped to
+a global norm before. Scoring can take the experts' weights in 8 bits.
 
   python -m jax_tpu_embedding.sparsecore.examples.ranking_moe --steps 100
 """
@@ -36,6 +37,7 @@ class Config:
   state_bits: int = 8
   learning_rate: float = 2e-3
   table_learning_rate: float = 0.05
+  max_norm: float | None = None  # of all gradients
   seed: int = 0
 
   @property
@@ -94,24 +96,36 @@ class RankingModel:
         num_sc_per_device=1)
     return pre, [a.detach().requires_grad_() for a in acts]
 
-  def logits(self, acts):
-    """A logit per sample from the features' activations."""
+  def logits(self, acts, experts_8=None):
+    """A logit per sample from the features' activations. experts_8: the
+    experts' weights in 8 bits (quantize_experts), for scoring."""
     t = _native.torch()
     c, w = self.config, self.weights
     x = dense.layer_norm(t.cat(acts, 1), w["norm_in"], w["norm_in_bias"])
     scores, ids = (x @ w["router"]).topk(c.choices, dim=1)
+    # How many rows an expert gets stays on the GPU: nothing waits for it.
     order = dense.sort_by_expert(ids, c.experts)
+    def product(rows, name):
+      if experts_8 is None:
+        return dense.expert_matmul(rows, w[name], order)
+      return dense.matmul_8bit(rows, experts_8[name], order)
     rows = dense.tokens_to_experts(x, order)
-    # The experts' layers are products of sizes that the host gives, so this
-    # waits for the GPU, and a step as written here cannot be captured. A model
-    # with a fixed capacity for each expert needs no such wait.
-    first = order.offsets.tolist()
-    rows = t.cat([
-        t.relu(rows[first[e]:first[e + 1]] @ w["up"][e]) @ w["down"][e]
-        for e in range(c.experts)])
+    rows = product(t.relu(product(rows, "up")), "down")
     y = dense.tokens_from_experts(rows, scores.softmax(1), order)
     y = dense.layer_norm(x + y, w["norm_out"], w["norm_out_bias"])
     return (y @ w["logit"]).squeeze(1)
+
+  def quantize_experts(self):
+    """The experts' weights in 8 bits, once for many batches to score."""
+    return {k: dense.quantize_weights(self.weights[k].detach())
+            for k in ("up", "down")}
+
+  def score(self, ids, experts_8=None):
+    """The probability of a click per sample."""
+    t = _native.torch()
+    with t.no_grad():
+      _, acts = self.lookup(ids)
+      return self.logits(acts, experts_8).sigmoid()
 
   def step(self, ids, clicks):
     """One training step; returns the loss before it."""
@@ -121,11 +135,17 @@ class RankingModel:
         self.logits(acts), clicks)
     params = list(self.weights.values())
     grads = t.autograd.grad(loss, acts + params)
+    of_acts, of_params = list(grads[:len(acts)]), grads[len(acts):]
+    factor = None
+    if self.config.max_norm is not None:
+      _, factor = dense.gradient_norm(grads, max_norm=self.config.max_norm)
+      of_acts = [g * factor for g in of_acts]
     self.tables = embedding.tpu_sparse_dense_matmul_grad(
-        list(grads[:len(acts)]), pre, self.tables, self.feature_specs,
-        global_device_count=1, num_sc_per_device=1)
-    dense.adamw_update(params, grads[len(acts):], self.state,
-                       learning_rate=self.config.learning_rate)
+        of_acts, pre, self.tables, self.feature_specs, global_device_count=1,
+        num_sc_per_device=1)
+    dense.adamw_update(params, of_params, self.state,
+                       learning_rate=self.config.learning_rate,
+                       grad_scale=factor)
     return loss.detach()
 
 
@@ -161,9 +181,10 @@ def main():
   parser.add_argument("--batch", type=int, default=Config.batch)
   parser.add_argument("--state_bits", type=int, default=Config.state_bits,
                       choices=(8, 32))
+  parser.add_argument("--max_norm", type=float, default=None)
   args = parser.parse_args()
-  losses = train(Config(batch=args.batch, state_bits=args.state_bits),
-                 args.steps)
+  losses = train(Config(batch=args.batch, state_bits=args.state_bits,
+                        max_norm=args.max_norm), args.steps)
   for i in range(0, len(losses), max(1, len(losses) // 10)):
     print(f"step {i}: loss {losses[i]:.4f}")
   print(f"step {len(losses) - 1}: loss {losses[-1]:.4f}")
