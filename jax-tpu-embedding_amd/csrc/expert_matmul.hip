@@ -1,5 +1,22 @@
 // Rows in the order of their experts times each expert's weights, and the
-// gradients of both.
+// gradients of both: y[r] = x[r] W[e], dx[r] = dy[r] W[e]^T,
+// dW[e] = sum of x[r]^T dy[r] over the expert's rows.
+//
+// A work-group makes a tile of one expert's result with matrix instructions
+// (tiles.h). How many rows an expert has is known on the GPU alone: the launch
+// has work-groups for the most tiles there can be (a partial one for every
+// expert), each finds its own from the offsets, and those past the last end at
+// once. The rows' gradient is the product with the weights' dimensions changed
+// about, so only which dimension is contiguous makes different kernels.
+//
+// Many rows are bound by the matrix cores at the clock that the chip's power
+// leaves them, few rows by the weights' bytes. Measured, bfloat16, 8192^3: 827 us
+// weights by input (1.33 PFLOP/s; the library's dense product 806), 819 by output
+// (716), the weights' gradient 818 (939). 64 experts with 0 to 32,378 of 131,072
+// rows, 1024 x 4096: forwards 1.17 ms, of which about a quarter is writing 1.07
+// GB between the products; backwards 2.1 ms. 128 rows of 64 experts: 46 us, the
+// weights of the experts that have any at HBM's rate. float32 8192^3: 7.6 ms, 0.92
+// of the library's rate.
 #include <algorithm>
 
 #include "tiles.h"
@@ -175,7 +192,7 @@ struct RowsCall {
                         w.expert * kBytes % 16 == 0 &&
                         depth * kBytes % 16 == 0 &&
                         (kB == Along::kDepth || columns * kBytes % 16 == 0);
-    const bool small = rows <= 32ll * experts;
+    const bool small = WorthSmall(rows, columns, experts);
     if (!direct) {
       return small ? Launch<SmallTile<T, Along::kDepth, kB, false>>()
                    : Launch<MiddleTile<T, Along::kDepth, kB, false>>();

@@ -10,6 +10,12 @@
 // after another (zeros behind the last), so both operands of the product are
 // panels along the depth and a step of the product is a block: a scale for each
 // row and one for 128 columns.
+//
+// Measured, bfloat16 rows, 64 experts with 131,072 rows, 1024 x 4096: 830 us, 86
+// of them the rows' quantisation (HBM, 4.7 TB/s) and the rest the product, whose
+// eight steps a tile take about as long as writing its result (1.07 GB in all);
+// 32 rows: 16 us, the weights at HBM's rate after 5 us of a first launch; 20,011
+// rows, 3328 x 1000 float16 113 us, 36 of them the quantisation.
 #include <algorithm>
 #include <type_traits>
 
@@ -291,7 +297,7 @@ struct Call8 {
     constexpr Along kDepth = Along::kDepth;
     // float32 results are those of float32 sums.
     using E = std::conditional_t<sizeof(Out) == 4, E4m3Wide, E4m3>;
-    if (rows <= 32ll * experts) {
+    if (WorthSmall(rows, columns, experts)) {
       return Launch<SmallTile<E, kDepth, kDepth, true>>();
     }
     if (rows >= 256ll * experts && WorthLarge(rows, columns)) {

@@ -824,6 +824,15 @@ using LargeTile = Tile<T, kA, kB, 256, 256, 2, 4, true>;
 
 constexpr int kCus = 256;
 
+// Whether small tiles are worth it: rows of an expert are few, or middle ones
+// would leave a quarter of the CUs without work (float32, 1000 rows of 4 experts,
+// 2048 x 256, 16 tiles: 141 us, 53 with small ones; bfloat16, 2000 rows, 1024 x
+// 1024, 128 tiles: 16 and 11; 3900 rows, 248 tiles: 16 and 18).
+inline bool WorthSmall(int64_t rows, int64_t columns, int64_t experts) {
+  return rows <= 32 * experts ||
+         4 * CeilDiv(rows, 128) * CeilDiv(columns, 128) < 3 * kCus;
+}
+
 // Whether large tiles, one at a time on a CU, are worth it: they are a fifth
 // faster where the last round of them is full enough (64 experts, 131,072 rows,
 // 1024 x 4096: bfloat16 1173 us, with middle ones 1417; 8 bits 839 and 1026; but
