@@ -1,5 +1,5 @@
 // Device helpers of the dense operators (layer_norm.hip, experts.hip,
-// adamw.hip): element types, vectors of them, and sums over lanes.
+// adamw.hip, expert_matmul.hip, matmul_8bit.hip, gradient_norm.hip): element types, vectors of them, and sums over lanes.
 #pragma once
 
 #include "../../include/scemb.h"

@@ -1,7 +1,7 @@
 """The dense operators of a ranking model that trains beside its tables.
 
 No counterpart in the reference, whose users take these from their framework's
-compiler. Three families, each a hand-written gfx950 kernel behind the C ABI:
+compiler. Families of hand-written gfx950 kernels behind the C ABI:
 
   layer_norm, layer_norm_grad
       layer norm of the activations that the lookups return, and its
@@ -9,14 +9,22 @@ compiler. Three families, each a hand-written gfx950 kernel behind the C ABI:
   sort_by_expert, tokens_to_experts, tokens_from_experts (and their _grad)
       a mixture of experts' tokens in the order of their experts and back,
       with the router's weights applied;
+  expert_matmul, expert_matmul_grad
+      the experts' layers between the two: products grouped by expert, whose
+      numbers of rows stay on the GPU, and their gradients;
+  quantize_weights, matmul_8bit
+      the same products, or one plain product, in 8-bit floating point with a
+      scale for each block of 128, for serving;
+  gradient_norm, clip_gradients
+      the global norm of all gradients, and gradients clipped to it;
   init_adamw_state, adamw_update, adamw_moments
       AdamW over all dense weights in one or a few launches, with moments in
       float32 or in 8 bits.
 
 Arrays are torch tensors on the current GPU, work is enqueued on the current
 stream and nothing waits for it; arguments that do not fit raise ValueError.
-layer_norm, tokens_to_experts and tokens_from_experts take part in torch's
-autograd; the _grad functions are the same gradients for callers that keep
+layer_norm, tokens_to_experts, expert_matmul and tokens_from_experts take part in
+torch's autograd; the _grad functions are the same gradients for callers that keep
 their own tape, as embedding.tpu_sparse_dense_matmul_grad's are. Nothing here
 has forward-mode derivatives: tensors that carry a tangent are refused.
 """
