@@ -80,7 +80,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   if (piece != 0) {
     const RowTile t = FindRowTile(offsets, experts, rows, part, piece);
     if (t.segment < 0 || t.segment == experts) return;
-    s = {t.row, min(t.end, t.row + piece)};
+    s = {t.row, t.end - t.row > piece ? t.row + piece : t.end};
   } else {
     // The longest sums first: one that begins last is all that runs then (64
     // experts, the largest with a quarter of all rows: 1345 us in their order,
@@ -102,17 +102,19 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
           outer, m, n, lds0);
 }
 
-// out[e] = the sum of the pieces of segment e, in their order.
+// out[e] = the sum of the pieces of segment e, in their order; there are `most`
+// of all, whatever the offsets hold.
 constexpr int kJoinBlock = 256;
 template <typename T>
 __global__ __launch_bounds__(kJoinBlock) void JoinPieces(
     const float* pieces, int64_t size, const int32_t* offsets, int32_t experts,
-    int32_t rows, int32_t piece, T* out) {
+    int32_t rows, int32_t piece, int32_t most, T* out) {
   constexpr int V = 4;
   const int32_t e = blockIdx.y;
-  const int32_t n =
-      TilesOf(SegmentOf(offsets, experts, rows, e), piece);
-  const int64_t first = TilesBefore(offsets, experts, rows, e, piece);
+  const int64_t first =
+      min(max(TilesBefore(offsets, experts, rows, e, piece), 0), most);
+  const int32_t n = min(TilesOf(SegmentOf(offsets, experts, rows, e), piece),
+                        most - static_cast<int32_t>(first));
   const float* from = pieces + first * size;
   T* to = out + e * size;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kJoinBlock +
@@ -294,7 +296,7 @@ struct WeightsCall {
                     static_cast<uint32_t>(experts));
     hipLaunchKernelGGL(JoinPieces<T>, grid, dim3(kJoinBlock), 0, stream, parts,
                        size, offsets, experts, static_cast<int32_t>(rows),
-                       plan.piece, dw);
+                       plan.piece, static_cast<int32_t>(plan.pieces), dw);
     SCEMB_LAUNCH_CHECK();
     return 0;
   }

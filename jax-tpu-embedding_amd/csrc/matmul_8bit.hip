@@ -312,13 +312,18 @@ int RunRows(const void* x, int64_t stride, int64_t rows, int64_t dim,
             const int32_t* kept, uint8_t* codes, int32_t* exponents,
             hipStream_t stream) {
   const int64_t padded = PaddedOf(dim);
-  const dim3 grid(static_cast<uint32_t>(CeilDiv(rows, kRowBlocks)),
-                  static_cast<uint32_t>(
-                      std::min<int64_t>(padded / kBlock, 65535)));
-  if (static_cast<int64_t>(grid.x) * grid.y > MostGroups(kRowThreads)) {
+  // Work-groups of 16 rows, and as many columns of blocks at once as a launch
+  // takes.
+  const int64_t down = CeilDiv(rows, kRowBlocks);
+  const int64_t across = std::min<int64_t>(padded / kBlock, 65535);
+  if (down > MostGroups(kRowThreads)) {
     return Fail(SCEMB_ERR_INVALID_ARGUMENT,
-                "8-bit product: more blocks than a launch takes");
+                "8-bit product: more rows than a launch takes");
   }
+  const dim3 grid(
+      static_cast<uint32_t>(down),
+      static_cast<uint32_t>(std::max<int64_t>(
+          std::min(across, MostGroups(kRowThreads) / down), 1)));
   hipLaunchKernelGGL(QuantizeRows<T>, grid, dim3(kRowThreads), 0, stream,
                      static_cast<const T*>(x), stride,
                      static_cast<int32_t>(rows), static_cast<int32_t>(dim),

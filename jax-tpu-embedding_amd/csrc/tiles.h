@@ -355,8 +355,11 @@ struct RowTile {
   int32_t row;
   int32_t end;
 };
+// Tiles of `rows` rows; the sum may pass 31 bits.
 __device__ __forceinline__ int32_t TilesOf(const Segment& s, int32_t rows) {
-  return (s.end - s.begin + rows - 1) / rows;
+  const uint32_t n = static_cast<uint32_t>(s.end - s.begin);
+  return static_cast<int32_t>((n + static_cast<uint32_t>(rows) - 1) /
+                              static_cast<uint32_t>(rows));
 }
 __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
                                                int32_t experts, int32_t n,

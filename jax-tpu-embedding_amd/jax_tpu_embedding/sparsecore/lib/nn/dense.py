@@ -284,7 +284,8 @@ def expert_matmul(rows, weights, order: ExpertOrder):
     for the experts' numbers of rows.
 
   Sums are float32, rounded once. float32 products are exact to float32's own
-  rounding (no shortened operands).
+  rounding (no shortened operands). Calls of more than about 2^24 tiles (of 32 x
+  128 values of the result, or larger ones) are refused.
   """
   calls = _calls()
   if calls.wants_grad(rows, weights):
@@ -331,7 +332,7 @@ def quantize_weights(weights) -> Weights8:
   at least) with no magnitude of the block above 448 times it; values are
   rounded to the nearest code, which is 2^-4 of the value off at most (2^-10 of
   the scale where that is more). A block that holds an infinity or a NaN is NaN
-  throughout.
+  throughout. Autograd does not follow the codes.
   """
   inner = weights.shape[-2] if getattr(weights, "ndim", 0) >= 2 else 0
   return Weights8(*_calls().quantize_weights(weights), inner)
@@ -349,8 +350,10 @@ def matmul_8bit(rows, weights: Weights8, order: ExpertOrder | None = None):
     tokens_to_experts returns them; rows of dropped choices are not read and
     give zeros.
 
-  Products of codes are summed in float32 and rounded once. A row that holds an
-  infinity or a NaN gives a row of NaN.
+  Products of codes are summed in float32 and rounded once; for results of 16
+  bits the instructions cut products 13 bits below the largest of eight. A row
+  that holds an infinity or a NaN gives a row of NaN. The limit on tiles is
+  expert_matmul's.
   """
   calls = _calls()
   if calls.wants_grad(rows):

@@ -333,6 +333,22 @@ def test_offsets_that_do_not_fit_reach_no_memory():
   assert torch.equal(y, dense.expert_matmul(x, w, _order([0, 20, 40, 50])))
 
 
+def test_offsets_that_do_not_fit_in_pieces():
+  """The weights' gradient in pieces: segments that overlap have more pieces
+  than there are places for."""
+  n, experts = 20_000, 9
+  x, dy = _values((n, 16), torch.float32, 1, True), _values(
+      (n, 8), torch.float32, 2, True)
+  w = _values((experts, 16, 8), torch.float32, 3, True)
+  good = _order([i * n // experts for i in range(experts + 1)])
+  expected = dense.expert_matmul_grad(dy, x, w, good)
+  for offsets in ([0, n] * 5, [n, 0] * 5, [-5] * 9 + [2**31 - 1]):
+    dx, dw = dense.expert_matmul_grad(dy, x, w, _order(offsets))
+    assert dx.shape == x.shape and dw.shape == w.shape
+  for a, b in zip(dense.expert_matmul_grad(dy, x, w, good), expected):
+    assert torch.equal(a, b)
+
+
 def test_refusals():
   x = torch.zeros((6, 8), device="cuda")
   w = torch.zeros((2, 8, 4), device="cuda")
