@@ -387,6 +387,8 @@ __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
     const Segment s = SegmentOf(offsets, experts, n, i);
     const int32_t tiles = TilesOf(s, tile_rows);
     if (at < tiles || i == experts) {
+      // Counts of segments that overlap may wrap: no tile then.
+      if (at < 0 || at >= tiles) return {-1, 0, 0};
       return {__builtin_amdgcn_readfirstlane(i),
               __builtin_amdgcn_readfirstlane(s.begin + at * tile_rows),
               __builtin_amdgcn_readfirstlane(s.end)};
