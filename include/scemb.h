@@ -718,12 +718,17 @@ int scemb_tokens_from_experts_grad(
  * is at e * expert_stride + i * inner_stride + o * outer_stride, one of the last
  * two being 1; y is [num_rows, outer] contiguous. With inner and outer changed
  * about it is the gradient of the rows. Offsets do not fall; others reach no
- * memory past the rows, but what is written is undefined. */
+ * memory past the rows, but what is written is undefined. The workspace size is 0
+ * where none is needed (and for what the call refuses). */
+size_t scemb_expert_matmul_workspace_size(int32_t type, int64_t num_rows,
+                                          int64_t inner, int64_t outer,
+                                          int32_t num_experts);
 int scemb_expert_matmul(const void* rows, int32_t type, int64_t rows_stride,
                         int64_t num_rows, int64_t inner, int64_t outer,
                         const void* weights, int64_t expert_stride,
                         int64_t inner_stride, int64_t outer_stride,
                         const int32_t* offsets, int32_t num_experts, void* y,
+                        void* workspace, size_t workspace_bytes,
                         void* stream);
 
 /* The weights' gradient, [num_experts, inner, outer] contiguous: the sum over

@@ -41,6 +41,7 @@ struct Library {
   decltype(&scemb_tokens_to_experts) tokens_to_experts;
   decltype(&scemb_tokens_from_experts) tokens_from_experts;
   decltype(&scemb_tokens_from_experts_grad) tokens_from_experts_grad;
+  decltype(&scemb_expert_matmul_workspace_size) expert_matmul_workspace;
   decltype(&scemb_expert_matmul) expert_matmul;
   decltype(&scemb_expert_matmul_weights_grad_workspace_size)
       expert_matmul_weights_grad_workspace;
@@ -637,23 +638,36 @@ void CheckInner(const ExpertWeights& w, const Tensor& rows) {
   }
 }
 
-// expert_matmul(rows, weights, offsets) -> y
+// rows * weights, or with `turned` rows * the weights' transpose.
+Tensor Product(const Rows& r, const ExpertWeights& w, bool turned,
+               const Tensor& offsets, PyObject* workspace, int dev) {
+  const int64_t inner = turned ? w.outer : w.inner;
+  const int64_t outer = turned ? w.inner : w.outer;
+  const int32_t code = Code(r.t.scalar_type());
+  const int32_t experts = static_cast<int32_t>(w.experts);
+  const Tensor y = New({r.n, outer}, r.t.scalar_type(), r.t);
+  const size_t bytes =
+      lib.expert_matmul_workspace(code, r.n, inner, outer, experts);
+  const Tensor ws = bytes > 0 ? Workspace(workspace, bytes) : Tensor();
+  Check(lib.expert_matmul(
+      r.t.data_ptr(), code, r.stride, r.n, inner, outer, w.t.data_ptr(),
+      w.stride->expert, turned ? w.stride->outer : w.stride->inner,
+      turned ? w.stride->inner : w.stride->outer,
+      static_cast<const int32_t*>(offsets.data_ptr()), experts, y.data_ptr(),
+      Data(ws), bytes, Stream(dev)));
+  return y;
+}
+
+// expert_matmul(rows, weights, offsets, workspace) -> y
 PyObject* ExpertMatmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject* {
-    if (n != 3) Refuse("expert_matmul takes 3 arguments");
+    if (n != 4) Refuse("expert_matmul takes 4 arguments");
     const int dev = CurrentDevice();
     const Tensor x = ExpertRows(a[0], dev);
     const Tensor offsets = OffsetsArg(a[2], dev);
     const ExpertWeights w(a[1], offsets, x, dev);
     CheckInner(w, x);
-    const Rows r = RowsOf(x, w.inner);
-    const Tensor y = New({r.n, w.outer}, x.scalar_type(), x);
-    Check(lib.expert_matmul(
-        r.t.data_ptr(), Code(x.scalar_type()), r.stride, r.n, w.inner, w.outer,
-        w.t.data_ptr(), w.stride->expert, w.stride->inner, w.stride->outer,
-        static_cast<const int32_t*>(offsets.data_ptr()),
-        static_cast<int32_t>(w.experts), y.data_ptr(), Stream(dev)));
-    return Wrap(y);
+    return Wrap(Product(RowsOf(x, w.inner), w, false, offsets, a[3], dev));
   });
 }
 
@@ -673,13 +687,7 @@ PyObject* ExpertMatmulGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t code = Code(x.scalar_type());
     const int32_t experts = static_cast<int32_t>(w.experts);
     Tensor drows, dw;
-    if (a[4] == Py_True) {
-      drows = New({g.n, w.inner}, x.scalar_type(), x);
-      Check(lib.expert_matmul(g.t.data_ptr(), code, g.stride, g.n, w.outer,
-                              w.inner, w.t.data_ptr(), w.stride->expert,
-                              w.stride->outer, w.stride->inner, first, experts,
-                              drows.data_ptr(), Stream(dev)));
-    }
+    if (a[4] == Py_True) drows = Product(g, w, true, offsets, a[6], dev);
     if (a[5] == Py_True) {
       const Rows r = RowsOf(x, w.inner);
       // The transposed gradient is that of the operands changed about.

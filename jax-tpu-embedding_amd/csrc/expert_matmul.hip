@@ -34,12 +34,14 @@ struct Weights {
   int64_t stride;  // of the dimension that is not contiguous
 };
 
-// y[r] = x[r] * W[expert of r] for rows in segments; zeros for rows of none.
-template <typename C>
+// y[r] = x[r] * W[expert of r] for rows in segments; zeros for rows of none. With
+// more than one split, the sums over that part of the depth, [splits, rows,
+// columns].
+template <typename C, typename Out>
 __global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
     const typename C::T* x, int64_t x_stride, int32_t rows, int32_t depth,
     Weights w, int32_t columns, const int32_t* offsets, int32_t experts,
-    typename C::T* y, TileGrid grid) {
+    Out* y, int32_t splits, TileGrid grid) {
   using T = typename C::T;
   __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
   __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
@@ -47,17 +49,61 @@ __global__ __launch_bounds__(C::kThreads, 2) void RowsKernel(
   if (!grid.Tile(blockIdx.x, &tile, &column)) return;
   const RowTile t = FindRowTile(offsets, experts, rows, tile, C::kM);
   if (t.segment < 0) return;
+  int32_t begin = 0, count = depth;
+  if (splits > 1) {
+    const int32_t across = grid.columns / splits;
+    const int32_t split = column / across;
+    column -= split * across;
+    const int32_t steps = (depth + C::kDepth - 1) / C::kDepth;
+    const int32_t each = (steps + splits - 1) / splits * C::kDepth;
+    begin = min(split * each, depth);
+    count = min(each, depth - begin);
+    y += static_cast<int64_t>(split) * rows * columns;
+  }
   column *= C::kN;
   const int m = min(t.end - t.row, C::kM);
   const int n = min(columns - column, C::kN);
   C c;
   const T* b = static_cast<const T*>(w.data) + t.segment * w.expert +
-               (C::kAlongB == Along::kDepth ? column * w.stride : column);
-  c.Run(x + t.row * x_stride, x_stride, m, depth, b, w.stride, n,
+               (C::kAlongB == Along::kDepth ? column * w.stride + begin
+                                            : column + begin * w.stride);
+  c.Run(x + t.row * x_stride + begin, x_stride, m, depth, b, w.stride, n,
         C::kAlongB == Along::kDepth ? depth : columns,
-        t.segment < experts ? depth : 0, lds0, lds1, NoScales{});
+        t.segment < experts ? count : 0, lds0, lds1, NoScales{});
   c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n,
           lds0);
+}
+
+// y[i] = the sum over the splits of parts[split][i], in their order.
+constexpr int kJoinBlock = 256;
+template <typename T>
+__global__ __launch_bounds__(kJoinBlock) void JoinSplits(const float* parts,
+                                                         int64_t size,
+                                                         int32_t splits, T* y) {
+  constexpr int V = 4;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kJoinBlock +
+                    threadIdx.x) * V;
+       i < size; i += static_cast<int64_t>(gridDim.x) * kJoinBlock * V) {
+    if (i + V <= size) {
+      float sum[V] = {};
+#pragma unroll 4
+      for (int p = 0; p < splits; ++p) {
+        const auto x = LoadVec<float, V>(parts + p * size + i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += x.v[j];
+      }
+      Vec<T, V> v;
+#pragma unroll
+      for (int j = 0; j < V; ++j) v.v[j] = static_cast<T>(sum[j]);
+      StoreVec<T, V>(y + i, v);
+    } else {
+      for (int64_t j = i; j < size; ++j) {
+        float sum = 0.f;
+        for (int p = 0; p < splits; ++p) sum += parts[p * size + j];
+        y[j] = static_cast<T>(sum);
+      }
+    }
+  }
 }
 
 // dw[e] = the sum over the segment's rows of x[r]^T dy[r]; with `piece` not 0
@@ -67,7 +113,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
     const typename C::T* x, int64_t x_stride, int32_t inner,
     const typename C::T* dy, int64_t dy_stride, int32_t outer, int32_t rows,
     const int32_t* offsets, int32_t experts, Out* dw, int32_t piece,
-    TileGrid grid) {
+    bool ranked, TileGrid grid) {
   __shared__ __attribute__((aligned(16))) char lds0[C::kLds];
   __shared__ __attribute__((aligned(16))) char lds1[C::kLds];
   int32_t tile, column;
@@ -84,10 +130,9 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   } else {
     // The longest sums first: one that begins last is all that runs then (64
     // experts, the largest with a quarter of all rows: 1345 us in their order,
-    // 1081 this way).
-    if (experts <= kMostRanked) {
-      part = ExpertOfRank(offsets, experts, rows, part);
-    }
+    // 1081 this way). Finding which costs a few microseconds, which short sums
+    // are not worth.
+    if (ranked) part = ExpertOfRank(offsets, experts, rows, part);
     s = SegmentOf(offsets, experts, rows, part);
     s = {__builtin_amdgcn_readfirstlane(s.begin),
          __builtin_amdgcn_readfirstlane(s.end)};
@@ -104,7 +149,6 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
 
 // out[e] = the sum of the pieces of segment e, in their order; there are `most`
 // of all, whatever the offsets hold.
-constexpr int kJoinBlock = 256;
 template <typename T>
 __global__ __launch_bounds__(kJoinBlock) void JoinPieces(
     const float* pieces, int64_t size, const int32_t* offsets, int32_t experts,
@@ -159,6 +203,22 @@ int TooMany() {
               "expert matmul: more tiles than a launch takes");
 }
 
+// Into how many parts of the depth the product is cut: where small tiles, of
+// which every expert that has rows has one at least, leave CUs without work and
+// the sums are long enough to pay for a second launch.
+int32_t SplitsOf(int bytes, int64_t rows, int64_t depth, int64_t columns,
+                 int64_t experts) {
+  const int64_t tiles = std::max(CeilDiv(rows, 32), std::min(rows, experts)) *
+                        CeilDiv(columns, 128);
+  const int64_t steps = CeilDiv(depth * bytes, 128);
+  if (tiles == 0 || tiles >= kCus || steps < 16 ||
+      !WorthSmall(rows, columns, experts)) {
+    return 1;
+  }
+  return static_cast<int32_t>(std::max<int64_t>(
+      std::min({CeilDiv(2 * kCus, tiles), steps / 4, int64_t{16}}), 1));
+}
+
 template <typename T>
 struct RowsCall {
   const T* x;
@@ -170,17 +230,35 @@ struct RowsCall {
   const int32_t* offsets;
   int32_t experts;
   T* y;
+  float* parts;
+  int32_t splits;
   hipStream_t stream;
 
-  template <typename C>
-  int Launch() const {
-    const TileGrid grid(rows / C::kM + experts + 1, CeilDiv(columns, C::kN));
+  template <typename C, typename Out>
+  int Launch(Out* out) const {
+    const TileGrid grid(rows / C::kM + experts + 1,
+                        CeilDiv(columns, C::kN) * splits);
     if (grid.Groups() > MostGroups(C::kThreads)) return TooMany();
-    hipLaunchKernelGGL(RowsKernel<C>, dim3(grid.Groups()), dim3(C::kThreads),
-                       0, stream, x, x_stride, static_cast<int32_t>(rows),
-                       static_cast<int32_t>(depth), w,
-                       static_cast<int32_t>(columns), offsets, experts, y,
-                       grid);
+    hipLaunchKernelGGL((RowsKernel<C, Out>), dim3(grid.Groups()),
+                       dim3(C::kThreads), 0, stream, x, x_stride,
+                       static_cast<int32_t>(rows), static_cast<int32_t>(depth),
+                       w, static_cast<int32_t>(columns), offsets, experts, out,
+                       splits, grid);
+    SCEMB_LAUNCH_CHECK();
+    return 0;
+  }
+
+  template <typename C>
+  int LaunchSmall() const {
+    if (splits == 1) return Launch<C>(y);
+    const int rc = Launch<C>(parts);
+    if (rc != 0) return rc;
+    const int64_t size = rows * columns;
+    hipLaunchKernelGGL(
+        JoinSplits<T>,
+        dim3(static_cast<uint32_t>(std::min(CeilDiv(size, 4 * kJoinBlock),
+                                            MostGroups(kJoinBlock)))),
+        dim3(kJoinBlock), 0, stream, parts, size, splits, y);
     SCEMB_LAUNCH_CHECK();
     return 0;
   }
@@ -189,23 +267,23 @@ struct RowsCall {
   template <Along kB>
   int Run() const {
     constexpr int kBytes = sizeof(T);
+    constexpr Along kDepth = Along::kDepth;
     const bool direct = Loadable(x, x_stride, kBytes) &&
                         Loadable(w.data, w.stride, kBytes) &&
                         w.expert * kBytes % 16 == 0 &&
                         depth * kBytes % 16 == 0 &&
-                        (kB == Along::kDepth || columns * kBytes % 16 == 0);
-    const bool small = WorthSmall(rows, columns, experts);
-    if (!direct) {
-      return small ? Launch<SmallTile<T, Along::kDepth, kB, false>>()
-                   : Launch<MiddleTile<T, Along::kDepth, kB, false>>();
+                        (kB == kDepth || columns * kBytes % 16 == 0);
+    if (WorthSmall(rows, columns, experts)) {
+      return direct ? LaunchSmall<SmallTile<T, kDepth, kB, true>>()
+                    : LaunchSmall<SmallTile<T, kDepth, kB, false>>();
     }
-    if (small) return Launch<SmallTile<T, Along::kDepth, kB, true>>();
+    if (!direct) return Launch<MiddleTile<T, kDepth, kB, false>>(y);
     if constexpr (kBytes == 2) {
       if (rows >= 256ll * experts && WorthLarge(rows, columns)) {
-        return Launch<LargeTile<T, Along::kDepth, kB>>();
+        return Launch<LargeTile<T, kDepth, kB>>(y);
       }
     }
-    return Launch<MiddleTile<T, Along::kDepth, kB, true>>();
+    return Launch<MiddleTile<T, kDepth, kB, true>>(y);
   }
 };
 
@@ -267,7 +345,8 @@ struct WeightsCall {
                        dim3(C::kThreads), 0, stream, x, x_stride,
                        static_cast<int32_t>(inner), dy, dy_stride,
                        static_cast<int32_t>(outer), static_cast<int32_t>(rows),
-                       offsets, experts, out, plan.piece, grid);
+                       offsets, experts, out, plan.piece,
+                       experts <= kMostRanked && rows >= 256ll * experts, grid);
     SCEMB_LAUNCH_CHECK();
     return 0;
   }
@@ -322,11 +401,22 @@ int CheckSizes(int32_t type, int64_t rows, int64_t inner, int64_t outer,
 
 extern "C" {
 
+size_t scemb_expert_matmul_workspace_size(int32_t type, int64_t num_rows,
+                                          int64_t inner, int64_t outer,
+                                          int32_t num_experts) {
+  using namespace scemb;
+  if (CheckSizes(type, num_rows, inner, outer, num_experts) != 0) return 0;
+  const int32_t splits =
+      SplitsOf(TypeBytes(type), num_rows, inner, outer, num_experts);
+  return splits == 1 ? 0 : static_cast<size_t>(splits) * num_rows * outer * 4;
+}
+
 int scemb_expert_matmul(const void* rows, int32_t type, int64_t rows_stride,
                         int64_t num_rows, int64_t inner, int64_t outer,
                         const void* weights, int64_t expert_stride,
                         int64_t inner_stride, int64_t outer_stride,
                         const int32_t* offsets, int32_t num_experts, void* y,
+                        void* workspace, size_t workspace_bytes,
                         void* stream) {
   using namespace scemb;
   const int bad = CheckSizes(type, num_rows, inner, outer, num_experts);
@@ -340,6 +430,11 @@ int scemb_expert_matmul(const void* rows, int32_t type, int64_t rows_stride,
                 "expert matmul: an operand is missing, a negative stride, or "
                 "weights that are contiguous in neither inner nor outer");
   }
+  const size_t need = scemb_expert_matmul_workspace_size(
+      type, num_rows, inner, outer, num_experts);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    return Fail(SCEMB_ERR_WORKSPACE, "expert matmul: workspace too small");
+  }
   const auto run = [&](auto zero) {
     using T = decltype(zero);
     const bool along_outer = outer_stride == 1;
@@ -347,6 +442,8 @@ int scemb_expert_matmul(const void* rows, int32_t type, int64_t rows_stride,
         static_cast<const T*>(rows), rows_stride, num_rows, inner,
         {weights, expert_stride, along_outer ? inner_stride : outer_stride},
         outer, offsets, num_experts, static_cast<T*>(y),
+        static_cast<float*>(workspace),
+        SplitsOf(sizeof(T), num_rows, inner, outer, num_experts),
         static_cast<hipStream_t>(stream)};
     return along_outer ? call.template Run<Along::kOuter>()
                        : call.template Run<Along::kDepth>();

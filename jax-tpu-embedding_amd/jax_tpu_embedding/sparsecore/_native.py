@@ -88,6 +88,7 @@ EXPORTED_SYMBOLS = (
     "scemb_tokens_to_experts",
     "scemb_tokens_from_experts",
     "scemb_tokens_from_experts_grad",
+    "scemb_expert_matmul_workspace_size",
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",
@@ -434,6 +435,7 @@ _DENSE_FUNCTIONS = (
     "scemb_tokens_to_experts",
     "scemb_tokens_from_experts",
     "scemb_tokens_from_experts_grad",
+    "scemb_expert_matmul_workspace_size",
     "scemb_expert_matmul",
     "scemb_expert_matmul_weights_grad_workspace_size",
     "scemb_expert_matmul_weights_grad",

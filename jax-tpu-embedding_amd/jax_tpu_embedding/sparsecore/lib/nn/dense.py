@@ -124,7 +124,7 @@ def _function(name: str):
       @staticmethod
       def forward(ctx, rows, weights, offsets):
         ctx.save_for_backward(rows, weights, offsets)
-        return _calls().expert_matmul(rows, weights, offsets)
+        return _calls().expert_matmul(rows, weights, offsets, _workspace)
 
       @staticmethod
       @once
@@ -290,7 +290,7 @@ def expert_matmul(rows, weights, order: ExpertOrder):
   calls = _calls()
   if calls.wants_grad(rows, weights):
     return _function("product").apply(rows, weights, order.offsets)
-  return calls.expert_matmul(rows, weights, order.offsets)
+  return calls.expert_matmul(rows, weights, order.offsets, _workspace)
 
 
 def expert_matmul_grad(y_grad, rows, weights, order: ExpertOrder, *,

@@ -38,10 +38,10 @@ SIZES = [dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=2**31 - 1),
 
 
 def _product(x=SOME, type=F32, stride=8, rows=4, inner=8, outer=6, w=SOME,  # pylint: disable=redefined-builtin
-             se=48, si=6, so=1, offsets=SOME, experts=2, y=SOME):
+             se=48, si=6, so=1, offsets=SOME, experts=2, y=SOME, ws=0, size=0):
   return _call("scemb_expert_matmul", VP(x), I32(type), I64(stride), I64(rows),
                I64(inner), I64(outer), VP(w), I64(se), I64(si), I64(so),
-               VP(offsets), I32(experts), VP(y), VP(0))
+               VP(offsets), I32(experts), VP(y), VP(ws), SZ(size), VP(0))
 
 
 @pytest.mark.parametrize("bad", SIZES + [
@@ -51,6 +51,22 @@ def test_expert_matmul(bad):
   assert _product(**bad) == INVALID
   assert _native.load_library().scemb_last_error()
   assert _product(rows=0, x=0, y=0) == OK
+
+
+def test_expert_matmul_workspace():
+  name = "scemb_expert_matmul_workspace_size"
+  size = lambda rows, inner, outer, experts: _size(
+      name, I32(F32), I64(rows), I64(inner), I64(outer), I32(experts))
+  # A few rows and a long sum are cut along it: the parts' sums.
+  need = size(100, 4096, 64, 1)
+  assert need > 0 and need % (100 * 64 * 4) == 0
+  for args in ((100, 64, 64, 1), (100_000, 4096, 4096, 1), (0, 4096, 64, 1),
+               (100, 0, 64, 1), (128, 4096, 4096, 64)):
+    assert size(*args) == 0
+  long = dict(rows=100, inner=4096, stride=4096, outer=64, si=64, se=4096 * 64,
+              experts=1)
+  assert _product(**long) == WORKSPACE
+  assert _product(**long, ws=SOME, size=need - 1) == WORKSPACE
 
 
 def _weights_grad(x=SOME, dy=SOME, type=F32, rows=100_000, inner=8, outer=6,  # pylint: disable=redefined-builtin

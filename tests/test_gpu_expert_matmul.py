@@ -149,6 +149,24 @@ def test_many_rows(stored, dtype):
   _run(x, w, dy, offsets, True)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("stored", ["in_out", "out_in"])
+@pytest.mark.parametrize("inner,outer", [(4096, 40), (1100, 128), (2051, 130),
+                                         (1999, 3), (1024, 256)])
+def test_long_sums_of_few_rows(inner, outer, stored, dtype):
+  """Cut along the sum, forwards and, with inner and outer changed about,
+  backwards; some parts are shorter or have nothing."""
+  offsets, n = _offsets([40, 0, 3, 61], 6)
+  x = _values((n, inner), dtype, 1, True)
+  w = _values((4, inner, outer), dtype, 2, True)
+  if stored == "out_in":
+    w = w.transpose(1, 2).contiguous().transpose(1, 2)
+  dy = _values((n, outer), dtype, 3, True)
+  # float16 ends at 65504: sums of 4096 products of 9 stay below.
+  _run(x, w, dy, offsets, True)
+  _run(dy, w.transpose(1, 2), x, offsets, True)
+
+
 def _strided(x, how):
   """The same values in other memory."""
   if how == "padded_rows":
