@@ -205,7 +205,8 @@ int TooMany() {
 
 // Into how many parts of the depth the product is cut: where small tiles, of
 // which every expert that has rows has one at least, leave CUs without work and
-// the sums are long enough to pay for a second launch.
+// the sums are long enough to pay for a second launch (float32, 512 rows, 4096 x
+// 128: 17 us, uncut 93; bfloat16, 1000 rows of 4 experts, 2048 x 256: 14 and 18).
 int32_t SplitsOf(int bytes, int64_t rows, int64_t depth, int64_t columns,
                  int64_t experts) {
   const int64_t tiles = std::max(CeilDiv(rows, 32), std::min(rows, experts)) *
