@@ -2,22 +2,22 @@
 //
 // A scale is a power of two, 2^e with the least e that leaves no value of the
 // block above 448, the largest code: dividing by it is exact, so a code is the
-// value rounded once, and the matrix instructions multiply by it on their way.
-// They take the exponent as 8 bits, which are kept in 32 so that a lane loads
-// its row's with one instruction. Sums are float32.
+// value rounded once. The products are bfloat16's (E4m3 in tiles.h says why): a
+// code times its power of two is one conversion, two codes an instruction. The
+// exponents are kept in 32 bits so that a lane loads its row's with one
+// instruction. Sums are float32.
 //
 // Codes are laid out by row and by output column, 128 of the sum's index one
 // after another (zeros behind the last), so both operands of the product are
 // panels along the depth and a step of the product is a block: a scale for each
 // row and one for 128 columns.
 //
-// Measured, bfloat16 rows, 64 experts with 131,072 rows, 1024 x 4096: 830 us, 86
-// of them the rows' quantisation (HBM, 4.7 TB/s) and the rest the product, whose
-// eight steps a tile take about as long as writing its result (1.07 GB in all);
-// 32 rows: 16 us, the weights at HBM's rate after 5 us of a first launch; 20,011
-// rows, 3328 x 1000 float16 113 us, 36 of them the quantisation.
+// Measured, bfloat16 rows, 64 experts with 131,072 rows, 1024 x 4096: 1118 us, 86
+// of them the rows' quantisation (HBM, 4.7 TB/s) and the rest the product (1.07
+// PFLOP/s; by the 8-bit instructions, which cut products, 840 in all); 32 rows:
+// 15 us, the weights at HBM's rate after 5 us of a first launch; 20,011 rows, 3328
+// x 1000 float16 154 us, 36 of them the quantisation (115 by the 8-bit ones).
 #include <algorithm>
-#include <type_traits>
 
 #include "tiles.h"
 
@@ -295,15 +295,13 @@ struct Call8 {
 
   int Run() const {
     constexpr Along kDepth = Along::kDepth;
-    // float32 results are those of float32 sums.
-    using E = std::conditional_t<sizeof(Out) == 4, E4m3Wide, E4m3>;
     if (WorthSmall(rows, columns, experts)) {
-      return Launch<SmallTile<E, kDepth, kDepth, true>>();
+      return Launch<SmallTile<E4m3, kDepth, kDepth, true>>();
     }
     if (rows >= 256ll * experts && WorthLarge(rows, columns)) {
-      return Launch<LargeTile<E, kDepth, kDepth>>();
+      return Launch<LargeTile<E4m3, kDepth, kDepth>>();
     }
-    return Launch<MiddleTile<E, kDepth, kDepth, true>>();
+    return Launch<MiddleTile<E4m3, kDepth, kDepth, true>>();
   }
 };
 

@@ -279,35 +279,14 @@ __device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
   }
 }
 
-// 8-bit operands (e4m3), whose values of a block share a power of two.
+// 8-bit operands (e4m3), whose values of a block share a power of two. They are
+// multiplied as bfloat16, whose products are exact and whose sums are float32's:
+// the instructions of 8-bit operands add eight products at a time, each cut off
+// 13 bits below the largest one's power of two, which is as much as a 16-bit
+// result's own rounding where a long sum is small beside its terms.
 struct E4m3 {
   uint8_t bits;
 };
-// The same that are multiplied as bfloat16, which holds them and their scale
-// exactly.
-struct E4m3Wide {
-  uint8_t bits;
-};
-
-// The sum over half a step (32 of each lane's bytes) of operands in 8 bits.
-// scale: exponents, with a bias of 127. The instruction adds eight products at a
-// time, each cut off 13 bits below the largest one's power of two, and adds that
-// to the float32 sum. For 64 products of normal values that is 2.7e-6 of the
-// magnitudes' sum (of any codes 2.9e-5, 3.2e-4 at most): the codes themselves are
-// off by up to 2^-4, half a step of a 16-bit result is 2^-9 or 2^-11 of it. It is
-// far above float32's, whose results take E4m3Wide.
-__device__ __forceinline__ void MultiplyAdd8(const U32x4& b0, const U32x4& b1,
-                                             int32_t b_scale, const U32x4& a0,
-                                             const U32x4& a1, int32_t a_scale,
-                                             F32x16* acc) {
-  using V = int __attribute__((ext_vector_type(8)));
-  const V b = __builtin_bit_cast(
-      V, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
-  const V a = __builtin_bit_cast(
-      V, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-  *acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-      b, a, *acc, /*e4m3*/ 0, /*e4m3*/ 0, 0, b_scale, 0, a_scale);
-}
 
 // 16 codes as bfloat16.
 struct Wide {
@@ -614,7 +593,7 @@ struct Tile {
   template <typename Scales>
   __device__ __forceinline__ void Multiply(const Fragments& f,
                                            const Scales& scales) {
-    if constexpr (__is_same(T, E4m3Wide)) {
+    if constexpr (sizeof(T) == 1) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         Wide b[kFragN];
@@ -630,15 +609,6 @@ struct Tile {
               MultiplyAdd<bf16>(b[j].v[part], a.v[part], &acc[i][j]);
             }
           }
-        }
-      }
-    } else if constexpr (sizeof(T) == 1) {
-#pragma unroll
-      for (int i = 0; i < kFragM; ++i) {
-#pragma unroll
-        for (int j = 0; j < kFragN; ++j) {
-          MultiplyAdd8(f.b[0][j], f.b[1][j], scales.b, f.a[0][i], f.a[1][i],
-                       scales.a[i], &acc[i][j]);
         }
       }
     } else {

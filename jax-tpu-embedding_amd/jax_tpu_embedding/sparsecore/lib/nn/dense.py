@@ -350,9 +350,8 @@ def matmul_8bit(rows, weights: Weights8, order: ExpertOrder | None = None):
     tokens_to_experts returns them; rows of dropped choices are not read and
     give zeros.
 
-  Products of codes are summed in float32 and rounded once; for results of 16
-  bits the instructions cut products 13 bits below the largest of eight. A row
-  that holds an infinity or a NaN gives a row of NaN. The limit on tiles is
+  Products of codes are exact, summed in float32 and rounded once. A row that
+  holds an infinity or a NaN gives a row of NaN. The limit on tiles is
   expert_matmul's.
   """
   calls = _calls()
