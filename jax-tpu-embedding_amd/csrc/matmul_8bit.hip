@@ -95,8 +95,9 @@ __global__ __launch_bounds__(kRowThreads) void QuantizeRows(
     *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(row) * padded + at) =
         uint2{c[0] | c[1] << 16, c[2] | c[3] << 16};
     if (threadIdx.x % 16 == 0) {
+      // Zeros are zeros with any power: one that bfloat16 holds.
       exponents[static_cast<int64_t>(block) * rows + row] =
-          finite ? e + kBias : kBias;
+          finite && top > 0.f ? e + kBias : kBias;
     }
   }
 }
@@ -175,7 +176,10 @@ __global__ __launch_bounds__(kWeightThreads) void QuantizeWeights(
 // The product.
 // ---------------------------------------------------------------------------
 
-// The scales of a wavefront's rows and of its columns, a step ahead.
+// The scales of a wavefront's rows and of its columns, a step ahead. A code times
+// its power of two is past bfloat16 near the ends of float32 (256 * 2^120, 2^-9 *
+// 2^-126): what the columns' power is out of, the rows' make up for; `lost` says
+// that the rows' were out of it themselves, in any lane and step.
 template <int kFragM>
 struct Scales {
   const int32_t* a_from;  // of the tile's first row in the next block
@@ -184,6 +188,7 @@ struct Scales {
   int32_t row[kFragM];
   int32_t a[kFragM];
   int32_t b;
+  bool lost;
   int32_t next_a[kFragM];
   int32_t next_b;
 
@@ -195,11 +200,63 @@ struct Scales {
     ++b_from;
   }
   __device__ __forceinline__ void Take() {
+    b = min(max(next_b, kLeastHeld), kMostHeld);
+    bool held = true;
 #pragma unroll
-    for (int i = 0; i < kFragM; ++i) a[i] = next_a[i];
-    b = next_b;
+    for (int i = 0; i < kFragM; ++i) {
+      a[i] = next_a[i] + next_b - b;
+      held = held && a[i] >= kLeastHeld && a[i] <= kMostHeld;
+    }
+    lost = lost || __builtin_amdgcn_ballot_w64(!held) != 0;
   }
 };
+
+// The tile's results of a wavefront whose scales were lost: the codes' own
+// products, and a block's sum times its powers of two. From memory, 32 rows after
+// another: it is rare, and needs no registers that the other way has use for.
+template <typename C, typename Out>
+__device__ __forceinline__ void StoreUnscaled(
+    const uint8_t* x, const int32_t* x_exponents, int64_t x_step, int m,
+    const uint8_t* w, const int32_t* w_exponents, int n, int32_t padded, Out* y,
+    int64_t columns, char* lds) {
+  using R = RowsOut<Out, C::kFragN>;
+  const int lane = threadIdx.x % kWave;
+  const int part = lane / 32 * 16;
+  lds += __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * R::kBytes;
+#pragma unroll 1
+  for (int i = 0; i < C::kFragM; ++i) {
+    const int row = C::WaveM() + i * 32;
+    if (row >= m) break;
+    const int32_t mine = min(row + lane % 32, m - 1);
+    F32x16 acc[C::kFragN] = {};
+#pragma unroll 1
+    for (int32_t block = 0; block < padded / kBlock; ++block) {
+      const int power = x_exponents[block * x_step + mine] +
+                        w_exponents[block] - 2 * kBias;
+#pragma unroll
+      for (int j = 0; j < C::kFragN; ++j) {
+        const int32_t column = min(C::WaveN() + j * 32 + lane % 32, n - 1);
+        F32x16 sum = {};
+#pragma unroll
+        for (int k = 0; k < kBlock; k += 32) {
+          const int64_t at = block * kBlock + k + part;
+          const Wide a = Widen(*reinterpret_cast<const U32x4*>(
+              x + static_cast<int64_t>(mine) * padded + at), kUnscaled);
+          const Wide b = Widen(*reinterpret_cast<const U32x4*>(
+              w + static_cast<int64_t>(column) * padded + at), kUnscaled);
+          MultiplyAdd<bf16>(b.v[0], a.v[0], &sum);
+          MultiplyAdd<bf16>(b.v[1], a.v[1], &sum);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          acc[j][k] += __builtin_ldexpf(sum[k], power);
+        }
+      }
+    }
+    R::Store(acc, lds, y + row * columns + C::WaveN(), columns, m - row,
+             n - C::WaveN());
+  }
+}
 
 template <typename C, typename Out>
 __global__ __launch_bounds__(C::kThreads, 2) void Product8(
@@ -235,11 +292,21 @@ __global__ __launch_bounds__(C::kThreads, 2) void Product8(
                static_cast<int64_t>(t.row) * padded;
   const E* b = reinterpret_cast<const E*>(w) +
                (static_cast<int64_t>(t.segment) * columns + column) * padded;
+  scales.lost = false;
   c.Run(a, padded, m, padded, b, padded, n, padded,
         t.segment < experts ? padded : 0, lds0,
         lds1, scales);
-  c.Store(y + static_cast<int64_t>(t.row) * columns + column, columns, m, n,
-          lds0);
+  Out* to = y + static_cast<int64_t>(t.row) * columns + column;
+  if (__builtin_expect(scales.lost, 0)) {
+    StoreUnscaled<C>(reinterpret_cast<const uint8_t*>(a),
+                     x_exponents + t.row, rows, m,
+                     reinterpret_cast<const uint8_t*>(b),
+                     w_exponents + (static_cast<int64_t>(t.segment) * across +
+                                    block) * (padded / kBlock),
+                     n, padded, to, columns, lds0);
+  } else {
+    c.Store(to, columns, m, n, lds0);
+  }
 }
 
 // ---------------------------------------------------------------------------

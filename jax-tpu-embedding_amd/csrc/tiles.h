@@ -288,7 +288,7 @@ struct E4m3 {
   uint8_t bits;
 };
 
-// 16 codes as bfloat16.
+// 16 codes times 2^(scale - 127) as bfloat16.
 struct Wide {
   U32x4 v[2];
 };
@@ -306,6 +306,11 @@ __device__ __forceinline__ Wide Widen(const U32x4& codes, int32_t scale) {
   }
   return w;
 }
+// The exponents with which bfloat16 holds every code, 2^-9 to 448, as a normal
+// value; of codes without a power of two.
+constexpr int32_t kUnscaled = 127;
+constexpr int32_t kLeastHeld = kUnscaled - 126 + 9;
+constexpr int32_t kMostHeld = kUnscaled + 119;
 
 // ---------------------------------------------------------------------------
 // Rows in segments: those of expert e are [offsets[e], offsets[e + 1]); the
@@ -645,8 +650,9 @@ struct Tile {
   __device__ __forceinline__ void Run(const T* a, int64_t a_stride, int m,
                                       int32_t a_total, const T* b,
                                       int64_t b_stride, int n,
-                                      int32_t b_total, int32_t depth, char* lds0, char* lds1,
-                                      Scales scales) {
+                                      int32_t b_total, int32_t depth,
+                                      char* lds0, char* lds1,
+                                      Scales&& scales) {
 #pragma unroll
     for (int i = 0; i < kFragM; ++i) {
 #pragma unroll
