@@ -1086,6 +1086,7 @@ struct Gradients {
 
   Gradients(const Sequence& grads, int dev, bool write) {
     list.reserve(grads.n);
+    const bool recorded = at::GradMode::is_enabled();
     for (Py_ssize_t i = 0; i < grads.n; ++i) {
       if (grads[i] == Py_None) continue;
       const bool fits = Fits(grads[i], dev, kRowTypes);
@@ -1100,6 +1101,12 @@ struct Gradients {
         keep.push_back(t._is_zerotensor() ? t.clone()
                        : whole            ? t
                                           : t.contiguous());
+      }
+      // Autograd would take what comes out for constants.
+      if (recorded && THPVariable_Unpack(grads[i]).requires_grad()) {
+        Refuse(At("grads", i) + " takes part in a graph that the norm does not "
+                                "follow: call under torch.no_grad(), or "
+                                "detach it");
       }
       const Tensor& t = fits ? THPVariable_Unpack(grads[i]) : keep.back();
       list.push_back({t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(),

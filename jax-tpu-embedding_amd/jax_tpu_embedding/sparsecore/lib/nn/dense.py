@@ -536,7 +536,9 @@ def gradient_norm(grads, *, max_norm: float | None = None):
   clipped to a global norm without a pass that writes them.
 
   grads: a sequence of float32, bfloat16 or float16 tensors of any shapes and
-    strides, or None (left out). What is given twice counts twice.
+    strides, or None (left out). What is given twice counts twice. No gradients
+    flow through the norm: tensors that autograd would follow (made with
+    create_graph) are refused, unless under torch.no_grad().
   max_norm: not negative.
 
   Squares are summed in 64 bits, in an order that the sizes decide. With an
