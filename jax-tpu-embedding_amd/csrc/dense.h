@@ -1,5 +1,6 @@
 // Device helpers of the dense operators (layer_norm.hip, experts.hip,
-// adamw.hip, expert_matmul.hip, matmul_8bit.hip, gradient_norm.hip): element types, vectors of them, and sums over lanes.
+// adamw.hip, expert_matmul.hip, matmul_8bit.hip, gradient_norm.hip): element
+// types, vectors of them, and sums over lanes.
 #pragma once
 
 #include "../../include/scemb.h"
@@ -118,14 +119,15 @@ __device__ __forceinline__ void StoreSpan(T* row, const Span<kCut, V>& s,
 }
 
 // Calls of layer norm's gradient (rows in registers), of the rows to their
-// experts and back, and of AdamW that move more than the last cache holds (256
-// MB) read past it what they read once (the other kernels were not timed that
-// way): 65,536 x 1024 bfloat16 backwards through layer norm 80 us
-// through the caches, 74 past them, the sum of two rows of 1024 for each of
-// 65,536 tokens 77 and 66; but 16,384 x 1024 24 and 27, and 20,011 tokens 20 and
-// 25. Results are always written through the caches, for whoever reads them
-// next (past them, a product or an activation that follows takes 1 to 8% longer
-// than the write saves).
+// experts and back, of AdamW, and of the gradients' norm and clipping that move
+// more than the last cache holds (256 MB) read past it what they read once (the
+// other kernels were not timed that way): 65,536 x 1024 bfloat16 backwards through
+// layer norm 80 us through the caches, 74 past them, the sum of two rows of 1024
+// for each of 65,536 tokens 77 and 66; but 16,384 x 1024 24 and 27, and 20,011
+// tokens 20 and 25. Results are written through the caches, for whoever reads them next (past
+// them, a product or an activation that follows takes 1 to 8% longer than the
+// write saves), but for gradients that are clipped in place (gradient_norm.hip
+// has its figures).
 constexpr int64_t kCacheBytes = 256 << 20;
 
 inline Cut CutOf(int64_t dim, int v) {

@@ -13,8 +13,9 @@
 // leaves them, few rows by the weights' bytes. Measured, bfloat16, 8192^3: 827 us
 // weights by input (1.33 PFLOP/s; the library's dense product 806), 819 by output
 // (716), the weights' gradient 818 (939). 64 experts with 0 to 32,378 of 131,072
-// rows, 1024 x 4096: forwards 1.17 ms, of which about a quarter is writing 1.07
-// GB between the products; backwards 2.1 ms. 128 rows of 64 experts: 46 us, the
+// rows, 1024 x 4096: forwards 1.18 ms, of which about a quarter is writing 1.07
+// GB between the products (the library's one dense product of these sizes 0.98);
+// backwards 2.1 ms (0.75 and 1.11). 128 rows of 64 experts: 43 to 46 us, the
 // weights of the experts that have any at HBM's rate. float32 8192^3: 7.6 ms, 0.92
 // of the library's rate.
 #include <algorithm>
@@ -130,8 +131,10 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   } else {
     // The longest sums first: one that begins last is all that runs then (64
     // experts, the largest with a quarter of all rows: 1345 us in their order,
-    // 1081 this way). Finding which costs a few microseconds, which short sums
-    // are not worth.
+    // 1081 this way). Finding which costs a work-group a few microseconds: 64
+    // experts of 2048 rows each, 1024 x 4096, take 1097 us and 1028 in their
+    // order, and sums of fewer than 256 rows are not worth it (64 rows each, 512 x
+    // 512: 20 us, in their order 12).
     if (ranked) part = ExpertOfRank(offsets, experts, rows, part);
     s = SegmentOf(offsets, experts, rows, part);
     s = {__builtin_amdgcn_readfirstlane(s.begin),
@@ -289,8 +292,11 @@ struct RowsCall {
 };
 
 // How the weights' gradient is cut: its tiles, and into pieces of how many rows
-// each expert's sum (0: none), so that there are four work-groups for every CU
-// whatever the experts' shares, where tiles are fewer than two for each.
+// each expert's sum (0: none). Where tiles of 128 x 128 are fewer than two for
+// every CU, so that there are four work-groups for each whatever the experts'
+// shares. With more tiles no sum is cut, and a call takes as long as its longest
+// one: 64 experts of 131,072 rows in all, 512 x 512, 96 us with 2048 rows each, 284
+// where one has 12,659.
 struct WeightsPlan {
   bool large;
   int32_t piece;

@@ -12,11 +12,12 @@
 // panels along the depth and a step of the product is a block: a scale for each
 // row and one for 128 columns.
 //
-// Measured, bfloat16 rows, 64 experts with 131,072 rows, 1024 x 4096: 1118 us, 86
-// of them the rows' quantisation (HBM, 4.7 TB/s) and the rest the product (1.07
-// PFLOP/s; by the 8-bit instructions, which cut products, 840 in all); 32 rows:
-// 15 us, the weights at HBM's rate after 5 us of a first launch; 20,011 rows, 3328
-// x 1000 float16 154 us, 36 of them the quantisation (115 by the 8-bit ones).
+// Measured, bfloat16 rows, 64 experts with 131,072 rows, 1024 x 4096: 1130 us, 84
+// of them the rows' quantisation (HBM, 4.8 TB/s) and the rest the product (1.05
+// PFLOP/s; by the 8-bit instructions, which cut products, 840 in all), 3750 where
+// every row's powers are past bfloat16; 32 rows: 16 us, the weights at HBM's rate
+// after 5 us of a first launch; 20,011 rows, 3328 x 1000 float16 155 us, 36 of them
+// the quantisation (115 by the 8-bit ones), 1 to 64 of them 19.
 #include <algorithm>
 
 #include "tiles.h"

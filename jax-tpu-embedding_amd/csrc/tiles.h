@@ -282,8 +282,10 @@ __device__ __forceinline__ void MultiplyAdd(const U32x4& b, const U32x4& a,
 // 8-bit operands (e4m3), whose values of a block share a power of two. They are
 // multiplied as bfloat16, whose products are exact and whose sums are float32's:
 // the instructions of 8-bit operands add eight products at a time, each cut off
-// 13 bits below the largest one's power of two, which is as much as a 16-bit
-// result's own rounding where a long sum is small beside its terms.
+// 13 bits below the largest one's power of two. For codes of any size that is
+// 2.9e-5 of the terms' magnitudes, and the sum of n terms of either sign is about
+// sqrt(n) smaller than those: from 300 terms on more than float16's own rounding,
+// 2^-11 of the result.
 struct E4m3 {
   uint8_t bits;
 };
@@ -814,10 +816,10 @@ inline bool WorthSmall(int64_t rows, int64_t columns, int64_t experts) {
          4 * CeilDiv(rows, 128) * CeilDiv(columns, 128) < 3 * kCus;
 }
 
-// Whether large tiles, one at a time on a CU, are worth it: they are a fifth
+// Whether large tiles, one at a time on a CU, are worth it: they are up to a fifth
 // faster where the last round of them is full enough (64 experts, 131,072 rows,
-// 1024 x 4096: bfloat16 1173 us, with middle ones 1417; 8 bits 839 and 1026; but
-// 20,011 rows, 3328 x 1000, which is 316 tiles, 8 bits 133 and 115).
+// 1024 x 4096: bfloat16 1173 us, with middle ones 1417; 8 bits 1200 and 1283 on one
+// box; but 20,011 rows, 3328 x 1000, which is 316 tiles, 8 bits 194 and 148).
 inline bool WorthLarge(int64_t rows, int64_t columns) {
   const int64_t tiles = CeilDiv(rows, 256) * CeilDiv(columns, 256);
   return 5 * tiles >= 4 * RoundUp(tiles, kCus);
