@@ -126,7 +126,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void WeightsKernel(
   Segment s;
   if (piece != 0) {
     const RowTile t = FindRowTile(offsets, experts, rows, part, piece);
-    if (t.segment < 0 || t.segment == experts) return;
+    if (t.segment < 0 || t.segment >= experts) return;
     s = {t.row, t.end - t.row > piece ? t.row + piece : t.end};
   } else {
     // The longest sums first: one that begins last is all that runs then (64
@@ -240,7 +240,7 @@ struct RowsCall {
 
   template <typename C, typename Out>
   int Launch(Out* out) const {
-    const TileGrid grid(rows / C::kM + experts + 1,
+    const TileGrid grid(rows / C::kM + experts + kNone,
                         CeilDiv(columns, C::kN) * splits);
     if (grid.Groups() > MostGroups(C::kThreads)) return TooMany();
     hipLaunchKernelGGL((RowsKernel<C, Out>), dim3(grid.Groups()),

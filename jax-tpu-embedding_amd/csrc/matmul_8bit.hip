@@ -58,9 +58,13 @@ constexpr int kRowBlocks = kRowThreads / 16;  // of a work-group, in one column
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void QuantizeRows(
     const T* x, int64_t stride, int32_t rows, int32_t dim, int32_t padded,
-    const int32_t* kept, uint8_t* codes, int32_t* exponents) {
+    const int32_t* offsets, int32_t experts, uint8_t* codes,
+    int32_t* exponents) {
   const int32_t row = blockIdx.x * kRowBlocks + threadIdx.x / 16;
-  if (row >= rows || (kept != nullptr && row >= *kept)) return;
+  if (row >= rows) return;
+  if (offsets != nullptr && (row < offsets[0] || row >= offsets[experts])) {
+    return;
+  }
   const T* from = x + row * stride;
   for (int32_t block = blockIdx.y; block < padded / kBlock;
        block += gridDim.y) {
@@ -346,7 +350,8 @@ struct Call8 {
 
   template <typename C>
   int Launch() const {
-    const TileGrid grid(rows / C::kM + experts + 1, CeilDiv(columns, C::kN));
+    const TileGrid grid(rows / C::kM + experts + kNone,
+                        CeilDiv(columns, C::kN));
     if (grid.Groups() > MostGroups(C::kThreads)) {
       return Fail(SCEMB_ERR_INVALID_ARGUMENT,
                   "8-bit product: more tiles than a launch takes");
@@ -375,8 +380,8 @@ struct Call8 {
 
 template <typename T>
 int RunRows(const void* x, int64_t stride, int64_t rows, int64_t dim,
-            const int32_t* kept, uint8_t* codes, int32_t* exponents,
-            hipStream_t stream) {
+            const int32_t* offsets, int32_t experts, uint8_t* codes,
+            int32_t* exponents, hipStream_t stream) {
   const int64_t padded = PaddedOf(dim);
   // Work-groups of 16 rows, and as many columns of blocks at once as a launch
   // takes.
@@ -393,7 +398,8 @@ int RunRows(const void* x, int64_t stride, int64_t rows, int64_t dim,
   hipLaunchKernelGGL(QuantizeRows<T>, grid, dim3(kRowThreads), 0, stream,
                      static_cast<const T*>(x), stride,
                      static_cast<int32_t>(rows), static_cast<int32_t>(dim),
-                     static_cast<int32_t>(padded), kept, codes, exponents);
+                     static_cast<int32_t>(padded), offsets, experts, codes,
+                     exponents);
   SCEMB_LAUNCH_CHECK();
   return 0;
 }
@@ -496,10 +502,10 @@ int scemb_matmul_8bit(const void* rows, int32_t type, int64_t rows_stride,
                 "bytes");
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int32_t* kept = offsets == nullptr ? nullptr : offsets + num_experts;
   const auto run = [&](auto zero) {
     using T = decltype(zero);
-    const int rc = RunRows<T>(rows, rows_stride, num_rows, inner, kept, x, e, s);
+    const int rc = RunRows<T>(rows, rows_stride, num_rows, inner, offsets,
+                              num_experts, x, e, s);
     if (rc != 0) return rc;
     const Call8<T> call = {x, e, num_rows, PaddedOf(inner), codes, exponents,
                            outer, offsets, num_experts, static_cast<T*>(y), s};

@@ -316,11 +316,12 @@ constexpr int32_t kMostHeld = kUnscaled + 119;
 
 // ---------------------------------------------------------------------------
 // Rows in segments: those of expert e are [offsets[e], offsets[e + 1]); the
-// ones behind the last belong to no expert.
+// ones behind the last and before the first belong to no expert.
 // ---------------------------------------------------------------------------
 
-// The rows of segment s, inside [0, n) whatever the offsets hold; segment
-// `experts` is the rows of none.
+// The rows of segment s, inside [0, n) whatever the offsets hold; segments
+// `experts` and `experts` + 1 are the rows of none, behind and before.
+constexpr int kNone = 2;
 struct Segment {
   int32_t begin;
   int32_t end;
@@ -328,6 +329,7 @@ struct Segment {
 __device__ __forceinline__ Segment SegmentOf(const int32_t* offsets,
                                              int32_t experts, int32_t n,
                                              int32_t s) {
+  if (s > experts) return {0, min(max(offsets[0], 0), n)};
   const int32_t begin = min(max(offsets[s], 0), n);
   const int32_t end = s < experts ? max(min(offsets[s + 1], n), begin) : n;
   return {begin, end};
@@ -355,11 +357,13 @@ __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
     if (tile >= (n + tile_rows - 1) / tile_rows) return {-1, 0, 0};
     return {0, tile * tile_rows, n};
   }
-  const int per = experts / kWave + 1;  // segments of a lane, experts + 1 in all
+  // Segments of a lane.
+  const int segments = experts + kNone;
+  const int per = (segments + kWave - 1) / kWave;
   const int first = LaneId() * per;
   int32_t count = 0;
   for (int i = 0; i < per; ++i) {
-    if (first + i <= experts) {
+    if (first + i < segments) {
       const Segment s = SegmentOf(offsets, experts, n, first + i);
       count += TilesOf(s, tile_rows);
     }
@@ -372,7 +376,7 @@ __device__ __forceinline__ RowTile FindRowTile(const int32_t* offsets,
   for (int i = who * per;; ++i) {
     const Segment s = SegmentOf(offsets, experts, n, i);
     const int32_t tiles = TilesOf(s, tile_rows);
-    if (at < tiles || i == experts) {
+    if (at < tiles || i == segments - 1) {
       // Counts of segments that overlap may wrap: no tile then.
       if (at < 0 || at >= tiles) return {-1, 0, 0};
       return {__builtin_amdgcn_readfirstlane(i),

@@ -281,7 +281,9 @@ def expert_matmul(rows, weights, order: ExpertOrder):
     dimensions may be the contiguous one (others are copied first), so weights
     stored by output are given as their transpose.
   order: sort_by_expert's; only its offsets are used, on the GPU: nothing waits
-    for the experts' numbers of rows.
+    for the experts' numbers of rows. With a part of the offsets, and of the
+    weights, it is the product of some experts: rows of the others are not read
+    and give zeros.
 
   Sums are float32, rounded once. float32 products are exact to float32's own
   rounding (no shortened operands). Calls of more than about 2^24 tiles (of 32 x
