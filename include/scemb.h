@@ -713,8 +713,8 @@ int scemb_tokens_from_experts_grad(
 /* Products of rows in the order of their experts (scemb_tokens_to_experts)
  * with each expert's weights: y[r] = rows[r] * W[e] for the rows r of expert e,
  * [offsets[e], offsets[e + 1]); zeros for rows of none (from
- * offsets[num_experts] on and before offsets[0], which are not read). Sums are float32, rounded once
- * to the type of all operands. Value (e, i, o) of W [num_experts, inner, outer]
+ * offsets[num_experts] on and before offsets[0], which are not read). Sums are
+ * float32, rounded once to the type of all operands. Value (e, i, o) of W [num_experts, inner, outer]
  * is at e * expert_stride + i * inner_stride + o * outer_stride, one of the last
  * two being 1; y is [num_rows, outer] contiguous. With inner and outer changed
  * about it is the gradient of the rows. Offsets do not fall; others reach no
